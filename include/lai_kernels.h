@@ -55,9 +55,10 @@ enum {
  * bounded wait on its own asynchronous copies ran out (never expected; the kernel
  * drains what it issued and returns instead of hanging). LAI_DEVERR_SMEM_ALIGN: a
  * tensor-core kernel found its dynamic shared memory less than 1 KiB aligned and
- * computed nothing (never expected). */
+ * computed nothing (never expected). LAI_DEVERR_PAGE: a page table entry was outside the
+ * cache's pages. */
 enum { LAI_DEVERR_TOKEN_ID = 1, LAI_DEVERR_POSITION = 2, LAI_DEVERR_TIMEOUT = 4,
-       LAI_DEVERR_SMEM_ALIGN = 8 };
+       LAI_DEVERR_SMEM_ALIGN = 8, LAI_DEVERR_PAGE = 16 };
 
 LAI_API const char *lai_status_string(int status);
 LAI_API int lai_version(void); /* major*10000 + minor*100 + patch */
@@ -312,6 +313,81 @@ LAI_API int lai_prefill_attention_rope_f32(float *out, const float *q, const flo
                                            int n_heads, int n_kv_heads, int head_dim, float scale,
                                            const float *cos_t, const float *sin_t,
                                            int64_t table_rows, lai_stream_t stream);
+
+/* ---- paged key/value cache ------------------------------------------------------------------
+ * One pool of pages holds the keys and values of many sequences, so a sequence takes memory for
+ * the tokens it has and not for max_seq of them (the reference keeps one dense F32 block per
+ * layer, src/tts_native.c:324-332). The cache of one layer:
+ *   k, v              [n_pages, n_kv_heads, page_size, head_dim] in `format`
+ *   k_scale, v_scale  [n_pages, n_kv_heads, page_size] F32; NULL for LAI_KV_BF16
+ * LAI_KV_BF16 holds rne(x). LAI_KV_E4M3 and LAI_KV_I8 hold, per token and head, the scale
+ * s = max|x| / 448 (E4M3) or / 127 (I8), 1 where that is 0, and c = rne(x / s), which stands for
+ * c * s (F32 divisions; ties to even). A row with an infinity or NaN gets scale NaN and c = 0.
+ * page_size 16, 32, 64, 128 or 256; head_dim 64 or 128; tensors 16-byte aligned.
+ *
+ * A batch is ragged. The new tokens of sequence s are rows q_start[s] .. q_start[s + 1] - 1 of the
+ * row tensors ([n_rows, heads * head_dim], row r at + r * ld elements); kv_len[s] is its key count
+ * with these tokens; new token i of n has position kv_len[s] - n + i, and position p lies in page
+ * pages[s * max_pages + p / page_size], at p % page_size. All three are int32 on the device.
+ * Rows before q_start[0] and behind q_start[n_seqs] are left as they are. A sequence whose
+ * q_start leaves [0, n_rows], or whose kv_len leaves [0, max_pages * page_size], is skipped and
+ * sets LAI_DEVERR_POSITION; so does a q_start that decreases, and then other sequences may be
+ * skipped too (nothing outside the tensors is touched).
+ */
+enum { LAI_KV_BF16 = 0, LAI_KV_E4M3 = 1, LAI_KV_I8 = 2 };
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int64_t n_pages;
+    int32_t page_size, n_kv_heads, head_dim, format;
+} lai_paged_kv_t;
+typedef struct {
+    const int32_t *q_start; /* [n_seqs + 1] */
+    const int32_t *kv_len;  /* [n_seqs] */
+    const int32_t *pages;   /* [n_seqs, max_pages] */
+    int32_t n_seqs, max_pages;
+} lai_paged_batch_t;
+
+/* lai_paged_kv_append_*: write the rows k, v [n_rows, n_kv_heads * head_dim] to their positions.
+ * lai_paged_kv_read_*: the reverse, the values the cache stands for as rows (with kv_len as the
+ * lengths of q_start's ranges: whole sequences). A row whose position is negative (more rows than
+ * keys) is left alone and sets LAI_DEVERR_POSITION; a page outside [0, n_pages)
+ * LAI_DEVERR_PAGE. Two rows of one append must not have the same page and place. */
+LAI_API int lai_paged_kv_append_bf16(const lai_paged_kv_t *kv, const lai_paged_batch_t *batch,
+                                     const lai_bf16 *k, const lai_bf16 *v, int64_t ld,
+                                     int64_t n_rows, int *err, lai_stream_t stream);
+LAI_API int lai_paged_kv_append_f32(const lai_paged_kv_t *kv, const lai_paged_batch_t *batch,
+                                    const float *k, const float *v, int64_t ld, int64_t n_rows,
+                                    int *err, lai_stream_t stream);
+LAI_API int lai_paged_kv_read_bf16(lai_bf16 *k, lai_bf16 *v, int64_t ld, int64_t n_rows,
+                                   const lai_paged_kv_t *kv, const lai_paged_batch_t *batch,
+                                   int *err, lai_stream_t stream);
+LAI_API int lai_paged_kv_read_f32(float *k, float *v, int64_t ld, int64_t n_rows,
+                                  const lai_paged_kv_t *kv, const lai_paged_batch_t *batch,
+                                  int *err, lai_stream_t stream);
+
+/* Causal attention of the batch's new tokens, whose keys and values are in the cache already:
+ * qwen_causal_attention(out, q, K, V, n, kv_len, n_heads, n_kv, hd, scale, kv_len - n) per
+ * sequence (src/tts_native.c:576-578 a prompt, :653-655 one token). A token at position p sees
+ * keys p - window + 1 .. p (window 0: 0 .. p); a row that sees none (its position is negative)
+ * becomes 0. q [n_rows, n_heads * head_dim] with row stride ld_q elements, out dense; query head h
+ * reads kv head h / (n_heads / n_kv_heads), a group of at most 16. Keys in a page outside
+ * [0, n_pages) count as not seen and set LAI_DEVERR_PAGE. What lies in the cache behind kv_len,
+ * or at positions a row does not see, does not reach that row, whatever its bits. Scores, softmax
+ * and sums are F32; with F32 q the products are exact to about F32 too (16-bit operands split
+ * into terms), with BF16 q and a BF16 cache the weights of the values may be rounded to BF16.
+ * scratch: lai_paged_attention_scratch_bytes(head_dim) bytes, zeroed once before first use; every
+ * call leaves it reusable, but two calls that may run at the same time (other streams, graphs on
+ * other streams) need one each. */
+LAI_API size_t lai_paged_attention_scratch_bytes(int head_dim);
+LAI_API int lai_paged_attention_bf16(lai_bf16 *out, const lai_bf16 *q, int64_t ld_q,
+                                     int64_t n_rows, int n_heads, const lai_paged_kv_t *kv,
+                                     const lai_paged_batch_t *batch, float scale, int window,
+                                     void *scratch, int *err, lai_stream_t stream);
+LAI_API int lai_paged_attention_f32(float *out, const float *q, int64_t ld_q, int64_t n_rows,
+                                    int n_heads, const lai_paged_kv_t *kv,
+                                    const lai_paged_batch_t *batch, float scale, int window,
+                                    void *scratch, int *err, lai_stream_t stream);
 
 /* ---- token sampling on device logits ------------------------------------------------------
  * Per row r of logits [rows, vocab]: tts_apply_repetition_penalty(logits, vocab, history,

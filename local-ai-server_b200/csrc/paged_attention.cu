@@ -1,0 +1,600 @@
+// paged_attention.cu - attention of new tokens over the paged cache: the entry points, and the
+// kernel for few query rows per sequence (decoding, drafted tokens).
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q . k_j - max)   over the keys a row sees
+//
+// (qwen_causal_attention in the reference, src/tts_native.c:576-578, 653-655.) With few rows the
+// cost is reading K and V once: HBM bound, 2 head_dim bytes per key and kv head for an 8-bit
+// cache. What stands in the way of that bound is arithmetic per key (group x 2 head_dim products,
+// and the conversion of 8-bit values), so the products go through the tensor cores with keys and
+// values straight from global memory in the operand layout of mma.m16n8k16: no shared memory, no
+// barrier in the loop, every warp with its own keys and loads in flight.
+//   * The sums over head_dim and over keys do not depend on the order of their terms. A lane
+//     takes 16-byte runs of K, and the query is loaded with the same permutation; a lane's n
+//     columns of V are a 16-byte run too, and the output is written back with that permutation.
+//   * An MMA has 16 rows and a tile has 8: rows 8-15 carry the second term of the first 8. F32
+//     queries become hi + lo in binary16 (22 bits; the 8-bit formats are exact in binary16), or
+//     three bfloat16 terms (24 bits) over a BF16 cache, and so do the weights p. With BF16
+//     queries the second rows still make the weights exact to 16 bits or more.
+//   * Each block's P V starts from zero and is added to the F32 accumulators by the FMA that
+//     rescales them, so a long sequence does not add up the MMA's truncated sums.
+//   * 8-bit: a key's scale multiplies its score, a value's scale its weight. Weights in binary16
+//     are taken relative to the largest value scale so far (a power of two per warp) and lifted
+//     by 2^13, so that small ones keep their bits.
+#include "paged_attention.cuh"
+
+namespace lai {
+
+namespace {
+
+using namespace paged;
+
+constexpr int kThreads = 128, kWarps = 4;
+constexpr int kRows = 8;      // rows of a tile
+constexpr int kCtasPerSm = 3;
+constexpr int kMaxCtas = kSMs * kCtasPerSm;
+
+template <int FMT> __host__ __device__ constexpr int step_keys() { return FMT == LAI_KV_BF16 ? 16 : 32; }  // per warp
+template <int FMT> __host__ __device__ constexpr int block_keys() { return kWarps * step_keys<FMT>(); }
+__host__ __device__ constexpr int part_floats(int hd) { return kRows * (hd + 2); }
+
+// ---- operands ----------------------------------------------------------------------------------
+template <bool F16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <bool F16> __device__ __forceinline__ float2 unpack2(uint32_t p) {
+    float2 f;
+    if (F16)
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+            : "=f"(f.x), "=f"(f.y)
+            : "r"(p));
+    else
+        f = make_float2(bf16_lo(p), bf16_hi(p));
+    return f;
+}
+// x as a 16-bit pair, x becoming what is left of it.
+template <bool F16> __device__ __forceinline__ uint32_t take2(float &x0, float &x1) {
+    const uint32_t p = pack2<F16>(x0, x1);
+    const float2 f = unpack2<F16>(p);
+    x0 -= f.x;
+    x1 -= f.y;
+    return p;
+}
+template <bool F16>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                    uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+            "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+            "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Zero an element of a pair that is an infinity or NaN; true if there was one.
+template <bool F16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &p) {
+    constexpr uint32_t kLo = F16 ? 0x7c00u : 0x7f80u, kHi = kLo << 16;
+    const bool lo = (p & kLo) == kLo, hi = (p & kHi) == kHi;
+    p &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+    return lo || hi;
+}
+
+// One stored element as F32, without its scale.
+template <int FMT> __device__ __forceinline__ float element(const unsigned char *v, int64_t i) {
+    if (FMT == LAI_KV_BF16) return to_f(reinterpret_cast<const uint16_t *>(v)[i]);
+    if (FMT == LAI_KV_I8) return (float)reinterpret_cast<const int8_t *>(v)[i];
+    return unpack2<true>(e4m3x2_to_f16x2(v[i])).x;
+}
+
+template <int HD>
+struct Smem {
+    SchedSmem sched;
+    float m[kWarps][kRows], l[kWarps][kRows];
+    float o[kWarps][kRows][HD + 4];  // rows apart by 4 banks
+    int bad, last;
+};
+
+template <int HD, int FMT, bool QF32>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) {
+    constexpr bool kF16 = FMT != LAI_KV_BF16;
+    constexpr bool kThird = QF32 && !kF16;           // a third bfloat16 term
+    constexpr int kBytes = Fmt<FMT>::kBytes;
+    constexpr int kStep = step_keys<FMT>(), U = block_keys<FMT>();
+    constexpr int NB = kStep / 8, NK = kStep / 16;   // 8-key and 16-key groups of a warp's step
+    constexpr int kChunks = HD * kBytes / 64;        // 16-byte runs of K per lane and key
+    constexpr int kPerChunk = kF16 ? 4 : 2;          // k16 steps that a run feeds
+    constexpr int KS = HD / 16;                      // k16 steps of a score
+    constexpr int ND = HD / 8;                       // 8-column groups of the output
+    constexpr int VW = HD * kBytes / 32;             // 32-bit words of V per lane and key
+    constexpr float kLift = kF16 ? 13.f : 0.f;
+    static_assert(kChunks * kPerChunk == KS, "a lane's runs cover its share of head_dim");
+
+    __shared__ Smem<HD> sm;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    pdl_wait_prior();
+    pdl_launch_dependents();
+    if (blockIdx.x == 0)
+        for (int s = threadIdx.x; s < a.kv.n_seqs; s += kThreads)
+            if (!load_seq(a.kv, s).ok) flag(a.err, LAI_DEVERR_POSITION);
+    Range w = find_range<kRows, U, kThreads>(a, sm.sched);
+    if (w.w0 >= w.w1) return;
+
+    using S = Sched<kRows, U>;
+    const int n_heads = a.kv.n_kv * a.group, in_page = a.kv.page_size() - 1;
+    int64_t pos = w.w0;
+    int slot = w.slot, seq = w.seq;
+    int64_t slot_at = w.at;
+    Tile tl = S::tile(a, slot, seq);
+    while (pos < w.w1) {
+        while (pos >= slot_at + (int64_t)tl.cost * a.kv.n_kv) {  // on to the slot that holds pos
+            slot_at += (int64_t)tl.cost * a.kv.n_kv;
+            // the lengths must not change under the kernel; if they do, it still ends
+            if (++slot >= w.n_slots) return;
+            while (seq + 1 < a.kv.n_seqs && S::base(a, seq + 1) <= slot) seq++;
+            tl = S::tile(a, slot, seq);
+        }
+        const int head = (int)((pos - slot_at) / tl.cost);
+        const int64_t item0 = slot_at + (int64_t)head * tl.cost, item1 = item0 + tl.cost;
+        const int blk0 = tl.b0 + (int)(pos - item0);
+        const int blk1 = tl.b0 + (int)(min(item1, w.w1) - item0);
+        const int first = tl.pos0 + tl.row0 / a.group;
+        const int last = tl.pos0 + (tl.row0 + tl.rows - 1) / a.group;
+
+        // the query: lane (g, t) holds row g's elements 4 at a time, hi in the MMA's row g and
+        // the rest of it in row g + 8
+        uint32_t qa[KS][kThird ? 6 : 4];
+        float row_scale = a.scale_log2;
+        const int row = tl.row0 + g, tok = row / a.group;
+        const bool row_ok = g < tl.rows;
+        const int row_pos = row_ok ? tl.pos0 + tok : -1;
+        const int row_from = a.window ? row_pos - a.window : -1;  // sees keys in (row_from, row_pos]
+        {
+            const int64_t at = ((int64_t)tl.q_row0 + tok) * a.ld_q +
+                               (int64_t)(head * a.group + (row - tok * a.group)) * HD;
+            float x[KS][4];
+            uint32_t top = 0;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const int d = (s / kPerChunk * 4 + t) * (kPerChunk * 4) + s % kPerChunk * 4;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[s][e] = 0.f;
+                if (row_ok) {
+                    if (QF32) {
+                        const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(qp) + at + d);
+                        x[s][0] = f.x; x[s][1] = f.y; x[s][2] = f.z; x[s][3] = f.w;
+                    } else {
+                        const uint2 f = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(qp) + at + d);
+                        x[s][0] = bf16_lo(f.x); x[s][1] = bf16_hi(f.x);
+                        x[s][2] = bf16_lo(f.y); x[s][3] = bf16_hi(f.y);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[s][e]) & 0x7fffffffu);
+            }
+            if (kF16) {  // the row's largest into [2^13, 2^14)
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = (int)(top >> 23) - 127;
+                const float up = pow2i(13 - e);
+                row_scale *= pow2i(e - 13);
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[s][i] *= up;
+            }
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                qa[s][0] = take2<kF16>(x[s][0], x[s][1]);
+                qa[s][2] = take2<kF16>(x[s][2], x[s][3]);
+                qa[s][1] = QF32 ? take2<kF16>(x[s][0], x[s][1]) : 0u;
+                qa[s][3] = QF32 ? take2<kF16>(x[s][2], x[s][3]) : 0u;
+                if constexpr (kThird) {
+                    qa[s][4] = pack2<false>(x[s][0], x[s][1]);
+                    qa[s][5] = pack2<false>(x[s][2], x[s][3]);
+                }
+            }
+        }
+
+        float m = neg_inf(), l = 0.f, o[ND][2];
+#pragma unroll
+        for (int n = 0; n < ND; n++) o[n][0] = o[n][1] = 0.f;
+        int vexp = -126;  // accumulators are in units of 2^vexp (8-bit)
+        bool bad = false;
+
+        for (int blk = blk0; blk < blk1; blk++) {
+            const int j0 = blk * U + warp * kStep;
+            if (j0 >= tl.k1 || j0 + kStep <= tl.k0) continue;
+            // ---- loads: this step's keys, values and scales
+            int64_t at[NK];  // cache position of each 16-key group
+            bool there[NK];
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++) {
+                const int j = j0 + 16 * kk;
+                int page = -1;
+                if (j < tl.k1) {
+                    page = __ldg(a.kv.pages + (int64_t)tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
+                    if ((page < 0 || page >= a.kv.n_pages) && lane == 0 && j + 16 > tl.k0)
+                        flag(a.err, LAI_DEVERR_PAGE);
+                }
+                there[kk] = page >= 0 && page < a.kv.n_pages;
+                at[kk] = a.kv.page_base(there[kk] ? page : 0, head) + (j & in_page);
+            }
+            uint4 kr[NB][kChunks];
+            uint32_t vr[NK][4][VW];
+            float2 ks[NB], vs[NB];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const int j = j0 + 8 * n + g;
+                const bool ok = there[n / 2] && j >= tl.k0 && j < tl.k1;
+                const unsigned char *p = a.kv.k + (at[n / 2] + 8 * (n & 1) + g) * (HD * kBytes) + 16 * t;
+#pragma unroll
+                for (int c = 0; c < kChunks; c++)
+                    kr[n][c] = ok ? ld_stream(p + 64 * c) : make_uint4(0, 0, 0, 0);
+            }
+            if (kF16) {
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    const int64_t i = at[n / 2] + 8 * (n & 1) + 2 * t;
+                    ks[n] = __ldg(reinterpret_cast<const float2 *>(a.kv.k_scale + i));
+                    vs[n] = __ldg(reinterpret_cast<const float2 *>(a.kv.v_scale + i));
+                }
+            }
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int off = 2 * t + (i & 1) + 8 * (i >> 1), j = j0 + 16 * kk + off;
+                    const bool ok = there[kk] && j >= tl.k0 && j < tl.k1;
+                    const unsigned char *p = a.kv.v + (at[kk] + off) * (HD * kBytes);
+#pragma unroll
+                    for (int c = 0; c < VW; c++) vr[kk][i][c] = 0u;
+                    if (ok) {
+                        if constexpr (VW == 2) {
+                            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p + 8 * g));
+                            vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < VW / 4; c++) {
+                                const uint4 x = ld_stream(p + 16 * g + 128 * c);
+                                vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
+                                vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
+                            }
+                        }
+                    }
+                }
+            // ---- scores
+            float sc[NB][2];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const uint4 r = kr[n][s / kPerChunk];
+                    uint32_t b0, b1;
+                    if constexpr (kF16) {
+                        const int i = s % 4;
+                        const uint32_t x = i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w;
+                        b0 = half2_of<FMT, false>(x);
+                        b1 = half2_of<FMT, true>(x);
+                    } else {
+                        b0 = s % 2 ? r.z : r.x;
+                        b1 = s % 2 ? r.w : r.y;
+                    }
+                    if constexpr (kThird) mma<kF16>(c, qa[s][4], 0u, qa[s][5], 0u, b0, b1);
+                    mma<kF16>(c, qa[s][0], qa[s][1], qa[s][2], qa[s][3], b0, b1);
+                }
+                sc[n][0] = c[0] + c[2];
+                sc[n][1] = c[1] + c[3];
+            }
+            // ---- mask, running maximum
+            float top = neg_inf();
+            uint32_t vtop = 0;
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int j = j0 + 8 * n + 2 * t + i;
+                    const bool see = j <= row_pos && j > row_from && there[n / 2];
+                    float x = sc[n][i] * row_scale;
+                    if (kF16) x *= i ? ks[n].y : ks[n].x;
+                    sc[n][i] = see ? x : neg_inf();
+                    if (kF16) {
+                        float &f = i ? vs[n].y : vs[n].x;
+                        f = see ? f : 0.f;
+                        const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
+                        vtop = max(vtop, u < 0x7f800000u ? u : 0u);
+                    }
+                    top = fmaxf(top, sc[n][i]);
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float mn = fmaxf(m, top);
+            const float mu = (mn == neg_inf() ? 0.f : mn) - kLift;
+            float alpha = ex2(m - (mu + kLift));  // m = -inf: nothing to keep
+            m = mn;
+            l *= alpha;
+            float down = 1.f;
+            if (kF16) {
+                vtop = __reduce_max_sync(0xffffffffu, vtop);
+                const int e = max(vexp, min((int)(vtop >> 23) - 127, 126));
+                alpha *= pow2i(vexp - e);
+                down = pow2i(-e);
+                vexp = e;
+            }
+            // ---- weights
+            uint32_t pa[NK][kThird ? 6 : 4];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                float p0 = ex2(sc[n][0] - mu), p1 = ex2(sc[n][1] - mu);
+                l += p0 + p1;
+                if (kF16) {  // a masked value's scale is 0 by now
+                    p0 *= vs[n].x * down;
+                    p1 *= vs[n].y * down;
+                }
+                uint32_t *pk = pa[n / 2] + (n & 1) * 2;
+                pk[0] = take2<kF16>(p0, p1);
+                pk[1] = take2<kF16>(p0, p1);
+                if constexpr (kThird) pa[n / 2][4 + (n & 1)] = pack2<false>(p0, p1);
+            }
+            // ---- values. A step whose keys some rows of the tile see and others do not gives
+            // every row 0 x v for the keys it must not see: infinities and NaN are taken out of
+            // such a step, and added to the rows that see them at the end.
+            const int jf = max(j0, tl.k0), jl = min(j0 + kStep, tl.k1) - 1;
+            const bool mixed = FMT != LAI_KV_I8 && (jl > first || (a.window && jf <= last - a.window));
+            auto column = [&](int n, uint32_t (&b0)[NK], uint32_t (&b1)[NK]) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < NK; kk++) {
+                    if (mixed) {
+                        bad |= drop_nonfinite<kF16>(b0[kk]);
+                        bad |= drop_nonfinite<kF16>(b1[kk]);
+                    }
+                    const uint32_t *pk = pa[kk];
+                    if constexpr (kThird) mma<kF16>(c, pk[4], 0u, pk[5], 0u, b0[kk], b1[kk]);
+                    mma<kF16>(c, pk[0], pk[1], pk[2], pk[3], b0[kk], b1[kk]);
+                }
+                o[n][0] = fmaf(o[n][0], alpha, c[0] + c[2]);
+                o[n][1] = fmaf(o[n][1], alpha, c[1] + c[3]);
+            };
+#pragma unroll
+            for (int wd = 0; wd < VW; wd++) {
+                uint32_t b0[NK], b1[NK];
+                if constexpr (kF16) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {  // bytes 2h, 2h + 1 of the word
+                        uint32_t x[NK], y[NK];
+#pragma unroll
+                        for (int kk = 0; kk < NK; kk++) {
+                            x[kk] = prmt(vr[kk][0][wd], vr[kk][1][wd], h ? 0x7362 : 0x5140);
+                            y[kk] = prmt(vr[kk][2][wd], vr[kk][3][wd], h ? 0x7362 : 0x5140);
+                            b0[kk] = half2_of<FMT, false>(x[kk]);
+                            b1[kk] = half2_of<FMT, false>(y[kk]);
+                        }
+                        column(4 * wd + 2 * h, b0, b1);
+#pragma unroll
+                        for (int kk = 0; kk < NK; kk++) {
+                            b0[kk] = half2_of<FMT, true>(x[kk]);
+                            b1[kk] = half2_of<FMT, true>(y[kk]);
+                        }
+                        column(4 * wd + 2 * h + 1, b0, b1);
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int kk = 0; kk < NK; kk++) {
+                            b0[kk] = prmt(vr[kk][0][wd], vr[kk][1][wd], h ? 0x7632 : 0x5410);
+                            b1[kk] = prmt(vr[kk][2][wd], vr[kk][3][wd], h ? 0x7632 : 0x5410);
+                        }
+                        column(2 * wd + h, b0, b1);
+                    }
+                }
+            }
+        }
+
+        // ---- join the warps
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        __syncthreads();  // the shared memory of the item before is read
+        if (threadIdx.x == 0) sm.bad = 0;
+        if (t == 0) {
+            sm.m[warp][g] = m;
+            sm.l[warp][g] = l;
+        }
+        {
+            const float unit = kF16 ? pow2i(vexp) : 1.f;
+#pragma unroll
+            for (int n = 0; n < ND; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    // column 2t + i of group n: the lane that holds it took its V from the run
+                    // of lanes with g = 2t + i
+                    const int gg = 2 * t + i;
+                    int d;
+                    if constexpr (VW == 2) d = gg * 8 + n;
+                    else if constexpr (kF16) d = gg * 16 + n;
+                    else d = (gg + 8 * (n / 8)) * 8 + n % 8;
+                    sm.o[warp][g][d] = o[n][i] * unit;
+                }
+        }
+        __syncthreads();
+        if (FMT != LAI_KV_I8) {
+            if (bad) sm.bad = 1;
+            __syncthreads();
+        }
+        constexpr int kPer = kRows * HD / kThreads;
+        float acc[kPer], jm[kPer], jl_[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
+            float mx = sm.m[0][r];
+#pragma unroll
+            for (int x = 1; x < kWarps; x++) mx = fmaxf(mx, sm.m[x][r]);
+            const float mu = mx == neg_inf() ? 0.f : mx;
+            float sum = 0.f, v = 0.f;
+#pragma unroll
+            for (int x = 0; x < kWarps; x++) {
+                const float c = ex2(sm.m[x][r] - mu);
+                sum = fmaf(sm.l[x][r], c, sum);
+                v = fmaf(sm.o[x][r][d], c, v);
+            }
+            acc[i] = v;
+            jm[i] = mx;
+            jl_[i] = sum;
+        }
+        if (FMT != LAI_KV_I8 && sm.bad) {
+            for (int j = max(blk0 * U, tl.k0); j < min(blk1 * U, tl.k1); j++) {
+                const int j0 = j / kStep * kStep;
+                const int jf = max(j0, tl.k0), jl = min(j0 + kStep, tl.k1) - 1;
+                if (!(jl > first || (a.window && jf <= last - a.window))) continue;
+                const int page = __ldg(a.kv.pages + (int64_t)tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
+                if (page < 0 || page >= a.kv.n_pages) continue;
+                const int64_t at = (a.kv.page_base(page, head) + (j & in_page)) * HD;
+#pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
+                    const int p = tl.pos0 + (tl.row0 + r) / a.group;
+                    if (r >= tl.rows || j > p || (a.window && j <= p - a.window)) continue;
+                    const float v = element<FMT>(a.kv.v, at + d);
+                    if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) acc[i] += v;
+                }
+            }
+        }
+        bool write = pos == item0 && item1 <= w.w1;
+        if (!write) {
+            const int64_t slot_no = (int64_t)blockIdx.x * 2 + (pos == item0 ? 1 : 0);
+            float *pp = a.parts + slot_no * part_floats(HD);
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
+                if (d == 0) {
+                    pp[r] = jm[i];
+                    pp[kRows + r] = jl_[i];
+                }
+                pp[2 * kRows + e] = acc[i];
+            }
+            __threadfence();
+            __syncthreads();
+            const int c0 = cta_of(w, item0), c1 = cta_of(w, item1 - 1);
+            if (threadIdx.x == 0) sm.last = atomicAdd(a.counters + c0, 1) == c1 - c0;
+            __syncthreads();
+            write = sm.last;
+            if (write) {
+                __threadfence();
+                if (threadIdx.x == 0) a.counters[c0] = 0;  // ready for the next call
+#pragma unroll
+                for (int i = 0; i < kPer; i++) acc[i] = jl_[i] = 0.f, jm[i] = neg_inf();
+                for (int c = c0; c <= c1; c++) {
+                    const float *pc = a.parts + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * part_floats(HD);
+#pragma unroll
+                    for (int i = 0; i < kPer; i++) {
+                        const int e = threadIdx.x + i * kThreads, r = e / HD;
+                        const float cm = __ldcg(pc + r), mx = fmaxf(jm[i], cm);
+                        const float mu = mx == neg_inf() ? 0.f : mx;
+                        const float ca = ex2(jm[i] - mu), cb = ex2(cm - mu);
+                        jl_[i] = fmaf(__ldcg(pc + kRows + r), cb, jl_[i] * ca);
+                        acc[i] = fmaf(__ldcg(pc + 2 * kRows + e), cb, acc[i] * ca);
+                        jm[i] = mx;
+                    }
+                }
+            }
+        }
+        if (write) {
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
+                if (r >= tl.rows) continue;
+                const int fr = tl.row0 + r, tk = fr / a.group;
+                const int64_t at = (((int64_t)tl.q_row0 + tk) * n_heads + head * a.group +
+                                    (fr - tk * a.group)) * HD + d;
+                const float x = jl_[i] == 0.f ? 0.f : acc[i] / jl_[i];
+                if (QF32) static_cast<float *>(out)[at] = x;
+                else static_cast<uint16_t *>(out)[at] = from_f<uint16_t>(x);
+            }
+        }
+        pos = min(item1, w.w1);
+    }
+}
+
+template <int HD, int FMT, bool QF32>
+void launch_few(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
+    constexpr int U = block_keys<FMT>();
+    const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.log_page) + U - 1) / U;
+    const int64_t most = Sched<kRows, U>::slots(a.kv.n_rows, a.group, a.kv.n_seqs) * a.kv.n_kv;
+    const int64_t ctas = most < kMaxCtas ? most * blocks : kMaxCtas;  // most * blocks fits
+    launch_pdl(paged_attn_few_kernel<HD, FMT, QF32>,
+               dim3((unsigned)(ctas < kMaxCtas ? ctas : kMaxCtas)), dim3(kThreads), 0, st, out, q, a);
+}
+
+template <bool QF32>
+int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int n_heads,
+                    const lai_paged_kv_t *kv, const lai_paged_batch_t *b, float scale, int window,
+                    void *scratch, int *err, lai_stream_t stream) {
+    AttnArgs a;
+    const int st = check(kv, b, n_rows, &a.kv);
+    if (st != LAI_OK) return st;
+    constexpr int kEsize = QF32 ? 4 : 2;
+    if (!out || !q || !scratch || n_heads <= 0 || window < 0 || n_heads % kv->n_kv_heads != 0 ||
+        n_heads / kv->n_kv_heads > 16)
+        return LAI_ERR_INVALID;
+    const int64_t width = (int64_t)n_heads * kv->head_dim;
+    if (ld_q < width || ld_q % (16 / kEsize) != 0 || !aligned16(q) || !aligned16(out) ||
+        !aligned16(scratch))
+        return LAI_ERR_INVALID;
+    if (n_rows == 0 || b->n_seqs == 0) return LAI_OK;
+    if (n_rows * (n_heads / kv->n_kv_heads) + b->n_seqs > INT32_MAX / 2) return LAI_ERR_RANGE;
+    const size_t ob = paged::row_bytes(n_rows, width, width, kEsize);
+    const size_t qb = paged::row_bytes(n_rows, ld_q, width, kEsize);
+    const size_t wb = lai_paged_attention_scratch_bytes(kv->head_dim);
+    if (overlaps(out, ob, q, qb) || hits_cache(kv, out, ob) || hits_cache(kv, scratch, wb) ||
+        overlaps(scratch, wb, out, ob) || overlaps(scratch, wb, q, qb))
+        return LAI_ERR_ALIAS;
+    a.group = n_heads / kv->n_kv_heads;
+    a.window = window < (1 << 30) ? window : 0;  // positions are below 2^31: it masks nothing
+    a.scale_log2 = scale * kLog2e;
+    a.ld_q = ld_q;
+    a.counters = static_cast<int *>(scratch);
+    a.parts = reinterpret_cast<float *>(a.counters + 1024);
+    a.err = err;
+    const cudaStream_t cs = as_stream(stream);
+#define LAI_FEW(FMT)                                                      \
+    if (kv->head_dim == 128) launch_few<128, FMT, QF32>(out, q, a, cs);   \
+    else launch_few<64, FMT, QF32>(out, q, a, cs)
+    switch (kv->format) {
+        case LAI_KV_BF16: LAI_FEW(LAI_KV_BF16); break;
+        case LAI_KV_E4M3: LAI_FEW(LAI_KV_E4M3); break;
+        default: LAI_FEW(LAI_KV_I8); break;
+    }
+#undef LAI_FEW
+    return launch_status();
+}
+
+}  // namespace
+}  // namespace lai
+
+extern "C" size_t lai_paged_attention_scratch_bytes(int head_dim) {
+    if (head_dim != 64 && head_dim != 128) return 0;
+    return 1024 * sizeof(int) + (size_t)lai::kMaxCtas * 2 * lai::part_floats(head_dim) * sizeof(float);
+}
+extern "C" int lai_paged_attention_bf16(lai_bf16 *out, const lai_bf16 *q, int64_t ld_q,
+                                        int64_t n_rows, int n_heads, const lai_paged_kv_t *kv,
+                                        const lai_paged_batch_t *batch, float scale, int window,
+                                        void *scratch, int *err, lai_stream_t stream) {
+    return lai::attention_entry<false>(out, q, ld_q, n_rows, n_heads, kv, batch, scale, window,
+                                       scratch, err, stream);
+}
+extern "C" int lai_paged_attention_f32(float *out, const float *q, int64_t ld_q, int64_t n_rows,
+                                       int n_heads, const lai_paged_kv_t *kv,
+                                       const lai_paged_batch_t *batch, float scale, int window,
+                                       void *scratch, int *err, lai_stream_t stream) {
+    return lai::attention_entry<true>(out, q, ld_q, n_rows, n_heads, kv, batch, scale, window,
+                                      scratch, err, stream);
+}

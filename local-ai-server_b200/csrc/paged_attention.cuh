@@ -1,0 +1,177 @@
+// paged_attention.cuh - how the paged attention kernels divide their work, and join it again.
+//
+// An item is a tile of up to R query rows (row = new token * group + head of the group) of one
+// sequence and one kv head; its cost is the number of U-key blocks that its rows see. All items
+// laid end to end are W blocks, and CTA c of N takes blocks [c W / N, (c + 1) W / N): every CTA
+// reads the same number of keys however long, short or few the sequences are, and nothing has to
+// be known on the host (the lengths live on the device, so a captured graph follows them). An item
+// that lies in one CTA is written by it. An item cut by a CTA's border leaves (max, sum,
+// accumulator) per row in the scratch, and the CTA that arrives last (a counter at the item's
+// first CTA) joins the parts in their order, so the result does not depend on who was last. A CTA
+// has at most two cut items: the one it starts with and the one it ends with.
+#pragma once
+
+#include "paged.cuh"
+
+namespace lai {
+namespace paged {
+
+constexpr int kSMs = 148;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^e for any e, held within the normal range.
+__device__ __forceinline__ float pow2i(int e) {
+    return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
+}
+
+struct AttnArgs {
+    View kv;
+    int group;      // query heads per kv head
+    int window;     // 0: every earlier key
+    float scale_log2;
+    int64_t ld_q;
+    int *counters;  // one per CTA of the grid, 0 between calls
+    float *parts;   // two cut items per CTA
+    int *err;
+};
+
+// An item without its kv head.
+struct Tile {
+    int seq, row0, q_row0;  // sequence, first flattened row in it, the sequence's first row
+    int rows;               // real rows, 0: no item
+    int pos0;               // position of new token 0
+    int k0, k1;             // keys any row sees
+    int b0, cost;           // first block, blocks (1 for a tile that sees no key)
+};
+
+template <int R, int U>
+struct Sched {
+    // Slots of tiles: sequence s has those from q_start[s] * group / R + s on, at least as many as
+    // it has tiles.
+    static __host__ __device__ int64_t slots(int64_t n_rows, int group, int n_seqs) {
+        return n_rows * group / R + n_seqs;
+    }
+    static __device__ __forceinline__ int base(const AttnArgs &a, int s) {
+        return (int)((int64_t)__ldg(a.kv.q_start + s) * a.group / R) + s;
+    }
+    // The last sequence whose slots start at or before `slot` (0 if none does).
+    static __device__ __forceinline__ int seq_of(const AttnArgs &a, int slot) {
+        int lo = 0, hi = a.kv.n_seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (base(a, mid) <= slot) lo = mid; else hi = mid;
+        }
+        return lo;
+    }
+    static __device__ __forceinline__ Tile tile(const AttnArgs &a, int slot, int s) {
+        Tile t = {};
+        const Seq q = load_seq(a.kv, s);
+        const int i = slot - base(a, s);
+        const int64_t r0 = (int64_t)i * R, all = (int64_t)q.n * a.group;
+        if (!q.ok || i < 0 || r0 >= all) return t;
+        t.seq = s;
+        t.row0 = (int)r0;
+        t.q_row0 = q.row0;
+        t.rows = (int)min((int64_t)R, all - r0);
+        t.pos0 = q.len - q.n;
+        const int first = t.pos0 + t.row0 / a.group;
+        const int last = t.pos0 + (t.row0 + t.rows - 1) / a.group;
+        t.k1 = max(last + 1, 0);
+        t.k0 = a.window ? max(first - a.window + 1, 0) : 0;
+        t.b0 = t.k0 / U;
+        t.cost = t.k1 > t.k0 ? (t.k1 + U - 1) / U - t.b0 : 1;
+        return t;
+    }
+};
+
+// Where a CTA starts, and how far it goes. Positions are in blocks of the whole work.
+struct Range {
+    int64_t total, w0, w1;  // all blocks; this CTA's
+    int64_t at;             // position of slot's first block
+    int slot, seq;
+    int ctas;               // CTAs that have work
+    int n_slots;
+};
+
+struct SchedSmem {
+    int64_t sums[32];
+    int64_t at;
+    int slot, seq;
+};
+
+template <int R, int U, int THREADS>
+__device__ __forceinline__ Range find_range(const AttnArgs &a, SchedSmem &sm) {
+    using S = Sched<R, U>;
+    const int n_slots = (int)S::slots(a.kv.n_rows, a.group, a.kv.n_seqs);
+    const int per = (n_slots + THREADS - 1) / THREADS;
+    const int s0 = min((int)threadIdx.x * per, n_slots), s1 = min(s0 + per, n_slots);
+    int64_t mine = 0;
+    int first_seq = 0;
+    if (s0 < s1) {
+        int s = first_seq = S::seq_of(a, s0);
+        for (int slot = s0; slot < s1; slot++) {
+            while (s + 1 < a.kv.n_seqs && S::base(a, s + 1) <= slot) s++;
+            mine += S::tile(a, slot, s).cost;
+        }
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) sm.sums[warp] = upto;
+    if (threadIdx.x == 0) sm.slot = n_slots;
+    __syncthreads();
+    int64_t total = 0, before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) {
+        if (w < warp) before += sm.sums[w];
+        total += sm.sums[w];
+    }
+    Range r;
+    r.total = total * a.kv.n_kv;
+    r.ctas = (int)min((int64_t)gridDim.x, r.total);
+    r.w0 = r.w1 = r.at = 0;
+    r.slot = r.seq = 0;
+    r.n_slots = n_slots;
+    if ((int)blockIdx.x >= r.ctas) return r;  // the whole CTA
+    r.w0 = r.total * blockIdx.x / r.ctas;
+    r.w1 = r.total * (blockIdx.x + 1) / r.ctas;
+    const int64_t nk = a.kv.n_kv;
+    if (before * nk <= r.w0 && r.w0 < (before + mine) * nk) {  // one thread's slots hold w0
+        int s = first_seq;
+        int64_t at = before;
+        for (int slot = s0; slot < s1; slot++) {
+            while (s + 1 < a.kv.n_seqs && S::base(a, s + 1) <= slot) s++;
+            const int c = S::tile(a, slot, s).cost;
+            if (r.w0 < (at + c) * nk) {
+                sm.slot = slot;
+                sm.seq = s;
+                sm.at = at * nk;
+                break;
+            }
+            at += c;
+        }
+    }
+    __syncthreads();
+    r.slot = sm.slot;
+    r.seq = sm.seq;
+    r.at = sm.at;
+    return r;
+}
+
+// The CTA that takes block x.
+__device__ __forceinline__ int cta_of(const Range &r, int64_t x) {
+    return (int)(((x + 1) * r.ctas - 1) / r.total);
+}
+
+}  // namespace paged
+}  // namespace lai

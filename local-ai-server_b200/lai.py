@@ -18,6 +18,8 @@ LIB_PATH = os.path.join(HERE, "liblai_kernels.so")
 LAI_OK, LAI_ERR_INVALID, LAI_ERR_CUDA, LAI_ERR_RANGE, LAI_ERR_ALIAS, LAI_ERR_NOMEM, LAI_ERR_TOOBIG = \
     0, -1, -2, -3, -4, -5, -6
 LAI_DEVERR_TOKEN_ID, LAI_DEVERR_POSITION, LAI_DEVERR_TIMEOUT, LAI_DEVERR_SMEM_ALIGN = 1, 2, 4, 8
+LAI_DEVERR_PAGE = 16
+LAI_KV_BF16, LAI_KV_E4M3, LAI_KV_I8 = 0, 1, 2
 
 _vp, _i32, _i64, _f32, _u64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_uint64
 
@@ -75,6 +77,15 @@ SIGNATURES: dict[str, tuple] = {
     "lai_decode_attention_qk_f32": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32,
                                            _i32, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _f32,
                                            _vp, _vp, _vp]),
+    "lai_paged_kv_append_bf16": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "lai_paged_kv_append_f32": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "lai_paged_kv_read_bf16": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "lai_paged_kv_read_f32": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "lai_paged_attention_scratch_bytes": (ctypes.c_size_t, [_i32]),
+    "lai_paged_attention_bf16": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _f32, _i32, _vp,
+                                        _vp, _vp]),
+    "lai_paged_attention_f32": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _f32, _i32, _vp,
+                                       _vp, _vp]),
     "lai_sample_topk_f32": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _i32, _f32, _f32, _i32, _vp,
                                    _vp]),
     "lai_voc_bigvgan_block_f32": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp,
@@ -409,6 +420,184 @@ def prefill_attention_rope(qkv, n_heads, n_kv_heads, head_dim, cos_t, sin_t, sca
     call("lai_prefill_attention_rope_f32", _p(out), base, base + 4 * qd, base + 4 * (qd + kvd), ld,
          ld, T, n_heads, n_kv_heads, head_dim, head_dim ** -0.5 if scale is None else scale,
          _p(cos_t), _p(sin_t), 0 if cos_t is None else cos_t.shape[0], _s(stream))
+    return out
+
+
+class _PagedKVC(ctypes.Structure):
+    """lai_paged_kv_t."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("n_pages", _i64),
+                ("page_size", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("format", ctypes.c_int32)]
+
+
+class _PagedBatchC(ctypes.Structure):
+    """lai_paged_batch_t."""
+    _fields_ = [("q_start", _vp), ("kv_len", _vp), ("pages", _vp), ("n_seqs", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32)]
+
+
+def _need_cuda(*tensors):
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and (t.device.type != "cuda" or t.device != dev):
+            raise ValueError("paged cache, batch and rows must be CUDA tensors of one device")
+
+
+class PagedKV:
+    """One layer's paged key/value cache (lai_paged_kv_t): k, v [n_pages, n_kv_heads, page_size,
+    head_dim] in torch.bfloat16, or in torch.float8_e4m3fn or torch.int8 with k_scale, v_scale
+    [n_pages, n_kv_heads, page_size] F32. The tensors are written in place and kept alive."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        import torch
+        fmt = {torch.bfloat16: LAI_KV_BF16, torch.float8_e4m3fn: LAI_KV_E4M3,
+               torch.int8: LAI_KV_I8}.get(k.dtype)
+        if fmt is None or v.dtype != k.dtype:
+            raise TypeError(f"unsupported cache dtypes {k.dtype}, {v.dtype}")
+        if k.dim() != 4 or v.shape != k.shape or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("k and v must be contiguous [n_pages, n_kv_heads, page_size, head_dim]")
+        scales = (k_scale, v_scale)
+        if (fmt != LAI_KV_BF16) != all(s is not None for s in scales) or \
+                (fmt == LAI_KV_BF16 and any(s is not None for s in scales)):
+            raise ValueError("8-bit caches need k_scale and v_scale (and only they take them)")
+        for s in scales:
+            if s is not None and (s.dtype != torch.float32 or s.shape != k.shape[:3]
+                                  or not s.is_contiguous()):
+                raise ValueError("scales must be contiguous F32 [n_pages, n_kv_heads, page_size]")
+        if k.shape[2] not in (16, 32, 64, 128, 256) or k.shape[3] not in (64, 128):
+            raise ValueError("page_size must be 16, 32, 64, 128 or 256 and head_dim 64 or 128")
+        _need_cuda(k, v, k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self.device = k.device
+        self._c = _PagedKVC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if fmt else None,
+                            v_scale.data_ptr() if fmt else None, *(k.shape[0], k.shape[2]),
+                            k.shape[1], k.shape[3], fmt)
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def allocate(cls, n_pages, n_kv_heads, page_size, head_dim, dtype, device="cuda"):
+        """An empty (zeroed) cache of `dtype`, its scales 1."""
+        import torch
+        k, v = (torch.zeros((n_pages, n_kv_heads, page_size, head_dim), dtype=torch.uint8 if
+                            dtype != torch.bfloat16 else dtype, device=device).view(dtype)
+                for _ in range(2))
+        if dtype == torch.bfloat16:
+            return cls(k, v)
+        return cls(k, v, *(torch.ones(k.shape[:3], device=device) for _ in range(2)))
+
+
+class PagedBatch:
+    """A ragged batch over a paged cache (lai_paged_batch_t), int32 CUDA tensors: sequence s's new
+    tokens are rows q_start[s] .. q_start[s + 1] - 1, kv_len[s] counts its keys with them, and
+    pages[s, j] holds its positions j * page_size ... The tensors may change between calls."""
+
+    def __init__(self, q_start, kv_len, pages):
+        import torch
+        for t in (q_start, kv_len, pages):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError("q_start, kv_len and pages must be contiguous int32")
+        if q_start.dim() != 1 or kv_len.dim() != 1 or pages.dim() != 2 or \
+                q_start.shape[0] != kv_len.shape[0] + 1 or pages.shape[0] != kv_len.shape[0]:
+            raise ValueError("a batch is q_start [n + 1], kv_len [n], pages [n, max_pages]")
+        _need_cuda(q_start, kv_len, pages)
+        self.q_start, self.kv_len, self.pages = q_start, kv_len, pages
+        self.device = q_start.device
+        self._c = _PagedBatchC(q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(),
+                               *pages.shape)
+        self._ref = ctypes.byref(self._c)
+
+
+def _paged_rows(t, width):
+    """Row stride of a [rows, width] tensor whose rows are dense (a column block will do)."""
+    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and t.shape[1] != 1):
+        raise ValueError(f"rows must be [n, {width}] with adjacent elements")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+def _paged_call(fn, device, args, stream):
+    """Launch on `stream`, or on the current stream of the tensors' device."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return call(fn, *args, _s(stream))
+    with torch.cuda.device(device):
+        return call(fn, *args, _s(stream))
+
+
+def _paged_dtype(t):
+    import torch
+    if t == torch.float32:
+        return "f32"
+    if t == torch.bfloat16:
+        return "bf16"
+    raise TypeError(f"rows must be float32 or bfloat16, not {t}")
+
+
+def paged_kv_append(kv, batch, k, v, err=None, stream=None):
+    """Write the new tokens' rows k, v [rows, n_kv_heads * head_dim] (F32 or BF16; column blocks
+    of one tensor will do) to their positions in the cache, quantising them if it is an 8-bit one."""
+    if v.dtype != k.dtype or v.shape != k.shape:
+        raise ValueError("k and v must have the same shape and dtype")
+    suffix = _paged_dtype(k.dtype)
+    ld = _paged_rows(k, kv.n_kv_heads * kv.head_dim)
+    if _paged_rows(v, kv.n_kv_heads * kv.head_dim) != ld:
+        raise ValueError("k and v must have the same row stride")
+    _need_cuda(kv.k, batch.q_start, k, v, err)
+    _paged_call("lai_paged_kv_append_" + suffix, kv.device,
+                (kv._ref, batch._ref, k.data_ptr(), v.data_ptr(), ld, k.shape[0], _p(err)), stream)
+
+
+def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None):
+    """The reverse of paged_kv_append: (k, v) [rows, n_kv_heads * head_dim], the values the cache
+    stands for at the positions of the batch's rows. With kv_len as the lengths of q_start's
+    ranges these are whole sequences."""
+    import torch
+    suffix, width = _paged_dtype(dtype), kv.n_kv_heads * kv.head_dim
+    k = torch.empty((rows, width), dtype=dtype, device=kv.device) if k is None else k
+    v = torch.empty((rows, width), dtype=dtype, device=kv.device) if v is None else v
+    if k.dtype != dtype or v.dtype != dtype or k.shape[0] != rows or v.shape[0] != rows:
+        raise ValueError("k and v must be [rows, n_kv_heads * head_dim] of dtype")
+    ld = _paged_rows(k, width)
+    if _paged_rows(v, width) != ld:
+        raise ValueError("k and v must have the same row stride")
+    _need_cuda(kv.k, batch.q_start, k, v, err)
+    _paged_call("lai_paged_kv_read_" + suffix, kv.device,
+                (k.data_ptr(), v.data_ptr(), ld, rows, kv._ref, batch._ref, _p(err)), stream)
+    return k, v
+
+
+def paged_attention_scratch(head_dim=128, device="cuda"):
+    """Zeroed scratch for paged_attention, of one size for every batch. It serves any number of
+    calls one after another; calls that may run at the same time need one each."""
+    import torch
+    nb = load().lai_paged_attention_scratch_bytes(head_dim)
+    return torch.zeros(nb // 4, dtype=torch.float32, device=device)
+
+
+def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, err=None,
+                    stream=None):
+    """Causal attention of the batch's new tokens q [rows, n_heads * head_dim] (F32 or BF16, any
+    row stride) over the paged cache, which holds their own keys and values already. window: a
+    token sees the last `window` keys up to itself (0: all). Returns out [rows, n_heads * head_dim]
+    (rows that belong to no sequence are not written)."""
+    import torch
+    suffix, hd = _paged_dtype(q.dtype), kv.head_dim
+    if q.dim() != 2 or q.shape[1] % (hd * kv.n_kv_heads):
+        raise ValueError("q must be [rows, n_heads * head_dim], n_heads a multiple of n_kv_heads")
+    ld = _paged_rows(q, q.shape[1])
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape and dtype")
+    if scratch is None:
+        scratch = paged_attention_scratch(hd, kv.device)
+    elif scratch.numel() * scratch.element_size() < load().lai_paged_attention_scratch_bytes(hd):
+        raise ValueError("scratch is too small: use paged_attention_scratch(head_dim)")
+    _need_cuda(kv.k, batch.q_start, q, out, scratch, err)
+    _paged_call("lai_paged_attention_" + suffix, kv.device,
+                (out.data_ptr(), q.data_ptr(), ld, q.shape[0], q.shape[1] // hd, kv._ref,
+                 batch._ref, hd ** -0.5 if scale is None else scale, window, scratch.data_ptr(),
+                 _p(err)), stream)
     return out
 
 

@@ -33,6 +33,8 @@ constexpr int kThreads = 128, kWarps = 4;
 constexpr int kRows = 8;      // rows of a tile
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxCtas = kSMs * kCtasPerSm;
+constexpr int kCounters = 1024;  // ints at the front of the scratch
+constexpr int kWideRows = 32;    // more rows per sequence (on average) go to the wide kernel
 
 template <int FMT> __host__ __device__ constexpr int step_keys() { return FMT == LAI_KV_BF16 ? 16 : 32; }  // per warp
 template <int FMT> __host__ __device__ constexpr int block_keys() { return kWarps * step_keys<FMT>(); }
@@ -562,9 +564,11 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
     a.scale_log2 = scale * kLog2e;
     a.ld_q = ld_q;
     a.counters = static_cast<int *>(scratch);
-    a.parts = reinterpret_cast<float *>(a.counters + 1024);
+    a.parts = reinterpret_cast<float *>(a.counters + kCounters);
     a.err = err;
     const cudaStream_t cs = as_stream(stream);
+    if (n_rows * a.group > (int64_t)kWideRows * b->n_seqs && a.scale_log2 >= 0.f)
+        return attention_wide(out, q, QF32, kv->head_dim, kv->format, a, cs);
 #define LAI_FEW(FMT)                                                      \
     if (kv->head_dim == 128) launch_few<128, FMT, QF32>(out, q, a, cs);   \
     else launch_few<64, FMT, QF32>(out, q, a, cs)
@@ -582,7 +586,9 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
 
 extern "C" size_t lai_paged_attention_scratch_bytes(int head_dim) {
     if (head_dim != 64 && head_dim != 128) return 0;
-    return 1024 * sizeof(int) + (size_t)lai::kMaxCtas * 2 * lai::part_floats(head_dim) * sizeof(float);
+    const size_t few = (size_t)lai::kMaxCtas * 2 * lai::part_floats(head_dim);
+    const size_t wide = lai::paged::wide_scratch_floats(head_dim);
+    return lai::kCounters * sizeof(int) + (few > wide ? few : wide) * sizeof(float);
 }
 extern "C" int lai_paged_attention_bf16(lai_bf16 *out, const lai_bf16 *q, int64_t ld_q,
                                         int64_t n_rows, int n_heads, const lai_paged_kv_t *kv,

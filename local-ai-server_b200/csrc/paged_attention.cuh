@@ -173,5 +173,11 @@ __device__ __forceinline__ int cta_of(const Range &r, int64_t x) {
     return (int)(((x + 1) * r.ctas - 1) / r.total);
 }
 
+// The kernel for many rows per sequence (paged_attention_wide.cu), scale_log2 >= 0: LAI_OK or an
+// error; and the F32 values of scratch it needs.
+int attention_wide(void *out, const void *q, bool f32, int head_dim, int format, const AttnArgs &a,
+                   cudaStream_t st);
+size_t wide_scratch_floats(int head_dim);
+
 }  // namespace paged
 }  // namespace lai

@@ -200,3 +200,31 @@ def test_attention_heads_and_pages(H, Hkv, hd, page, cache, dtype):
 @pytest.mark.parametrize("cache,dtype", [("bf16", "bf16"), ("i8", "f32"), ("e4m3", "f32")])
 def test_attention_window(window, cache, dtype):
     Case([1, 9, 60, 1], [1000, 300, 60, 4], 8, 4, 64, cache, 32, dtype, seed=window % 97).check(window=window)
+
+
+# many rows: one tile and its edges, blocks of 128 keys and theirs, several tiles, a long prefix,
+# long and short sequences in one batch, a sequence cut over many CTAs
+WIDE = [([64, 65, 63], [64, 200, 129]), ([128], [128]), ([129, 200], [1000, 257]), ([700], [700]),
+        ([300, 1, 40], [4000, 777, 40]), ([100], [20000])]
+
+
+@pytest.mark.parametrize("new,keys", WIDE)
+@pytest.mark.parametrize("cache", list(ref.FORMATS))
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+def test_attention_wide(new, keys, cache, dtype):
+    Case(new, keys, 8, 4, 128, cache, 32, dtype, seed=len(new) + keys[0]).check()
+
+
+@pytest.mark.parametrize("H,Hkv,hd,page", [(4, 4, 64, 16), (6, 2, 64, 32), (8, 1, 128, 64),
+                                           (3, 1, 128, 128), (16, 1, 64, 256), (2, 2, 128, 16)])
+@pytest.mark.parametrize("cache", list(ref.FORMATS))
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+def test_attention_wide_heads_and_pages(H, Hkv, hd, page, cache, dtype):
+    Case([150, 90], [333, 90], H, Hkv, hd, cache, page, dtype, seed=H).check()
+
+
+@pytest.mark.parametrize("window", [1, 37, 128, 300, 100000])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cache,dtype", [("bf16", "bf16"), ("i8", "f32"), ("e4m3", "bf16"), ("bf16", "f32")])
+def test_attention_wide_window(window, hd, cache, dtype):
+    Case([200, 400], [1000, 400], 4, 2, hd, cache, 16, dtype, seed=window % 89).check(window=window)

@@ -94,6 +94,10 @@ template <int FMT> __device__ __forceinline__ float element(const unsigned char 
     return unpack2<true>(e4m3x2_to_f16x2(v[i])).x;
 }
 
+// Extra cost of an item in blocks: none. (Its queries, join and output cost about as much as a
+// block of 64 keys, but with 3 CTAs on an SM they run beside the loads of the others.)
+template <int FMT> using FewSched = Sched<kRows, block_keys<FMT>(), 0>;
+
 template <int HD>
 struct Smem {
     SchedSmem sched;
@@ -126,29 +130,15 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     if (blockIdx.x == 0)
         for (int s = threadIdx.x; s < a.kv.n_seqs; s += kThreads)
             if (!load_seq(a.kv, s).ok) flag(a.err, LAI_DEVERR_POSITION);
-    Range w = find_range<kRows, U, kThreads>(a, sm.sched);
-    if (w.w0 >= w.w1) return;
+    const Range range = find_range<FewSched<FMT>, kThreads>(a, sm.sched);
+    if (range.w0 >= range.w1) return;
 
-    using S = Sched<kRows, U>;
     const int n_heads = a.kv.n_kv * a.group, in_page = a.kv.page_size() - 1;
-    int64_t pos = w.w0;
-    int slot = w.slot, seq = w.seq;
-    int64_t slot_at = w.at;
-    Tile tl = S::tile(a, slot, seq);
-    while (pos < w.w1) {
-        while (pos >= slot_at + (int64_t)tl.cost * a.kv.n_kv) {  // on to the slot that holds pos
-            slot_at += (int64_t)tl.cost * a.kv.n_kv;
-            // the lengths must not change under the kernel; if they do, it still ends
-            if (++slot >= w.n_slots) return;
-            while (seq + 1 < a.kv.n_seqs && S::base(a, seq + 1) <= slot) seq++;
-            tl = S::tile(a, slot, seq);
-        }
-        const int head = (int)((pos - slot_at) / tl.cost);
-        const int64_t item0 = slot_at + (int64_t)head * tl.cost, item1 = item0 + tl.cost;
-        const int blk0 = tl.b0 + (int)(pos - item0);
-        const int blk1 = tl.b0 + (int)(min(item1, w.w1) - item0);
-        const int first = tl.pos0 + tl.row0 / a.group;
-        const int last = tl.pos0 + (tl.row0 + tl.rows - 1) / a.group;
+    Walk<FewSched<FMT>> it;
+    it.start(a, range);
+    while (it.next(a)) {
+        const Tile &tl = it.tl;
+        const int head = it.head, blk0 = it.blk0, blk1 = it.blk1;
 
         // the query: lane (g, t) holds row g's elements 4 at a time, hi in the MMA's row g and
         // the rest of it in row g + 8
@@ -349,8 +339,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             // ---- values. A step whose keys some rows of the tile see and others do not gives
             // every row 0 x v for the keys it must not see: infinities and NaN are taken out of
             // such a step, and added to the rows that see them at the end.
-            const int jf = max(j0, tl.k0), jl = min(j0 + kStep, tl.k1) - 1;
-            const bool mixed = FMT != LAI_KV_I8 && (jl > first || (a.window && jf <= last - a.window));
+            const bool mixed = FMT != LAI_KV_I8 && it.mixed(a, j0, kStep);
             auto column = [&](int n, uint32_t (&b0)[NK], uint32_t (&b1)[NK]) {
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -454,9 +443,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         }
         if (FMT != LAI_KV_I8 && sm.bad) {
             for (int j = max(blk0 * U, tl.k0); j < min(blk1 * U, tl.k1); j++) {
-                const int j0 = j / kStep * kStep;
-                const int jf = max(j0, tl.k0), jl = min(j0 + kStep, tl.k1) - 1;
-                if (!(jl > first || (a.window && jf <= last - a.window))) continue;
+                if (!it.mixed(a, j / kStep * kStep, kStep)) continue;
                 const int page = __ldg(a.kv.pages + (int64_t)tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
                 if (page < 0 || page >= a.kv.n_pages) continue;
                 const int64_t at = (a.kv.page_base(page, head) + (j & in_page)) * HD;
@@ -470,9 +457,9 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                 }
             }
         }
-        bool write = pos == item0 && item1 <= w.w1;
+        bool write = it.begins && it.ends;
         if (!write) {
-            const int64_t slot_no = (int64_t)blockIdx.x * 2 + (pos == item0 ? 1 : 0);
+            const int64_t slot_no = (int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0);
             float *pp = a.parts + slot_no * part_floats(HD);
 #pragma unroll
             for (int i = 0; i < kPer; i++) {
@@ -485,7 +472,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             }
             __threadfence();
             __syncthreads();
-            const int c0 = cta_of(w, item0), c1 = cta_of(w, item1 - 1);
+            const int c0 = cta_of(range, it.item0), c1 = cta_of(range, it.item1 - 1);
             if (threadIdx.x == 0) sm.last = atomicAdd(a.counters + c0, 1) == c1 - c0;
             __syncthreads();
             write = sm.last;
@@ -522,7 +509,6 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                 else static_cast<uint16_t *>(out)[at] = from_f<uint16_t>(x);
             }
         }
-        pos = min(item1, w.w1);
     }
 }
 
@@ -530,7 +516,7 @@ template <int HD, int FMT, bool QF32>
 void launch_few(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
     constexpr int U = block_keys<FMT>();
     const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.log_page) + U - 1) / U;
-    const int64_t most = Sched<kRows, U>::slots(a.kv.n_rows, a.group, a.kv.n_seqs) * a.kv.n_kv;
+    const int64_t most = FewSched<FMT>::slots(a.kv.n_rows, a.group, a.kv.n_seqs) * a.kv.n_kv;
     const int64_t ctas = most < kMaxCtas ? most * blocks : kMaxCtas;  // most * blocks fits
     launch_pdl(paged_attn_few_kernel<HD, FMT, QF32>,
                dim3((unsigned)(ctas < kMaxCtas ? ctas : kMaxCtas)), dim3(kThreads), 0, st, out, q, a);

@@ -8,7 +8,8 @@
 // that lies in one CTA is written by it. An item cut by a CTA's border leaves (max, sum,
 // accumulator) per row in the scratch, and the CTA that arrives last (a counter at the item's
 // first CTA) joins the parts in their order, so the result does not depend on who was last. A CTA
-// has at most two cut items: the one it starts with and the one it ends with.
+// has at most two cut items: the one it starts with and the one it ends with. E blocks are added to
+// every item for what starting and ending one costs, so that CTAs with many short items get fewer.
 #pragma once
 
 #include "paged.cuh"
@@ -47,11 +48,12 @@ struct Tile {
     int rows;               // real rows, 0: no item
     int pos0;               // position of new token 0
     int k0, k1;             // keys any row sees
-    int b0, cost;           // first block, blocks (1 for a tile that sees no key)
+    int b0, blocks;         // first block, blocks (1 for a tile that sees no key)
 };
 
-template <int R, int U>
+template <int R, int U, int E>
 struct Sched {
+    static constexpr int kRowsPerTile = R, kBlock = U, kExtra = E;
     // Slots of tiles: sequence s has those from q_start[s] * group / R + s on, at least as many as
     // it has tiles.
     static __host__ __device__ int64_t slots(int64_t n_rows, int group, int n_seqs) {
@@ -60,6 +62,7 @@ struct Sched {
     static __device__ __forceinline__ int base(const AttnArgs &a, int s) {
         return (int)((int64_t)__ldg(a.kv.q_start + s) * a.group / R) + s;
     }
+    static __device__ __forceinline__ int cost(const Tile &t) { return t.rows ? t.blocks + E : 0; }
     // The last sequence whose slots start at or before `slot` (0 if none does).
     static __device__ __forceinline__ int seq_of(const AttnArgs &a, int slot) {
         int lo = 0, hi = a.kv.n_seqs;
@@ -85,7 +88,7 @@ struct Sched {
         t.k1 = max(last + 1, 0);
         t.k0 = a.window ? max(first - a.window + 1, 0) : 0;
         t.b0 = t.k0 / U;
-        t.cost = t.k1 > t.k0 ? (t.k1 + U - 1) / U - t.b0 : 1;
+        t.blocks = t.k1 > t.k0 ? (t.k1 + U - 1) / U - t.b0 : 1;
         return t;
     }
 };
@@ -105,9 +108,8 @@ struct SchedSmem {
     int slot, seq;
 };
 
-template <int R, int U, int THREADS>
+template <typename S, int THREADS>
 __device__ __forceinline__ Range find_range(const AttnArgs &a, SchedSmem &sm) {
-    using S = Sched<R, U>;
     const int n_slots = (int)S::slots(a.kv.n_rows, a.group, a.kv.n_seqs);
     const int per = (n_slots + THREADS - 1) / THREADS;
     const int s0 = min((int)threadIdx.x * per, n_slots), s1 = min(s0 + per, n_slots);
@@ -117,7 +119,7 @@ __device__ __forceinline__ Range find_range(const AttnArgs &a, SchedSmem &sm) {
         int s = first_seq = S::seq_of(a, s0);
         for (int slot = s0; slot < s1; slot++) {
             while (s + 1 < a.kv.n_seqs && S::base(a, s + 1) <= slot) s++;
-            mine += S::tile(a, slot, s).cost;
+            mine += S::cost(S::tile(a, slot, s));
         }
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -151,7 +153,7 @@ __device__ __forceinline__ Range find_range(const AttnArgs &a, SchedSmem &sm) {
         int64_t at = before;
         for (int slot = s0; slot < s1; slot++) {
             while (s + 1 < a.kv.n_seqs && S::base(a, s + 1) <= slot) s++;
-            const int c = S::tile(a, slot, s).cost;
+            const int c = S::cost(S::tile(a, slot, s));
             if (r.w0 < (at + c) * nk) {
                 sm.slot = slot;
                 sm.seq = s;
@@ -168,10 +170,68 @@ __device__ __forceinline__ Range find_range(const AttnArgs &a, SchedSmem &sm) {
     return r;
 }
 
-// The CTA that takes block x.
+// The CTA that takes position x.
 __device__ __forceinline__ int cta_of(const Range &r, int64_t x) {
     return (int)(((x + 1) * r.ctas - 1) / r.total);
 }
+
+// The items of a CTA in order. Roles of a CTA that walk by themselves see the same ones.
+template <typename S>
+struct Walk {
+    Range w;
+    int64_t pos, slot_at;    // how far; position of the slot's first item
+    int64_t item0, item1;    // positions of the item's blocks
+    Tile tl;
+    int slot, seq, cost;
+    int head, blk0, blk1;    // the item's kv head; this CTA's blocks of it
+    int first, last;         // positions of the item's first and last row
+    bool begins, ends;       // the item's first, last block is among them
+
+    __device__ __forceinline__ void start(const AttnArgs &a, const Range &r) {
+        w = r;
+        pos = r.w0;
+        slot = r.slot;
+        seq = r.seq;
+        slot_at = r.at;
+        cost = 0;
+        if (pos < w.w1) {
+            tl = S::tile(a, slot, seq);
+            cost = S::cost(tl);
+        }
+    }
+    __device__ __forceinline__ bool next(const AttnArgs &a) {
+        while (pos < w.w1) {
+            while (pos >= slot_at + (int64_t)cost * a.kv.n_kv) {
+                slot_at += (int64_t)cost * a.kv.n_kv;
+                // the lengths must not change under the kernel; if they do, it still ends
+                if (++slot >= w.n_slots) return false;
+                while (seq + 1 < a.kv.n_seqs && S::base(a, seq + 1) <= slot) seq++;
+                tl = S::tile(a, slot, seq);
+                cost = S::cost(tl);
+            }
+            head = (int)((pos - slot_at) / cost);
+            const int64_t at = slot_at + (int64_t)head * cost;
+            item0 = at + S::kExtra;
+            item1 = at + cost;
+            const int64_t lo = max(pos, item0), hi = min(item1, w.w1);
+            pos = hi;
+            if (lo >= hi) continue;  // only of the item's extra cost
+            blk0 = tl.b0 + (int)(lo - item0);
+            blk1 = tl.b0 + (int)(hi - item0);
+            begins = lo == item0;
+            ends = hi == item1;
+            first = tl.pos0 + tl.row0 / a.group;
+            last = tl.pos0 + (tl.row0 + tl.rows - 1) / a.group;
+            return true;
+        }
+        return false;
+    }
+    // Rows of the tile differ in which of the keys j0 .. j0 + n - 1 they see.
+    __device__ __forceinline__ bool mixed(const AttnArgs &a, int j0, int n) const {
+        const int jf = max(j0, tl.k0), jl = min(j0 + n, tl.k1) - 1;
+        return jl > first || (a.window && jf <= last - a.window);
+    }
+};
 
 // The kernel for many rows per sequence (paged_attention_wide.cu), scale_log2 >= 0: LAI_OK or an
 // error; and the F32 values of scratch it needs.

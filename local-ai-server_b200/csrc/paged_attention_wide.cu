@@ -3,21 +3,27 @@
 //
 // A tile is MT x 128 query rows (row = token * group + head of the group, so the heads that share
 // keys share a tile) against blocks of 128 keys. Per block S = Q K^T and then O += P V are
-// tcgen05 MMAs with M = 128; S, P and each block's P V live in TMEM.
-//   * K and V come row by row through the page table: a copy that may start and end anywhere in a
-//     page and that fills what is behind the last key with zeros, so it is done by a producer
-//     warpgroup (16-byte cp.async for BF16; for the 8-bit formats through registers, where they
-//     become binary16), in the 128-byte swizzle. K is K-major; V is the MN-major operand of P V in
-//     the same layout.
+// tcgen05 MMAs with M = 128; S, P and O (or a block's P V) live in TMEM.
+//   * One warp brings K and V through the page table, 16 keys at a time (a page holds a multiple
+//     of 16): BF16 with TMA tensor copies straight into the MMA's 128-byte swizzle, the 8-bit
+//     formats (and their scales) with bulk copies into a staging ring. A second warpgroup finishes
+//     each tile: it turns 8-bit values into binary16, and writes zeros over values behind the last
+//     key. K is K-major; V is the MN-major operand of P V in the same layout.
 //   * BF16 queries: two tiles of 128 rows share each K/V block, and one warpgroup's softmax runs
-//     under the other's MMAs. P overwrites S in TMEM.
+//     under the other's MMAs. A softmax thread owns a row (no shuffles) and holds the block's 128
+//     scores in registers; P overwrites S in TMEM. The maximum that weights are relative to only
+//     moves when it has grown by 2^8, so O is hardly ever rescaled.
 //   * F32 queries: one tile of 128 rows, its terms (hi + lo binary16; three bfloat16 terms over a
-//     BF16 cache) one after another into the same accumulator, the weights the same.
-//   * A softmax thread owns a row: no shuffles. It reads S twice (maximum, then weights), keeps
-//     the output row in registers, and adds each block's P V to it with the FMA that rescales it,
-//     so TMEM never needs a correction pass and long sequences do not add up truncated sums.
+//     BF16 cache) one after another into the same accumulator, smallest first, the weights the
+//     same. A block's P V starts from zero and is added to the output row, which the thread keeps
+//     in registers, so long sequences do not add up the MMA's truncated sums.
 //   * 8-bit: key scales multiply S, value scales P; both come with the block in shared memory.
+//     Weights are relative to the largest value scale too, so that they fit binary16.
 // Every wait is bounded; a wait that runs out raises LAI_DEVERR_TIMEOUT and ends the kernel.
+#include <cuda.h>
+
+#include <mutex>
+
 #include "paged_attention.cuh"
 #include "umma.cuh"
 
@@ -27,10 +33,12 @@ namespace {
 
 using bulk::smem_addr;
 
-constexpr int kThreads = 512;      // 2 softmax warpgroups, producers, MMA warp (+ 3 idle warps)
-constexpr int kU = 128;            // keys per block
-constexpr int kRing = 4;           // blocks whose scales and flags are kept
+constexpr int kThreads = 512;  // 2 softmax warpgroups, finishers, MMA warp, copy warp (+ 2 idle)
+constexpr int kU = 128;        // keys per block
+constexpr int kGroup = 16;     // keys per copy
+constexpr int kRing = 4;       // blocks whose scales and flags are kept
 constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr float kGrow = 8.f;   // log2 of how far weights may pass 1 before O is rescaled
 
 template <int HD, int FMT, bool QF32>
 struct Cfg {
@@ -38,19 +46,24 @@ struct Cfg {
     static constexpr int kTerms = QF32 ? (kF16 ? 2 : 3) : 1;
     static constexpr int MT = QF32 ? 1 : 2;
     static constexpr int R = 128 * MT;
-    static constexpr int kTile = 128 * HD * 2;  // bytes of an operand tile
-    static constexpr int kStages = kF16 || QF32 ? 4 : 5;
-    static constexpr float kLift = kF16 ? 13.f : 0.f;
+    static constexpr int kTile = 128 * HD * 2;         // bytes of an operand tile
+    static constexpr int kStages = kF16 ? 3 : QF32 ? 4 : 5;
+    static constexpr int kRaw = kF16 ? 3 : 0;          // 8-bit tiles in the staging ring
+    static constexpr int kRawTile = 128 * HD;
+    static constexpr int kLand = kF16 ? kRaw : kStages;  // tiles that copies land in
+    // binary16 weights: 2^kLift at the row's maximum, below 2^15 after kGrow and a value scale
+    static constexpr float kLift = kF16 ? 5.f : 0.f;
+    using S = Sched<R, kU, 3>;
 };
 
 template <int HD, int FMT, bool QF32>
 struct Ctl {
     using C = Cfg<HD, FMT, QF32>;
-    static constexpr int kScales = C::kF16 ? kU : 1;
-    uint64_t full[C::kStages], empty[C::kStages];
+    static constexpr int kScales = C::kF16 ? kU : 4;
+    float kscale[kRing][kScales], vscale[kRing][kScales];  // 16-byte aligned
+    uint64_t landed[C::kLand], taken[C::kLand], full[C::kStages], empty[C::kStages];
     uint64_t info[kRing];
     uint64_t q_full[2], s_full[2], p_full[2], pv_full[2], group[2];
-    float kscale[kRing][kScales], vscale[kRing][kScales];
     int vexp[kRing][4];
     int groups[kRing];  // bit i: 16-key group i of the block lies in a real page
     int vbad[kRing];    // the block (counted) from whose V infinities or NaN were taken out
@@ -100,15 +113,6 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                 "r"(real ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void st_shared16(uint32_t dst, const uint4 &v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z),
                  "r"(v.w)
@@ -147,21 +151,22 @@ template <bool F16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &p) 
     p &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
     return lo || hi;
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar))
+        : "memory");
+}
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
-// 8 elements of a row of q.
-template <bool F32> __device__ __forceinline__ void load8(const void *p, int64_t at, float (&x)[8]) {
-    if (F32) {
-        float lo[4], hi[4];
-        unpack<float>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + at)), lo);
-        unpack<float>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + at + 4)), hi);
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = lo[e], x[4 + e] = hi[e];
-    } else {
-        unpack<uint16_t>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at)), x);
-    }
-}
 
 // One element as F32, without its scale.
 template <int FMT> __device__ __forceinline__ float element(const unsigned char *v, int64_t i) {
@@ -173,65 +178,22 @@ template <int FMT> __device__ __forceinline__ float element(const unsigned char 
     return f;
 }
 
-// The items of a CTA in order; every role walks them by itself and sees the same ones.
-template <int R>
-struct Walk {
-    using S = Sched<R, kU>;
-    Range w;
-    int64_t pos, slot_at, item0, item1;
-    int slot, seq, head, blk0, blk1;
-    Tile tl;
-    __device__ __forceinline__ void start(const AttnArgs &a, const Range &r) {
-        w = r;
-        pos = r.w0;
-        slot = r.slot;
-        seq = r.seq;
-        slot_at = r.at;
-        if (pos < w.w1) tl = S::tile(a, slot, seq);
-    }
-    __device__ __forceinline__ bool next(const AttnArgs &a) {
-        if (pos >= w.w1) return false;
-        while (pos >= slot_at + (int64_t)tl.cost * a.kv.n_kv) {
-            slot_at += (int64_t)tl.cost * a.kv.n_kv;
-            if (++slot >= w.n_slots) return false;  // lengths that changed under the kernel
-            while (seq + 1 < a.kv.n_seqs && S::base(a, seq + 1) <= slot) seq++;
-            tl = S::tile(a, slot, seq);
-        }
-        head = (int)((pos - slot_at) / tl.cost);
-        item0 = slot_at + (int64_t)head * tl.cost;
-        item1 = item0 + tl.cost;
-        blk0 = tl.b0 + (int)(pos - item0);
-        const int64_t end = min(item1, w.w1);
-        blk1 = tl.b0 + (int)(end - item0);
-        begins = pos == item0;
-        ends = item1 <= w.w1;
-        pos = end;
-        return true;
-    }
-    bool begins, ends;
-    __device__ __forceinline__ int first(const AttnArgs &a) const { return tl.pos0 + tl.row0 / a.group; }
-    __device__ __forceinline__ int last(const AttnArgs &a) const {
-        return tl.pos0 + (tl.row0 + tl.rows - 1) / a.group;
-    }
-    // Rows of the tile differ in which keys of block blk they see.
-    __device__ __forceinline__ bool mixed(const AttnArgs &a, int blk, int first, int last) const {
-        const int jf = max(blk * kU, tl.k0), jl = min(blk * kU + kU, tl.k1) - 1;
-        return jl > first || (a.window && jf <= last - a.window);
-    }
-};
-
 template <int HD, int FMT, bool QF32>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) {
+paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
+                       const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<HD, FMT, QF32>;
+    using S = typename C::S;
     constexpr bool kF16 = C::kF16;
-    constexpr int MT = C::MT, R = C::R, kTerms = C::kTerms, ST = C::kStages;
+    constexpr int MT = C::MT, R = C::R, kTerms = C::kTerms, ST = C::kStages, LD = C::kLand;
     constexpr int kBytes = Fmt<FMT>::kBytes;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *q_smem = smem, *st_smem = smem + MT * kTerms * C::kTile;
-    auto &ctl = *reinterpret_cast<Ctl<HD, FMT, QF32> *>(st_smem + ST * C::kTile);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = threadIdx.x >> 7;
-    const int wt = threadIdx.x & 127;  // thread of its warpgroup
+    unsigned char *raw_smem = st_smem + ST * C::kTile;
+    auto &ctl = *reinterpret_cast<Ctl<HD, FMT, QF32> *>(raw_smem + C::kRaw * C::kRawTile);
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int wg = warp >> 2, wt = threadIdx.x & 127;  // warpgroup, thread of it
     volatile int *abort_flag = &ctl.abort;
 
     pdl_wait_prior();
@@ -243,19 +205,25 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a)
     if (blockIdx.x == 0)
         for (int s = threadIdx.x; s < a.kv.n_seqs; s += kThreads)
             if (!load_seq(a.kv, s).ok) flag(a.err, LAI_DEVERR_POSITION);
-    const Range range = find_range<R, kU, kThreads>(a, ctl.sched);
+    const Range range = find_range<S, kThreads>(a, ctl.sched);
     if (range.w0 >= range.w1) return;  // the whole CTA
     if (warp == 12) {
         umma::tmem_alloc(&ctl.tmem, 512);
         umma::tmem_relinquish();
     }
     if (threadIdx.x == 0) {
+        for (int i = 0; i < LD; i++) {
+            bulk::mbar_init(&ctl.landed[i], 1);
+            bulk::mbar_init(&ctl.taken[i], 4);
+        }
         for (int i = 0; i < ST; i++) {
-            bulk::mbar_init(&ctl.full[i], 128);
+            bulk::mbar_init(&ctl.full[i], 4);
             bulk::mbar_init(&ctl.empty[i], 1);
         }
-        for (int i = 0; i < kRing; i++) bulk::mbar_init(&ctl.info[i], 128);
-        for (int i = 0; i < kRing; i++) ctl.vbad[i] = -1;
+        for (int i = 0; i < kRing; i++) {
+            bulk::mbar_init(&ctl.info[i], 4);
+            ctl.vbad[i] = -1;
+        }
         for (int i = 0; i < 2; i++) {
             bulk::mbar_init(&ctl.q_full[i], 128);
             bulk::mbar_init(&ctl.group[i], 128);
@@ -270,250 +238,268 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a)
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = ctl.tmem;
-    // TMEM columns: S (and P over it with two tiles), P V; with one tile P has its own columns
+    // TMEM columns: S (and P over it with two tiles), then O or a block's P V; with one tile P has
+    // its own columns
     constexpr uint32_t kP = MT == 2 ? 0 : 128, kPV = MT == 2 ? 256 : 384;
 
-    // Bounded wait; false once this CTA gives up. wait_warp: the whole warp, which agrees.
+    // Bounded wait of a whole warp, which agrees on the answer; false once this CTA gives up.
     auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-        if (bulk::mbar_try_wait(bar, parity)) return true;
-        const uint64_t t0 = bulk::globaltimer_ns();
-        for (uint32_t n = 1;; n++) {
-            if (bulk::mbar_try_wait(bar, parity)) return true;
-            if ((n & 63u) == 0) {
-                if (*abort_flag) return false;
-                if (bulk::globaltimer_ns() - t0 > kWaitNs) {
-                    *abort_flag = 1;
-                    flag(a.err, LAI_DEVERR_TIMEOUT);
-                    return false;
+        bool ok = bulk::mbar_try_wait(bar, parity);
+        if (!ok) {
+            const uint64_t t0 = bulk::globaltimer_ns();
+            for (uint32_t n = 1; !ok; n++) {
+                ok = bulk::mbar_try_wait(bar, parity);
+                if (!ok && (n & 63u) == 0) {
+                    if (*abort_flag) break;
+                    if (bulk::globaltimer_ns() - t0 > kWaitNs) {
+                        *abort_flag = 1;
+                        flag(a.err, LAI_DEVERR_TIMEOUT);
+                        break;
+                    }
                 }
             }
         }
+        return __all_sync(0xffffffffu, ok);
     };
 
-    auto wait_warp = [&](uint64_t *bar, uint32_t parity) -> bool {
-        return __all_sync(0xffffffffu, wait(bar, parity));
-    };
-
-    Walk<R> it;
+    Walk<S> it;
     it.start(a, range);
-    if (wg == 2) {
-        // ================= producers: K and V block by block =================================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        constexpr int kIn = HD * kBytes / 16;          // 16-byte runs of a stored row
-        constexpr int kRowsAtOnce = 128 / kIn;         // rows that the warpgroup loads at a time
-        constexpr int kPasses = 128 / kRowsAtOnce;
-        constexpr int kAhead = FMT == LAI_KV_BF16 ? ST - 2 : 0;  // cp.async tiles under way
-        const int c = wt % kIn, r_in = wt / kIn;
-        const int in_page = a.kv.page_size() - 1;
-        uint32_t idx = 0, blocks = 0;              // operand tiles, blocks so far
-        uint32_t mixed_bits = 0;                   // bit i: the tile i before the newest is a mixed V
+    // The page of 16-key group `lane` (< 8) of the block at j0, or -1.
+    auto page_of = [&](int j0) -> int {
+        const int j = j0 + kGroup * lane;
+        if (lane >= kU / kGroup || j >= it.tl.k1) return -1;
+        const int page = __ldg(a.kv.pages + (int64_t)it.tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
+        return page >= 0 && page < a.kv.n_pages ? page : -1;
+    };
+    const int in_page = a.kv.page_size() - 1;
+
+    // Register shares: 2 x 128 x 192 + 2 x 128 x 64 = 512 x 128 (fewer where one warpgroup softmaxes)
+    if (wg < MT) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+
+    if (warp == 13) {
+        // ================= copies ============================================================
+        uint32_t idx = 0, blocks = 0;  // operand tiles, blocks so far
         bool ok = true;
-        // a cp.async tile has landed: mend it if it must be, and hand it over
-        auto publish = [&](uint32_t i, bool mixed_v) {
-            if (mixed_v) {
-                bool bad = false;
-                const uint32_t base = smem_addr(st_smem + (i % ST) * C::kTile);
-#pragma unroll 1
-                for (int p = 0; p < kPasses; p++) {
-                    const uint32_t at = base + chunk_off(p * kRowsAtOnce + r_in, c);
-                    uint4 v = ld_shared16(at);
-                    bool b = drop_nonfinite<false>(v.x);
-                    b |= drop_nonfinite<false>(v.y);
-                    b |= drop_nonfinite<false>(v.z);
-                    b |= drop_nonfinite<false>(v.w);
-                    if (b) st_shared16(at, v);
-                    bad |= b;
-                }
-                if (bad) ctl.vbad[(i / 2) % kRing] = (int)(i / 2);
-            }
-            bulk::fence_proxy_async_smem();
-            bulk::mbar_arrive(&ctl.full[i % ST]);
-        };
         while (ok && it.next(a)) {
-            const int first = it.first(a), last = it.last(a);
-            // ---- K and V
-            for (int blk = it.blk0; ok && blk < it.blk1; blk++) {
+            for (int blk = it.blk0; ok && blk < it.blk1; blk++, blocks++) {
                 const int j0 = blk * kU;
-                // lane i < 8 of every warp looks up the page of 16-key group i
-                int page = -1;
-                if (lane < 8 && j0 + 16 * lane < it.tl.k1) {
-                    page = __ldg(a.kv.pages + (int64_t)it.tl.seq * a.kv.max_pages +
-                                 ((j0 + 16 * lane) >> a.kv.log_page));
-                    if (page < 0 || page >= a.kv.n_pages) {
-                        if (wt < 8 && j0 + 16 * lane + 16 > it.tl.k0) flag(a.err, LAI_DEVERR_PAGE);
-                        page = -1;
+                const int page = page_of(j0);
+                const uint32_t groups = __ballot_sync(0xffffffffu, page >= 0);
+                for (int kv = 0; kv < 2; kv++, idx++) {
+                    const uint32_t land = idx % LD;
+                    if (idx >= (uint32_t)LD &&
+                        !(ok = wait(kF16 ? &ctl.taken[land] : &ctl.empty[land], (idx / LD - 1) & 1)))
+                        break;
+                    constexpr uint32_t kGroupBytes = kGroup * HD * kBytes;
+                    if (lane == 0) {
+                        const uint32_t n = __popc(groups);
+                        bulk::mbar_arrive_expect_tx(&ctl.landed[land],
+                                                    n * (kGroupBytes + (kF16 && kv == 0 ? 2 * kGroup * 4 : 0)));
+                    }
+                    __syncwarp();
+                    if constexpr (kF16) {
+                        if (page >= 0) {
+                            const int64_t at = a.kv.page_base(page, it.head) + ((j0 + kGroup * lane) & in_page);
+                            bulk::load(raw_smem + land * C::kRawTile + lane * kGroupBytes,
+                                       (kv ? a.kv.v : a.kv.k) + at * HD, kGroupBytes, &ctl.landed[land]);
+                            if (kv == 0) {
+                                bulk::load(&ctl.kscale[blocks % kRing][kGroup * lane], a.kv.k_scale + at, kGroup * 4, &ctl.landed[land]);
+                                bulk::load(&ctl.vscale[blocks % kRing][kGroup * lane], a.kv.v_scale + at, kGroup * 4, &ctl.landed[land]);
+                            }
+                        }
+                    } else {
+                        constexpr int kHalves = HD / 64;
+                        const int g = lane / kHalves, h = lane % kHalves;
+                        const int pg = __shfl_sync(0xffffffffu, page, g & 7);
+                        if (g < kU / kGroup && pg >= 0) {
+                            const int64_t at = a.kv.page_base(pg, it.head) + ((j0 + kGroup * g) & in_page);
+                            tma_load_2d(smem_addr(st_smem + land * C::kTile) + h * 16384 + g * (kGroup * 128),
+                                        kv ? &v_map : &k_map, h * 64, (int)at, &ctl.landed[land]);
+                        }
                     }
                 }
-                const int groups = (int)(__ballot_sync(0xffffffffu, page >= 0) & 0xffu);
-                const bool mixed = FMT != LAI_KV_I8 && it.mixed(a, blk, first, last);
-                const int slot = blocks % kRing;
-                const int j_mine = j0 + wt;  // this thread's key for the scales
-#pragma unroll 1
+            }
+        }
+        // an abort leaves copies in flight: they get a millisecond before shared memory goes
+        if (!ok) {
+            const uint64_t t0 = bulk::globaltimer_ns();
+            while (bulk::globaltimer_ns() - t0 < 1000000ull) {}
+        }
+    } else if (wg == 2) {
+        // ================= finishing tiles ===================================================
+        uint32_t idx = 0, blocks = 0;
+        bool ok = true;
+        while (ok && it.next(a)) {
+            for (int blk = it.blk0; ok && blk < it.blk1; blk++, blocks++) {
+                const int j0 = blk * kU, slot = blocks % kRing;
+                const int page = page_of(j0);
+                if (wt < kU / kGroup && page < 0 && j0 + kGroup * lane < it.tl.k1 &&
+                    j0 + kGroup * lane + kGroup > it.tl.k0)
+                    flag(a.err, LAI_DEVERR_PAGE);
+                const uint32_t groups = __ballot_sync(0xffffffffu, page >= 0);
+                const bool whole = groups == 0xff && j0 >= it.tl.k0 && j0 + kU <= it.tl.k1;
+                const bool mixed = FMT != LAI_KV_I8 && it.mixed(a, j0, kU);
+                auto there = [&](int r) {
+                    return j0 + r >= it.tl.k0 && j0 + r < it.tl.k1 && (groups >> (r / kGroup) & 1);
+                };
                 for (int kv = 0; kv < 2; kv++, idx++) {
-                    if (idx >= (uint32_t)ST && !wait_warp(&ctl.empty[idx % ST], (idx / ST - 1) & 1)) {
-                        ok = false;
-                        break;
-                    }
-                    if (kv == 0) {  // the block's scales and pages: its ring entry is free by now
+                    const uint32_t land = idx % LD;
+                    if (!(ok = wait(&ctl.landed[land], (idx / LD) & 1))) break;
+                    if (kF16 && idx >= (uint32_t)ST && !(ok = wait(&ctl.empty[idx % ST], (idx / ST - 1) & 1))) break;
+                    if (kv == 0) {  // the block's ring entries are free by now
                         if (kF16) {
-                            const int pg = __shfl_sync(0xffffffffu, page, (wt >> 4) & 7);
-                            float ks = 0.f, vs = 0.f;
-                            if (pg >= 0 && j_mine >= it.tl.k0 && j_mine < it.tl.k1) {
-                                const int64_t at = a.kv.page_base(pg, it.head) + (j_mine & in_page);
-                                ks = __ldg(a.kv.k_scale + at);
-                                vs = __ldg(a.kv.v_scale + at);
-                            }
-                            ctl.kscale[slot][kF16 ? wt : 0] = ks;
-                            ctl.vscale[slot][kF16 ? wt : 0] = vs;
+                            const float vs = there(wt) ? ctl.vscale[slot][kF16 ? wt : 0] : 0.f;
                             const uint32_t u = __float_as_uint(vs) & 0x7fffffffu;
                             const uint32_t top = __reduce_max_sync(0xffffffffu, u < 0x7f800000u ? u : 0u);
                             if (lane == 0) ctl.vexp[slot][wt >> 5] = (int)(top >> 23) - 127;
                         }
-                        if (wt == 0) ctl.groups[slot] = groups;
-                        bulk::mbar_arrive(&ctl.info[slot]);
+                        if (wt == 0) ctl.groups[slot] = (int)groups;
+                        __syncwarp();
+                        if (lane == 0) bulk::mbar_arrive(&ctl.info[slot]);
                     }
-                    const unsigned char *src = (kv ? a.kv.v : a.kv.k) + c * 16;
                     const uint32_t dst = smem_addr(st_smem + (idx % ST) * C::kTile);
-                    if constexpr (FMT == LAI_KV_BF16) {
-#pragma unroll
-                        for (int p = 0; p < kPasses; p++) {
-                            const int r = p * kRowsAtOnce + r_in, j = j0 + r;
-                            const int pg = __shfl_sync(0xffffffffu, page, p * kRowsAtOnce / 16);
-                            const bool real = pg >= 0 && j >= it.tl.k0 && j < it.tl.k1;
-                            const int64_t at = a.kv.page_base(real ? pg : 0, it.head) + (real ? j & in_page : 0);
-                            cp_async16(dst + chunk_off(r, c), src + at * (HD * 2), real);
-                        }
-                        cp_async_commit();
-                        mixed_bits = mixed_bits << 1 | (uint32_t)(mixed && kv);
-                        if (idx >= (uint32_t)kAhead) {
-                            cp_async_wait<kAhead>();
-                            publish(idx - kAhead, mixed_bits >> kAhead & 1);
-                        }
-                    } else {
-                        uint4 raw[kPasses];
-#pragma unroll
-                        for (int p = 0; p < kPasses; p++) {
-                            const int r = p * kRowsAtOnce + r_in, j = j0 + r;
-                            // rows p * kRowsAtOnce + r_in of one warp may span two groups (HD 64)
-                            const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
-                            raw[p] = make_uint4(0, 0, 0, 0);
-                            if (pg >= 0 && j >= it.tl.k0 && j < it.tl.k1)
-                                raw[p] = ld_stream(src + (a.kv.page_base(pg, it.head) + (j & in_page)) * HD);
-                        }
-                        bool bad = false;
-#pragma unroll
-                        for (int p = 0; p < kPasses; p++) {
-                            const int r = p * kRowsAtOnce + r_in;
-                            uint4 lo = make_uint4(half2_of<FMT, false>(raw[p].x), half2_of<FMT, true>(raw[p].x),
-                                                  half2_of<FMT, false>(raw[p].y), half2_of<FMT, true>(raw[p].y));
-                            uint4 hi = make_uint4(half2_of<FMT, false>(raw[p].z), half2_of<FMT, true>(raw[p].z),
-                                                  half2_of<FMT, false>(raw[p].w), half2_of<FMT, true>(raw[p].w));
+                    bool bad = false, wrote = kF16;
+                    if constexpr (kF16) {
+                        constexpr int kIn = HD / 16, kAtOnce = 128 / kIn;  // runs of a row, rows at a time
+                        const int c = wt % kIn, r_in = wt / kIn;
+                        // a row's 8 lanes write 8 different 16-byte columns of a 128-byte line
+                        const bool swap = HD == 128 && c >= kIn / 2;
+                        const uint32_t src = smem_addr(raw_smem + land * C::kRawTile) + wt * 16;
+#pragma unroll 4
+                        for (int p = 0; p < 128 / kAtOnce; p++) {
+                            const int r = p * kAtOnce + r_in;
+                            uint4 raw = ld_shared16(src + p * 2048);
+                            if (!whole && kv && !there(r)) raw = make_uint4(0, 0, 0, 0);
+                            uint4 lo = make_uint4(half2_of<FMT, false>(raw.x), half2_of<FMT, true>(raw.x),
+                                                  half2_of<FMT, false>(raw.y), half2_of<FMT, true>(raw.y));
+                            uint4 hi = make_uint4(half2_of<FMT, false>(raw.z), half2_of<FMT, true>(raw.z),
+                                                  half2_of<FMT, false>(raw.w), half2_of<FMT, true>(raw.w));
                             if (mixed && kv) {
                                 bad |= drop_nonfinite<true>(lo.x) | drop_nonfinite<true>(lo.y) |
                                        drop_nonfinite<true>(lo.z) | drop_nonfinite<true>(lo.w);
                                 bad |= drop_nonfinite<true>(hi.x) | drop_nonfinite<true>(hi.y) |
                                        drop_nonfinite<true>(hi.z) | drop_nonfinite<true>(hi.w);
                             }
-                            st_shared16(dst + chunk_off(r, 2 * c), lo);
-                            st_shared16(dst + chunk_off(r, 2 * c + 1), hi);
+                            st_shared16(dst + chunk_off(r, 2 * c + swap), swap ? hi : lo);
+                            st_shared16(dst + chunk_off(r, 2 * c + !swap), swap ? lo : hi);
                         }
-                        if (bad) ctl.vbad[slot] = (int)blocks;
-                        bulk::fence_proxy_async_smem();
+                    } else if (kv && (!whole || mixed)) {  // thread = row of the tile
+                        const bool gone = !there(wt);
+                        if (gone || mixed) {
+#pragma unroll 1
+                            for (int c = 0; c < HD / 8; c++) {
+                                const uint32_t at = dst + chunk_off(wt, c);
+                                uint4 v = make_uint4(0, 0, 0, 0);
+                                if (!gone) {
+                                    v = ld_shared16(at);
+                                    bad |= drop_nonfinite<false>(v.x) | drop_nonfinite<false>(v.y) |
+                                           drop_nonfinite<false>(v.z) | drop_nonfinite<false>(v.w);
+                                }
+                                st_shared16(at, v);
+                            }
+                        }
+                        wrote = true;
+                    }
+                    if (bad) ctl.vbad[slot] = (int)blocks;
+                    if (wrote) bulk::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
                         bulk::mbar_arrive(&ctl.full[idx % ST]);
+                        if (kF16) bulk::mbar_arrive(&ctl.taken[land]);
                     }
                 }
-                blocks++;
             }
         }
-        if constexpr (FMT == LAI_KV_BF16) {
-            cp_async_wait<0>();
-            if (ok)
-                for (uint32_t i = idx < (uint32_t)kAhead ? 0 : idx - kAhead; i < idx; i++)
-                    publish(i, mixed_bits >> (idx - 1 - i) & 1);
-        }
-    } else if (wg == 3) {
-        // ================= the MMA thread ====================================================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == 12 && lane == 0) {
-            constexpr uint32_t kIdS = idesc<kF16, 128, false>(), kIdO = idesc<kF16, HD, true>();
-            uint32_t idx = 0, n_q[2] = {0, 0}, n_mt[2] = {0, 0};
-            bool ok = true;
-            auto scores = [&](int mt, uint32_t i) {
-                const uint32_t kb = smem_addr(st_smem + (i % ST) * C::kTile);
+    } else if (warp == 12) {
+        // ================= MMAs ==============================================================
+        constexpr uint32_t kIdS = idesc<kF16, 128, false>(), kIdO = idesc<kF16, HD, true>();
+        const bool leader = elect_one();
+        uint32_t idx = 0, n_q[2] = {0, 0}, n_mt[2] = {0, 0};
+        bool ok = true;
+        // what the leader issued so far arrives on bar when it is done
+        auto commit = [&](uint64_t *bar) {
+            if (leader) umma::commit(bar);
+            __syncwarp();
+        };
+        auto scores = [&](int mt, uint32_t i) {
+            const uint64_t kd = desc_kmajor(smem_addr(st_smem + (i % ST) * C::kTile));
+            const uint64_t qd = desc_kmajor(smem_addr(q_smem) + mt * C::kTile);
+            if (leader) {
 #pragma unroll
-                for (int t = 0; t < kTerms; t++) {
-                    const uint32_t qb = smem_addr(q_smem) + (t * MT + mt) * C::kTile;
+                for (int t = kTerms - 1; t >= 0; t--)
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++) {
+                        constexpr uint32_t kT = MT * C::kTile;
                         const uint32_t off = (k / 4) * 16384 + (k % 4) * 32;
-                        mma_ss(tmem + mt * 128, desc_kmajor(qb + off), desc_kmajor(kb + off), kIdS, t || k);
+                        mma_ss(tmem + mt * 128, qd + ((t * kT + off) >> 4), kd + (off >> 4), kIdS,
+                               t != kTerms - 1 || k);
                     }
-                }
-                umma::commit(&ctl.s_full[mt]);
-            };
-            while (ok && it.next(a)) {
-                const int tiles = MT == 2 && it.tl.rows > 128 ? 2 : 1;
-                const int nb = it.blk1 - it.blk0;
-                ok = wait(&ctl.full[idx % ST], (idx / ST) & 1);
+            }
+            commit(&ctl.s_full[mt]);
+        };
+        while (ok && it.next(a)) {
+            const int tiles = MT == 2 && it.tl.rows > 128 ? 2 : 1;
+            const int nb = it.blk1 - it.blk0;
+            ok = wait(&ctl.full[idx % ST], (idx / ST) & 1);
+            for (int mt = 0; ok && mt < tiles; mt++) {
+                ok = wait(&ctl.q_full[mt], n_q[mt]++ & 1);
+                umma::fence_after_sync();
+                if (ok) scores(mt, idx);
+            }
+            if (!ok) break;
+            commit(&ctl.empty[idx % ST]);
+            for (int b = 0; ok && b < nb; b++) {
+                const uint32_t vi = idx + 1, ki = idx + 2;
+                const bool more = b + 1 < nb;
                 for (int mt = 0; ok && mt < tiles; mt++) {
-                    ok = wait(&ctl.q_full[mt], n_q[mt]++ & 1);
-                    umma::fence_after_sync();
-                    if (ok) scores(mt, idx);
-                }
-                if (!ok) break;
-                umma::commit(&ctl.empty[idx % ST]);
-                for (int b = 0; ok && b < nb; b++) {
-                    const uint32_t vi = idx + 1, ki = idx + 2;
-                    const bool more = b + 1 < nb;
-                    for (int mt = 0; ok && mt < tiles; mt++) {
-                        ok = wait(&ctl.p_full[mt], n_mt[mt] & 1);
-                        n_mt[mt]++;
-                        if (MT == 1 && ok && more) {  // the next scores while P V waits for V
-                            ok = wait(&ctl.full[ki % ST], (ki / ST) & 1);
-                            umma::fence_after_sync();
-                            if (ok) scores(mt, ki);
-                        }
-                        ok = ok && wait(&ctl.full[vi % ST], (vi / ST) & 1);
-                        if (!ok) break;
+                    if (!(ok = wait(&ctl.p_full[mt], n_mt[mt]++ & 1))) break;
+                    if (MT == 1 && more) {  // the next scores while P V waits for V
+                        if (!(ok = wait(&ctl.full[ki % ST], (ki / ST) & 1))) break;
                         umma::fence_after_sync();
-                        const uint32_t vb = smem_addr(st_smem + (vi % ST) * C::kTile);
+                        scores(mt, ki);
+                    }
+                    if (!(ok = wait(&ctl.full[vi % ST], (vi / ST) & 1))) break;
+                    umma::fence_after_sync();
+                    const uint64_t vd = desc_mnmajor(smem_addr(st_smem + (vi % ST) * C::kTile));
+                    if (leader) {
 #pragma unroll
-                        for (int t = 0; t < kTerms; t++)
+                        for (int t = kTerms - 1; t >= 0; t--)
 #pragma unroll
                             for (int k = 0; k < kU / 16; k++)
                                 mma_ts(tmem + kPV + mt * 128, tmem + kP + mt * 128 + t * 64 + k * 8,
-                                       desc_mnmajor(vb + k * 2048), kIdO, t || k);
-                        umma::commit(&ctl.pv_full[mt]);
-                        if (MT == 2 && more) {
-                            ok = wait(&ctl.full[ki % ST], (ki / ST) & 1);
-                            umma::fence_after_sync();
-                            if (ok) scores(mt, ki);
-                        }
+                                       vd + ((k * 2048) >> 4), kIdO,
+                                       (MT == 2 && b > 0) || t != kTerms - 1 || k);
                     }
-                    if (!ok) break;
-                    umma::commit(&ctl.empty[vi % ST]);
-                    if (more) umma::commit(&ctl.empty[ki % ST]);
-                    idx += 2;
+                    if (MT == 1 || !more) commit(&ctl.pv_full[mt]);
+                    if (MT == 2 && more) {
+                        if (!(ok = wait(&ctl.full[ki % ST], (ki / ST) & 1))) break;
+                        umma::fence_after_sync();
+                        scores(mt, ki);
+                    }
                 }
+                if (!ok) break;
+                commit(&ctl.empty[vi % ST]);
+                if (more) commit(&ctl.empty[ki % ST]);
+                idx += 2;
             }
-            // Every MMA is done before TMEM is given back: each result was waited for. After an
-            // abort nobody waits, so the MMAs in flight get a millisecond.
-            if (!ok) {
-                const uint64_t t0 = bulk::globaltimer_ns();
-                while (bulk::globaltimer_ns() - t0 < 1000000ull) {}
-            }
+        }
+        // Every MMA is done before TMEM is given back: each result was waited for. After an abort
+        // nobody waits, so the MMAs in flight get a millisecond.
+        if (!ok) {
+            const uint64_t t0 = bulk::globaltimer_ns();
+            while (bulk::globaltimer_ns() - t0 < 1000000ull) {}
         }
     } else if (wg < MT) {
         // ================= softmax: a thread per row =========================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int mt = wg;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + lane_base + mt * 128, t_p = t_s + kP, t_pv = tmem + lane_base + kPV + mt * 128;
-        uint32_t n = 0, blocks = 0, n_group = 0;  // this tile's blocks, all blocks, joins
+        uint32_t n = 0, blocks = 0, n_group = 0, n_items = 0;  // this tile's blocks, all blocks, joins, items
         bool ok = true;
         auto join = [&]() {  // all of the warpgroup, within the bound
             bulk::mbar_arrive(&ctl.group[mt]);
-            return wait_warp(&ctl.group[mt], n_group++ & 1);
+            return wait(&ctl.group[mt], n_group++ & 1);
         };
         while (ok && it.next(a)) {
             const int nb = it.blk1 - it.blk0;
@@ -525,33 +511,49 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a)
             const bool row_ok = r < it.tl.rows;
             const int row_pos = row_ok ? it.tl.pos0 + tok : -1;
             const int row_from = a.window ? row_pos - a.window : -1;  // sees (row_from, row_pos]
-            const int first = it.first(a), last = it.last(a);
+            const int row_head = it.head * a.group + (fr - tok * a.group);
             float c = a.scale_log2;
             {  // this row of Q into shared memory; the last scores of the item before are done
-                const int64_t at = ((int64_t)it.tl.q_row0 + tok) * a.ld_q +
-                                   (int64_t)(it.head * a.group + (fr - tok * a.group)) * HD;
+                const int64_t at = ((int64_t)it.tl.q_row0 + tok) * a.ld_q + (int64_t)row_head * HD;
                 const uint32_t dst = smem_addr(q_smem) + mt * C::kTile;
+                constexpr int kRuns = QF32 ? HD / 4 : HD / 8;
+                uint4 raw[kRuns];
+                const uint4 *src = reinterpret_cast<const uint4 *>(
+                    QF32 ? (const void *)(static_cast<const float *>(qp) + at)
+                         : (const void *)(static_cast<const uint16_t *>(qp) + at));
+#pragma unroll
+                for (int i = 0; i < kRuns; i++) raw[i] = row_ok ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
                 float up = 1.f;
                 if (kF16) {  // the row's largest into [2^13, 2^14)
                     uint32_t top = 0;
-                    if (row_ok)
-#pragma unroll 4
-                        for (int d = 0; d < HD; d += 8) {
-                            float x[8];
-                            load8<QF32>(qp, at + d, x);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                    for (int i = 0; i < kRuns; i++) {
+                        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (QF32) top = max(top, w[e] & 0x7fffffffu);
+                            else top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
                         }
+                    }
                     const int e = (int)(top >> 23) - 127;
                     up = pow2i(13 - e);
                     c *= pow2i(e - 13);
                 }
-#pragma unroll 4
-                for (int d = 0; d < HD; d += 8) {
-                    float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = 0.f;
-                    if (row_ok) load8<QF32>(qp, at + d, x);
+                for (int d = 0; d < HD / 8; d++) {
+                    if (!kF16 && !QF32) {
+                        st_shared16(dst + chunk_off(wt, d), raw[d]);
+                        continue;
+                    }
+                    float x[8];
+                    if (QF32) {
+                        const uint4 u = raw[(2 * d) % kRuns], v = raw[(2 * d + 1) % kRuns];
+                        const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = __uint_as_float(w[e]);
+                    } else {
+                        unpack<uint16_t>(raw[d], x);
+                    }
                     if (kF16)
 #pragma unroll
                         for (int e = 0; e < 8; e++) x[e] *= up;
@@ -562,212 +564,293 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a)
                         v.y = take2<kF16>(x[2], x[3]);
                         v.z = take2<kF16>(x[4], x[5]);
                         v.w = take2<kF16>(x[6], x[7]);
-                        st_shared16(dst + t * MT * C::kTile + chunk_off(wt, d / 8), v);
+                        st_shared16(dst + t * MT * C::kTile + chunk_off(wt, d), v);
                     }
                 }
                 bulk::fence_proxy_async_smem();
                 bulk::mbar_arrive(&ctl.q_full[mt]);
             }
-            float m = neg_inf(), l = 0.f, alpha = 0.f, o[HD];
-            int ve = -90;
+            // Weights are 2^(score - off + kLift), off = maximum + exponent of the value scales;
+            // l and O are sums of these.
+            float m = neg_inf(), off = neg_inf(), l = 0.f, alpha = 0.f;
+            int ve = kF16 ? -90 : 0;
             bool bad = false;
+            constexpr int kKeep = MT == 1 ? HD : 1;
+            float o[kKeep];
 #pragma unroll
-            for (int d = 0; d < HD; d++) o[d] = 0.f;
-            auto add_pv = [&](uint32_t block) {
+            for (int d = 0; d < kKeep; d++) o[d] = 0.f;
+            auto saw_bad = [&](uint32_t block) {
+                if (FMT != LAI_KV_I8) bad |= *(volatile int *)&ctl.vbad[block % kRing] == (int)block;
+            };
+            auto add_pv = [&]() {
                 umma::fence_after_sync();
 #pragma unroll
-                for (int g = 0; g < HD / 32; g++) {
+                for (int g = 0; g < kKeep / 32; g++) {
                     uint32_t x[32];
                     umma::tmem_ld_32x32b_x32(t_pv + 32 * g, x);
                     umma::tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 32; i++)
-                        o[32 * g + i] = fmaf(o[32 * g + i], alpha, __uint_as_float(x[i]));
+                        o[(32 * g + i) % kKeep] = fmaf(o[(32 * g + i) % kKeep], alpha, __uint_as_float(x[i]));
                 }
                 umma::fence_before_sync();
-                if (FMT != LAI_KV_I8) bad |= *(volatile int *)&ctl.vbad[block % kRing] == (int)block;
             };
             for (int b = 0; b < nb; b++, n++, blocks++) {
-                const int blk = it.blk0 + b, slot = blocks % kRing;
-                ok = wait_warp(&ctl.info[slot], (blocks / kRing) & 1) && wait_warp(&ctl.s_full[mt], n & 1);
-                if (!ok) break;
+                const int j0 = (it.blk0 + b) * kU, slot = blocks % kRing;
+                if (!(ok = wait(&ctl.info[slot], (blocks / kRing) & 1) && wait(&ctl.s_full[mt], n & 1))) break;
                 umma::fence_after_sync();
+                if (MT == 2 && b > 0) saw_bad(blocks - 1);  // its P V came before these scores
                 const int groups = ctl.groups[slot];
                 // element i of the block is seen where lo <= i <= hi
-                const int hi = row_pos - blk * kU, lo = row_from + 1 - blk * kU;
-                const bool masked = groups != 0xff || blk * kU + kU - 1 > first || it.tl.k0 > blk * kU ||
-                                    (a.window && blk * kU <= last - a.window) || it.tl.rows < mt * 128 + 128;
-                auto seen = [&](int i) { return i <= hi && i >= lo && (groups >> (i >> 4) & 1); };
-                // ---- the maximum
-                float top = neg_inf();
-                auto max_pass = [&](auto mask) {
-#pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        uint32_t x[32];
-                        umma::tmem_ld_32x32b_x32(t_s + 32 * g, x);
-                        umma::tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            float v = __uint_as_float(x[i]);
-                            if (kF16) v *= ctl.kscale[slot][kF16 ? 32 * g + i : 0];
-                            if (decltype(mask)::value) v = seen(32 * g + i) ? v : neg_inf();
-                            top = fmaxf(top, v);
-                        }
-                    }
-                };
-                if (masked) max_pass(Yes{}); else max_pass(No{});
-                if (MT == 1 && b > 0) {  // P V of the block before, while S waited
-                    ok = wait_warp(&ctl.pv_full[mt], (n - 1) & 1);
-                    if (!ok) break;
-                    add_pv(blocks - 1);
-                }
-                const float mn = fmaxf(m, top == neg_inf() ? top : top * c);
-                const float mu = mn == neg_inf() ? 0.f : mn;
-                alpha = ex2(m - mu);
-                m = mn;
-                float off = mu - C::kLift;
-                if (kF16) {  // sums and weights are in units of 2^ve, the largest value scale so far
+                const int hi = row_pos - j0, lo = row_from + 1 - j0;
+                const bool masked = groups != 0xff || j0 + kU - 1 > it.first || it.tl.k0 > j0 ||
+                                    (a.window && j0 <= it.last - a.window) || it.tl.rows < mt * 128 + 128;
+                auto seen = [&](int i) { return i <= hi && i >= lo && (groups >> (i / kGroup) & 1); };
+                const float4 *k4 = reinterpret_cast<const float4 *>(ctl.kscale[slot]);
+                const float4 *v4 = reinterpret_cast<const float4 *>(ctl.vscale[slot]);
+                if (kF16) {
                     const int *e4 = ctl.vexp[slot];
-                    const int e = min(max(max(max(e4[0], e4[1]), max(e4[2], e4[3])), ve), 90);
-                    alpha *= pow2i(ve - e);
-                    ve = e;
-                    off += (float)e;
+                    ve = min(max(max(max(e4[0], e4[1]), max(e4[2], e4[3])), ve), 90);
                 }
-                l *= alpha;
-                // ---- the weights
-                float sum0 = 0.f, sum1 = 0.f;
-                auto p_pass = [&](auto mask) {
+                // scores of 32 keys, scaled by their keys' scales and masked
+                auto fetch = [&](int g, float *x, auto mask) {
+                    uint32_t u[32];
+                    umma::tmem_ld_32x32b_x32(t_s + 32 * g, u);
+                    umma::tmem_wait_ld();
 #pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        uint32_t x[32];
-                        umma::tmem_ld_32x32b_x32(t_s + 32 * g, x);
-                        umma::tmem_wait_ld();
-                        uint32_t w[kTerms][16];
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 ks = make_float4(1.f, 1.f, 1.f, 1.f);
+                        if (kF16) ks = k4[kF16 ? 8 * g + i / 4 : 0];
+                        const float s4[4] = {ks.x, ks.y, ks.z, ks.w};
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            float p[2];
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                float v = __uint_as_float(x[i + h]);
-                                if (kF16) v *= ctl.kscale[slot][kF16 ? 32 * g + i + h : 0];
-                                v = ex2(fmaf(v, c, -off));
-                                if (decltype(mask)::value) v = seen(32 * g + i + h) ? v : 0.f;
-                                (h ? sum1 : sum0) += v;
-                                if (kF16) {
-                                    const float vs = ctl.vscale[slot][kF16 ? 32 * g + i + h : 0];
-                                    v = decltype(mask)::value ? (seen(32 * g + i + h) ? v * vs : 0.f) : v * vs;
-                                }
-                                p[h] = v;
-                            }
-#pragma unroll
-                            for (int t = 0; t < kTerms; t++) w[t][i / 2] = take2<kF16>(p[0], p[1]);
+                        for (int h = 0; h < 4; h++) {
+                            float v = __uint_as_float(u[i + h]);
+                            if (kF16) v *= s4[h];
+                            if (decltype(mask)::value) v = seen(32 * g + i + h) ? v : neg_inf();
+                            x[i + h] = v;
                         }
-#pragma unroll
-                        for (int t = 0; t < kTerms; t++) tmem_st_x16(t_p + t * 64 + 16 * g, w[t]);
                     }
                 };
-                if (masked) p_pass(Yes{}); else p_pass(No{});
-                l += sum0 + sum1;
+                auto max_of = [&](const float *x, float &t0, float &t1) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        t0 = fmaxf(t0, fmaxf(x[i], x[i + 1]));
+                        t1 = fmaxf(t1, fmaxf(x[i + 2], x[i + 3]));
+                    }
+                };
+                // weights of 32 keys, into P
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                auto weigh = [&](int g, const float *x, float base, auto mask) {
+                    uint32_t w[kTerms][16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 vs = make_float4(1.f, 1.f, 1.f, 1.f);
+                        if (kF16) vs = v4[kF16 ? 8 * g + i / 4 : 0];
+                        const float s4[4] = {vs.x, vs.y, vs.z, vs.w};
+                        float p[4];
+#pragma unroll
+                        for (int h = 0; h < 4; h++) {
+                            // a masked score is -inf, also after its product with c = 0
+                            p[h] = ex2(fmaf(x[i + h], c, -base));
+                            if (decltype(mask)::value) p[h] = seen(32 * g + i + h) ? p[h] : 0.f;
+                            sum[h] += p[h];
+                            if (kF16) {
+                                p[h] *= s4[h];
+                                if (decltype(mask)::value) p[h] = seen(32 * g + i + h) ? p[h] : 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < kTerms; t++) {
+                            w[t][i / 2] = take2<kF16>(p[0], p[1]);
+                            w[t][i / 2 + 1] = take2<kF16>(p[2], p[3]);
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < kTerms; t++) tmem_st_x16(t_p + t * 64 + 16 * g, w[t]);
+                };
+                // moves off to the block's maximum; what l and O must be multiplied with
+                auto move = [&](float top, float slack) -> float {
+                    m = fmaxf(m, top == neg_inf() ? top : top * c);
+                    const float to = m + (float)ve;
+                    if (!(to > off + slack)) return 1.f;
+                    const float f = ex2(off - to);  // off = -inf: 0
+                    off = to;
+                    l *= f;
+                    return f;
+                };
+                if constexpr (MT == 2) {
+                    auto block = [&](auto mask) {
+                        float x[kU], t0 = neg_inf(), t1 = neg_inf();
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+                            fetch(g, x + 32 * g, mask);
+                            max_of(x + 32 * g, t0, t1);
+                        }
+                        const float f = move(fmaxf(t0, t1), kGrow);
+                        if (b > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+                            // the scores' MMAs came after the last P V, so O is complete
+#pragma unroll 1
+                            for (int g = 0; g < HD / 16; g++) {
+                                uint32_t y[16];
+                                umma::tmem_ld_32x32b_x16(t_pv + 16 * g, y);
+                                umma::tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; i++) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                                tmem_st_x16(t_pv + 16 * g, y);
+                            }
+                        }
+                        const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
+#pragma unroll
+                        for (int g = 0; g < 4; g++) weigh(g, x + 32 * g, base, mask);
+                    };
+                    if (masked) block(Yes{}); else block(No{});
+                } else {
+                    auto pass1 = [&](auto mask) {
+                        float t0 = neg_inf(), t1 = neg_inf();
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+                            float x[32];
+                            fetch(g, x, mask);
+                            max_of(x, t0, t1);
+                        }
+                        return fmaxf(t0, t1);
+                    };
+                    const float top = masked ? pass1(Yes{}) : pass1(No{});
+                    if (b > 0) {  // P V of the block before, while S waited
+                        if (!(ok = wait(&ctl.pv_full[mt], (n - 1) & 1))) break;
+                        saw_bad(blocks - 1);
+                        add_pv();
+                    }
+                    alpha = move(top, 0.f);
+                    const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
+                    auto pass2 = [&](auto mask) {
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+                            float x[32];
+                            fetch(g, x, mask);
+                            weigh(g, x, base, mask);
+                        }
+                    };
+                    if (masked) pass2(Yes{}); else pass2(No{});
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 umma::fence_before_sync();
                 bulk::mbar_arrive(&ctl.p_full[mt]);
-                if (MT == 2) {
-                    ok = wait_warp(&ctl.pv_full[mt], n & 1);
-                    if (!ok) break;
-                    add_pv(blocks);
-                }
             }
             if (!ok) break;
-            if (MT == 1) {
-                ok = wait_warp(&ctl.pv_full[mt], (n - 1) & 1);
-                if (!ok) break;
-                add_pv(blocks - 1);
-            }
-            // infinities and NaN that were taken out of blocks whose rows differ in what they see
-            if (FMT != LAI_KV_I8 && bad) {
-                for (int j = max(it.blk0 * kU, it.tl.k0); j < min(it.blk1 * kU, it.tl.k1); j++) {
-                    if (!it.mixed(a, j / kU, first, last) || j > row_pos || j <= row_from) continue;
+            // the last P V: one commit per item with two tiles, one per block with one
+            if (!(ok = wait(&ctl.pv_full[mt], (MT == 2 ? n_items++ : n - 1) & 1))) break;
+            umma::fence_after_sync();
+            saw_bad(blocks - 1);
+            if (MT == 1) add_pv();
+            // columns 32 g .. of the output row, before the division
+            auto piece = [&](int g, float (&x)[32]) {
+                if constexpr (MT == 2) {
+                    uint32_t u[32];
+                    __syncwarp();
+                    umma::tmem_ld_32x32b_x32(t_pv + 32 * g, u);
+                    umma::tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = __uint_as_float(u[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = o[(32 * g + i) % kKeep];
+                }
+                // infinities and NaN that were taken out of blocks whose rows differ in what they see
+                const int jend = FMT != LAI_KV_I8 && bad ? min(it.blk1 * kU, it.tl.k1) : 0;
+                for (int j = max(it.blk0 * kU, it.tl.k0); j < jend; j++) {
+                    if (!it.mixed(a, j / kU * kU, kU) || j > row_pos || j <= row_from) continue;
                     const int page = __ldg(a.kv.pages + (int64_t)it.tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
                     if (page < 0 || page >= a.kv.n_pages) continue;
-                    const int64_t at = (a.kv.page_base(page, it.head) + (j & (a.kv.page_size() - 1))) * HD;
+                    const int64_t at = (a.kv.page_base(page, it.head) + (j & in_page)) * HD + 32 * g;
 #pragma unroll
-                    for (int d = 0; d < HD; d++) {
-                        const float v = element<FMT>(a.kv.v, at + d);
-                        if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[d] += v;
+                    for (int i = 0; i < 32; i++) {
+                        const float v = element<FMT>(a.kv.v, at + i);
+                        if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) x[i] += v;
                     }
                 }
-            }
-            if (kF16) {  // back to plain units for the join: weights relative to exp2(m) alone
-                const float unit = pow2i(ve);
-                l *= unit;
-#pragma unroll
-                for (int d = 0; d < HD; d++) o[d] *= unit;
-            }
-            bool write = it.begins && it.ends;
-            if (!write) {
-                // parts: [row] max, [row] sum, then [d / 4][row][4]
-                constexpr int64_t kPart = (int64_t)R * (HD + 2);
-                float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * kPart;
-                pp[r] = m;
-                pp[R + r] = l;
-#pragma unroll
-                for (int d = 0; d < HD; d += 4)
-                    *reinterpret_cast<float4 *>(pp + 2 * R + ((d / 4) * R + r) * 4) =
-                        make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-                __threadfence();
-                if (!(ok = join())) break;
-                const int c0 = cta_of(it.w, it.item0), c1 = cta_of(it.w, it.item1 - 1);
-                if (wt == 0) ctl.last[mt] = atomicAdd(a.counters + c0 * MT + mt, 1) == c1 - c0;
-                if (!(ok = join())) break;
-                write = *(volatile int *)&ctl.last[mt];
-                if (write) {
-                    __threadfence();
-                    if (wt == 0) a.counters[c0 * MT + mt] = 0;  // ready for the next call
-                    m = neg_inf();
-                    l = 0.f;
-#pragma unroll
-                    for (int d = 0; d < HD; d++) o[d] = 0.f;
-                    for (int cc = c0; cc <= c1; cc++) {
-                        const float *pc = a.parts + ((int64_t)cc * 2 + (cc == c0 ? 1 : 0)) * kPart;
-                        const float cm = __ldcg(pc + r), mx = fmaxf(m, cm);
-                        const float mu = mx == neg_inf() ? 0.f : mx;
-                        const float ca = ex2(m - mu), cb = ex2(cm - mu);
-                        l = fmaf(__ldcg(pc + R + r), cb, l * ca);
-                        m = mx;
-#pragma unroll
-                        for (int d = 0; d < HD; d += 4) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * R + ((d / 4) * R + r) * 4));
-                            o[d] = fmaf(v.x, cb, o[d] * ca);
-                            o[d + 1] = fmaf(v.y, cb, o[d + 1] * ca);
-                            o[d + 2] = fmaf(v.z, cb, o[d + 2] * ca);
-                            o[d + 3] = fmaf(v.w, cb, o[d + 3] * ca);
-                        }
-                    }
-                }
-            }
-            if (write && row_ok) {
-                const int64_t at = (((int64_t)it.tl.q_row0 + tok) * ((int64_t)a.kv.n_kv * a.group) +
-                                    it.head * a.group + (fr - tok * a.group)) * HD;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+            };
+            const int64_t dst = (((int64_t)it.tl.q_row0 + tok) * ((int64_t)a.kv.n_kv * a.group) + row_head) * HD;
+            auto store = [&](int g, const float (&x)[32], float inv) {
+                if (!row_ok) return;
                 if (QF32) {
-                    float *dst = static_cast<float *>(out) + at;
+                    float *to = static_cast<float *>(out) + dst + 32 * g;
 #pragma unroll
-                    for (int d = 0; d < HD; d += 4)
-                        *reinterpret_cast<float4 *>(dst + d) =
-                            make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4 *>(to + i) =
+                            make_float4(x[i] * inv, x[i + 1] * inv, x[i + 2] * inv, x[i + 3] * inv);
                 } else {
-                    uint16_t *dst = static_cast<uint16_t *>(out) + at;
+                    uint16_t *to = static_cast<uint16_t *>(out) + dst + 32 * g;
 #pragma unroll
-                    for (int d = 0; d < HD; d += 8) {
-                        const float y[8] = {o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv,
-                                            o[d + 4] * inv, o[d + 5] * inv, o[d + 6] * inv, o[d + 7] * inv};
-                        st_vec(dst + d, pack<uint16_t>(y));
+                    for (int i = 0; i < 32; i += 8) {
+                        const float y[8] = {x[i] * inv, x[i + 1] * inv, x[i + 2] * inv, x[i + 3] * inv,
+                                            x[i + 4] * inv, x[i + 5] * inv, x[i + 6] * inv, x[i + 7] * inv};
+                        st_vec(to + i, pack<uint16_t>(y));
                     }
                 }
+            };
+            if (it.begins && it.ends) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                for (int g = 0; g < HD / 32; g++) {
+                    float x[32];
+                    piece(g, x);
+                    store(g, x, inv);
+                }
+                umma::fence_before_sync();
+                continue;
+            }
+            // parts: [row] off, [row] sum, then [d / 4][row][4]
+            constexpr int64_t kPart = (int64_t)R * (HD + 2);
+            float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * kPart;
+            pp[r] = off;
+            pp[R + r] = l;
+#pragma unroll
+            for (int g = 0; g < HD / 32; g++) {
+                float x[32];
+                piece(g, x);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<float4 *>(pp + 2 * R + ((8 * g + i / 4) * R + r) * 4) =
+                        make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+            }
+            umma::fence_before_sync();
+            __threadfence();
+            if (!(ok = join())) break;
+            const int c0 = cta_of(range, it.item0), c1 = cta_of(range, it.item1 - 1);
+            if (wt == 0) ctl.last[mt] = atomicAdd(a.counters + c0 * MT + mt, 1) == c1 - c0;
+            if (!(ok = join())) break;
+            if (!*(volatile int *)&ctl.last[mt]) continue;
+            __threadfence();
+            if (wt == 0) a.counters[c0 * MT + mt] = 0;  // ready for the next call
+            auto part = [&](int cc) { return a.parts + ((int64_t)cc * 2 + (cc == c0 ? 1 : 0)) * kPart; };
+            float top = neg_inf();
+            for (int cc = c0; cc <= c1; cc++) top = fmaxf(top, __ldcg(part(cc) + r));
+            const float mu = top == neg_inf() ? 0.f : top;
+            float sum = 0.f;
+            for (int cc = c0; cc <= c1; cc++) sum = fmaf(__ldcg(part(cc) + R + r), ex2(__ldcg(part(cc) + r) - mu), sum);
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+            for (int g = 0; g < HD / 32; g++) {
+                float x[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) x[i] = 0.f;
+                for (int cc = c0; cc <= c1; cc++) {
+                    const float *pc = part(cc);
+                    const float f = ex2(__ldcg(pc + r) - mu);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * R + ((8 * g + i / 4) * R + r) * 4));
+                        x[i] = fmaf(v.x, f, x[i]);
+                        x[i + 1] = fmaf(v.y, f, x[i + 1]);
+                        x[i + 2] = fmaf(v.z, f, x[i + 2]);
+                        x[i + 3] = fmaf(v.w, f, x[i + 3]);
+                    }
+                }
+                store(g, x, inv);
             }
         }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     }
     umma::fence_before_sync();
     __syncthreads();
@@ -775,10 +858,38 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a)
     if (warp == 12) umma::tmem_dealloc(tmem, 512);
 }
 
+// The cache as rows of head_dim BF16 values, copied 16 rows x 64 columns at a time.
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                 CUtensorMapFloatOOBfill);
+EncodeTiled encode_fn() {
+    static std::once_flag once;
+    static EncodeTiled fn = nullptr;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiled>(p);
+    });
+    return fn;
+}
+bool row_map(CUtensorMap *m, unsigned char *base, int64_t rows, int hd) {
+    const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
+    const cuuint32_t box[2] = {64, kGroup}, es[2] = {1, 1};
+    const EncodeTiled fn = encode_fn();
+    return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int HD, int FMT, bool QF32>
 int launch_wide(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
     using C = Cfg<HD, FMT, QF32>;
-    constexpr size_t kSmem = (size_t)(C::MT * C::kTerms + C::kStages) * C::kTile + sizeof(Ctl<HD, FMT, QF32>);
+    constexpr size_t kSmem = (size_t)(C::MT * C::kTerms + C::kStages) * C::kTile +
+                             (size_t)C::kRaw * C::kRawTile + sizeof(Ctl<HD, FMT, QF32>);
     static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
     auto kern = paged_attn_wide_kernel<HD, FMT, QF32>;
     // the warpgroups' register shares (setmaxnreg) add up to what the block is launched with
@@ -786,7 +897,13 @@ int launch_wide(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
     if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || fa.numRegs != 128) return LAI_ERR_CUDA;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
         return LAI_ERR_CUDA;
-    launch_pdl(kern, dim3(kSMs), dim3(kThreads), kSmem, st, out, q, a);
+    CUtensorMap maps[2] = {};
+    if (FMT == LAI_KV_BF16) {
+        const int64_t rows = (a.kv.n_pages * a.kv.n_kv) << a.kv.log_page;
+        if (rows > INT32_MAX) return LAI_ERR_RANGE;  // 32-bit coordinates
+        if (!row_map(&maps[0], a.kv.k, rows, HD) || !row_map(&maps[1], a.kv.v, rows, HD)) return LAI_ERR_CUDA;
+    }
+    launch_pdl(kern, dim3(kSMs), dim3(kThreads), kSmem, st, out, q, a, maps[0], maps[1]);
     return launch_status();
 }
 

@@ -553,7 +553,7 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
     a.parts = reinterpret_cast<float *>(a.counters + kCounters);
     a.err = err;
     const cudaStream_t cs = as_stream(stream);
-    if (n_rows * a.group > (int64_t)kWideRows * b->n_seqs && a.scale_log2 >= 0.f)
+    if (n_rows * a.group > (int64_t)kWideRows * b->n_seqs && a.scale_log2 > 1e-30f)
         return attention_wide(out, q, QF32, kv->head_dim, kv->format, a, cs);
 #define LAI_FEW(FMT)                                                      \
     if (kv->head_dim == 128) launch_few<128, FMT, QF32>(out, q, a, cs);   \

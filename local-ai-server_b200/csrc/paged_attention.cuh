@@ -233,7 +233,7 @@ struct Walk {
     }
 };
 
-// The kernel for many rows per sequence (paged_attention_wide.cu), scale_log2 >= 0: LAI_OK or an
+// The kernel for many rows per sequence (paged_attention_wide.cu), scale_log2 > 0: LAI_OK or an
 // error; and the F32 values of scratch it needs.
 int attention_wide(void *out, const void *q, bool f32, int head_dim, int format, const AttnArgs &a,
                    cudaStream_t st);

@@ -39,6 +39,7 @@ constexpr int kGroup = 16;     // keys per copy
 constexpr int kRing = 4;       // blocks whose scales and flags are kept
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kGrow = 8.f;   // log2 of how far weights may pass 1 before O is rescaled
+constexpr int kPolyOf8 = 3;    // of 8 exponentials, those that the FMA pipe takes
 
 template <int HD, int FMT, bool QF32>
 struct Cfg {
@@ -63,7 +64,7 @@ struct Ctl {
     float kscale[kRing][kScales], vscale[kRing][kScales];  // 16-byte aligned
     uint64_t landed[C::kLand], taken[C::kLand], full[C::kStages], empty[C::kStages];
     uint64_t info[kRing];
-    uint64_t q_full[2], s_full[2], p_full[2], pv_full[2], group[2];
+    uint64_t q_full[2], s_full[2], p_full[2][2], pv_full[2], group[2];
     int vexp[kRing][4];
     int groups[kRing];  // bit i: 16-key group i of the block lies in a real page
     int vbad[kRing];    // the block (counted) from whose V infinities or NaN were taken out
@@ -164,6 +165,30 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar))
         : "memory");
 }
+// The largest of three, NaN if one of them is.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+// 2^y for y <= 127, below 2^-126 as 2^-126: n = round(y), and on [-1/2, 1/2] the cubic with the
+// smallest relative error, 7.5e-5 (2^-13.7; the weights are rounded to 2^-9 or 2^-12 after it).
+// It runs on the FMA pipe, where there is room beside the exponential unit (16 a cycle and SM),
+// which bounds the softmax otherwise.
+__device__ __forceinline__ float2 exp2_poly(float2 y) {
+    const float kBig = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+    const float2 big = make_float2(kBig, kBig), nbig = make_float2(-kBig, -kBig);
+    y = make_float2(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
+    const float2 n = __fadd2_rn(y, big);
+    const float2 r = __fadd2_rn(n, nbig);
+    const float2 f = __fadd2_rn(y, make_float2(-r.x, -r.y));
+    float2 p = __ffma2_rn(make_float2(0.05517167f, 0.05517167f), f, make_float2(0.24261112f, 0.24261112f));
+    p = __ffma2_rn(p, f, make_float2(0.69326099f, 0.69326099f));
+    p = __ffma2_rn(p, f, make_float2(0.99992807f, 0.99992807f));
+    // p is within a factor of 2 of 1: adding n to its exponent cannot pass zero or infinity
+    return make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + __float_as_uint(p.x)),
+                       __uint_as_float((__float_as_uint(n.y) << 23) + __float_as_uint(p.y)));
+}
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
@@ -228,7 +253,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             bulk::mbar_init(&ctl.q_full[i], 128);
             bulk::mbar_init(&ctl.group[i], 128);
             bulk::mbar_init(&ctl.s_full[i], 1);
-            bulk::mbar_init(&ctl.p_full[i], 128);
+            bulk::mbar_init(&ctl.p_full[i][0], 128);
+            bulk::mbar_init(&ctl.p_full[i][1], 128);
             bulk::mbar_init(&ctl.pv_full[i], 1);
         }
         ctl.abort = 0;
@@ -282,6 +308,15 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         uint32_t idx = 0, blocks = 0;  // operand tiles, blocks so far
         bool ok = true;
         while (ok && it.next(a)) {
+            for (int r = lane; r < it.tl.rows; r += 32) {  // the item's queries on their way to L2
+                const int fr = it.tl.row0 + r, tok = fr / a.group;
+                const char *q = static_cast<const char *>(qp) +
+                                (((int64_t)it.tl.q_row0 + tok) * a.ld_q +
+                                 (int64_t)(it.head * a.group + (fr - tok * a.group)) * HD) * (QF32 ? 4 : 2);
+#pragma unroll
+                for (int i = 0; i < HD * (QF32 ? 4 : 2); i += 128)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
+            }
             for (int blk = it.blk0; ok && blk < it.blk1; blk++, blocks++) {
                 const int j0 = blk * kU;
                 const int page = page_of(j0);
@@ -339,7 +374,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     flag(a.err, LAI_DEVERR_PAGE);
                 const uint32_t groups = __ballot_sync(0xffffffffu, page >= 0);
                 const bool whole = groups == 0xff && j0 >= it.tl.k0 && j0 + kU <= it.tl.k1;
-                const bool mixed = FMT != LAI_KV_I8 && it.mixed(a, j0, kU);
+                const bool mixed = it.mixed(a, j0, kU);
                 auto there = [&](int r) {
                     return j0 + r >= it.tl.k0 && j0 + r < it.tl.k1 && (groups >> (r / kGroup) & 1);
                 };
@@ -351,7 +386,12 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         if (kF16) {
                             const float vs = there(wt) ? ctl.vscale[slot][kF16 ? wt : 0] : 0.f;
                             const uint32_t u = __float_as_uint(vs) & 0x7fffffffu;
-                            const uint32_t top = __reduce_max_sync(0xffffffffu, u < 0x7f800000u ? u : 0u);
+                            const bool fine = u < 0x7f800000u;
+                            if (!whole || mixed) {  // weight 0 times a scale has to be 0
+                                ctl.vscale[slot][kF16 ? wt : 0] = mixed && !fine ? 0.f : vs;
+                                if (mixed && !fine) ctl.vbad[slot] = (int)blocks;
+                            }
+                            const uint32_t top = __reduce_max_sync(0xffffffffu, fine ? u : 0u);
                             if (lane == 0) ctl.vexp[slot][wt >> 5] = (int)(top >> 23) - 127;
                         }
                         if (wt == 0) ctl.groups[slot] = (int)groups;
@@ -375,7 +415,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                                                   half2_of<FMT, false>(raw.y), half2_of<FMT, true>(raw.y));
                             uint4 hi = make_uint4(half2_of<FMT, false>(raw.z), half2_of<FMT, true>(raw.z),
                                                   half2_of<FMT, false>(raw.w), half2_of<FMT, true>(raw.w));
-                            if (mixed && kv) {
+                            if (FMT == LAI_KV_E4M3 && mixed && kv) {
                                 bad |= drop_nonfinite<true>(lo.x) | drop_nonfinite<true>(lo.y) |
                                        drop_nonfinite<true>(lo.z) | drop_nonfinite<true>(lo.w);
                                 bad |= drop_nonfinite<true>(hi.x) | drop_nonfinite<true>(hi.y) |
@@ -453,24 +493,33 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 const uint32_t vi = idx + 1, ki = idx + 2;
                 const bool more = b + 1 < nb;
                 for (int mt = 0; ok && mt < tiles; mt++) {
-                    if (!(ok = wait(&ctl.p_full[mt], n_mt[mt]++ & 1))) break;
-                    if (MT == 1 && more) {  // the next scores while P V waits for V
+                    const uint64_t vd = desc_mnmajor(smem_addr(st_smem + (vi % ST) * C::kTile));
+                    // keys 64 h .. of the block, once their weights are there
+                    auto values = [&](int h) {
+                        if (leader) {
+#pragma unroll
+                            for (int t = kTerms - 1; t >= 0; t--)
+#pragma unroll
+                                for (int k = 0; k < kU / 32; k++)
+                                    mma_ts(tmem + kPV + mt * 128, tmem + kP + mt * 128 + t * 64 + (h * 4 + k) * 8,
+                                           vd + (((h * 4 + k) * 2048) >> 4), kIdO,
+                                           (MT == 2 && b > 0) || h || t != kTerms - 1 || k);
+                        }
+                        __syncwarp();
+                    };
+                    const uint32_t parity = n_mt[mt]++ & 1;
+                    if (!(ok = wait(&ctl.p_full[mt][0], parity))) break;
+                    if (!(ok = wait(&ctl.full[vi % ST], (vi / ST) & 1))) break;
+                    umma::fence_after_sync();
+                    values(0);
+                    if (!(ok = wait(&ctl.p_full[mt][1], parity))) break;
+                    umma::fence_after_sync();
+                    if (MT == 1 && more) {  // the next scores before the rest of P V
                         if (!(ok = wait(&ctl.full[ki % ST], (ki / ST) & 1))) break;
                         umma::fence_after_sync();
                         scores(mt, ki);
                     }
-                    if (!(ok = wait(&ctl.full[vi % ST], (vi / ST) & 1))) break;
-                    umma::fence_after_sync();
-                    const uint64_t vd = desc_mnmajor(smem_addr(st_smem + (vi % ST) * C::kTile));
-                    if (leader) {
-#pragma unroll
-                        for (int t = kTerms - 1; t >= 0; t--)
-#pragma unroll
-                            for (int k = 0; k < kU / 16; k++)
-                                mma_ts(tmem + kPV + mt * 128, tmem + kP + mt * 128 + t * 64 + k * 8,
-                                       vd + ((k * 2048) >> 4), kIdO,
-                                       (MT == 2 && b > 0) || t != kTerms - 1 || k);
-                    }
+                    values(1);
                     if (MT == 1 || !more) commit(&ctl.pv_full[mt]);
                     if (MT == 2 && more) {
                         if (!(ok = wait(&ctl.full[ki % ST], (ki / ST) & 1))) break;
@@ -508,65 +557,81 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 continue;
             }
             const int r = mt * 128 + wt, fr = it.tl.row0 + r, tok = fr / a.group;
-            const bool row_ok = r < it.tl.rows;
-            const int row_pos = row_ok ? it.tl.pos0 + tok : -1;
+            const int row_pos = it.tl.pos0 + tok;  // of a row behind the last: not stored
             const int row_from = a.window ? row_pos - a.window : -1;  // sees (row_from, row_pos]
-            const int row_head = it.head * a.group + (fr - tok * a.group);
+            // Q into shared memory, the warp's own 32 rows; the last scores of the item before are
+            // done. kLanes lanes take a row, so that a load reads whole lines.
+            const uint32_t my_rows = smem_addr(q_smem) + mt * C::kTile;  // this tile of the first term
+            const int wrow = (warp & 3) * 32;                            // the warp's first row of it
+            constexpr int kElem = QF32 ? 4 : 2, kLanes = HD * kElem / 16, kAtOnce = 32 / kLanes;
+            const int run = lane % kLanes, sub = lane / kLanes;
             float c = a.scale_log2;
-            {  // this row of Q into shared memory; the last scores of the item before are done
-                const int64_t at = ((int64_t)it.tl.q_row0 + tok) * a.ld_q + (int64_t)row_head * HD;
-                const uint32_t dst = smem_addr(q_smem) + mt * C::kTile;
-                constexpr int kRuns = QF32 ? HD / 4 : HD / 8;
-                uint4 raw[kRuns];
-                const uint4 *src = reinterpret_cast<const uint4 *>(
-                    QF32 ? (const void *)(static_cast<const float *>(qp) + at)
-                         : (const void *)(static_cast<const uint16_t *>(qp) + at));
+            {
+                constexpr int kBatch = 16 < 32 / kAtOnce ? 16 : 32 / kAtOnce;
+#pragma unroll 1
+                for (int p0 = 0; p0 < 32 / kAtOnce; p0 += kBatch) {
+                    uint4 raw[kBatch];
 #pragma unroll
-                for (int i = 0; i < kRuns; i++) raw[i] = row_ok ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-                float up = 1.f;
-                if (kF16) {  // the row's largest into [2^13, 2^14)
-                    uint32_t top = 0;
+                    for (int p = 0; p < kBatch; p++) {
+                        const int rr = (p0 + p) * kAtOnce + sub, f = it.tl.row0 + mt * 128 + wrow + rr, tk = f / a.group;
+                        raw[p] = make_uint4(0, 0, 0, 0);
+                        if (mt * 128 + wrow + rr < it.tl.rows)
+                            raw[p] = __ldg(reinterpret_cast<const uint4 *>(
+                                static_cast<const char *>(qp) +
+                                (((int64_t)it.tl.q_row0 + tk) * a.ld_q +
+                                 (int64_t)(it.head * a.group + (f - tk * a.group)) * HD) * kElem + run * 16));
+                    }
 #pragma unroll
-                    for (int i = 0; i < kRuns; i++) {
-                        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    for (int p = 0; p < kBatch; p++) {
+                        const int rr = (p0 + p) * kAtOnce + sub;
+                        float up = 1.f;
+                        if (kF16) {  // the row's largest into [2^13, 2^14)
+                            const uint32_t w[4] = {raw[p].x, raw[p].y, raw[p].z, raw[p].w};
+                            uint32_t top = 0;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if (QF32) top = max(top, w[e] & 0x7fffffffu);
-                            else top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
+                            for (int e = 0; e < 4; e++) {
+                                if (QF32) top = max(top, w[e] & 0x7fffffffu);
+                                else top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
+                            }
+#pragma unroll
+                            for (int o = kLanes / 2; o > 0; o >>= 1)
+                                top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            const int e = (int)(top >> 23) - 127;
+                            up = pow2i(13 - e);
+                            // the thread that owns the row keeps the other side of the scaling
+                            const int mine = __shfl_sync(0xffffffffu, e, lane % kAtOnce * kLanes);
+                            if (lane / kAtOnce == p0 + p) c = a.scale_log2 * pow2i(mine - 13);
+                        }
+                        if constexpr (QF32) {  // 4 values: half a 16-byte run of every term
+                            float x[4] = {__uint_as_float(raw[p].x), __uint_as_float(raw[p].y),
+                                          __uint_as_float(raw[p].z), __uint_as_float(raw[p].w)};
+#pragma unroll
+                            for (int e = 0; e < 4; e++) x[e] *= up;
+#pragma unroll
+                            for (int t = 0; t < kTerms; t++) {
+                                const uint32_t lo = take2<kF16>(x[0], x[1]), hi = take2<kF16>(x[2], x[3]);
+                                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(
+                                                 my_rows + t * MT * C::kTile + chunk_off(wrow + rr, run / 2) + run % 2 * 8),
+                                             "r"(lo), "r"(hi)
+                                             : "memory");
+                            }
+                        } else {
+                            uint4 v = raw[p];
+                            if (kF16) {
+                                float x[8];
+                                unpack<uint16_t>(v, x);
+#pragma unroll
+                                for (int e = 0; e < 8; e++) x[e] *= up;
+                                v.x = pack2<true>(x[0], x[1]);
+                                v.y = pack2<true>(x[2], x[3]);
+                                v.z = pack2<true>(x[4], x[5]);
+                                v.w = pack2<true>(x[6], x[7]);
+                            }
+                            st_shared16(my_rows + chunk_off(wrow + rr, run), v);
                         }
                     }
-                    const int e = (int)(top >> 23) - 127;
-                    up = pow2i(13 - e);
-                    c *= pow2i(e - 13);
                 }
-#pragma unroll
-                for (int d = 0; d < HD / 8; d++) {
-                    if (!kF16 && !QF32) {
-                        st_shared16(dst + chunk_off(wt, d), raw[d]);
-                        continue;
-                    }
-                    float x[8];
-                    if (QF32) {
-                        const uint4 u = raw[(2 * d) % kRuns], v = raw[(2 * d + 1) % kRuns];
-                        const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = __uint_as_float(w[e]);
-                    } else {
-                        unpack<uint16_t>(raw[d], x);
-                    }
-                    if (kF16)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] *= up;
-#pragma unroll
-                    for (int t = 0; t < kTerms; t++) {
-                        uint4 v;
-                        v.x = take2<kF16>(x[0], x[1]);
-                        v.y = take2<kF16>(x[2], x[3]);
-                        v.z = take2<kF16>(x[4], x[5]);
-                        v.w = take2<kF16>(x[6], x[7]);
-                        st_shared16(dst + t * MT * C::kTile + chunk_off(wt, d), v);
-                    }
-                }
+                c = fmaxf(c, 1.2e-38f);  // masked scores, -inf, stay -inf
                 bulk::fence_proxy_async_smem();
                 bulk::mbar_arrive(&ctl.q_full[mt]);
             }
@@ -580,7 +645,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
 #pragma unroll
             for (int d = 0; d < kKeep; d++) o[d] = 0.f;
             auto saw_bad = [&](uint32_t block) {
-                if (FMT != LAI_KV_I8) bad |= *(volatile int *)&ctl.vbad[block % kRing] == (int)block;
+                bad |= *(volatile int *)&ctl.vbad[block % kRing] == (int)block;
             };
             auto add_pv = [&]() {
                 umma::fence_after_sync();
@@ -601,75 +666,82 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 umma::fence_after_sync();
                 if (MT == 2 && b > 0) saw_bad(blocks - 1);  // its P V came before these scores
                 const int groups = ctl.groups[slot];
-                // element i of the block is seen where lo <= i <= hi
-                const int hi = row_pos - j0, lo = row_from + 1 - j0;
                 const bool masked = groups != 0xff || j0 + kU - 1 > it.first || it.tl.k0 > j0 ||
-                                    (a.window && j0 <= it.last - a.window) || it.tl.rows < mt * 128 + 128;
-                auto seen = [&](int i) { return i <= hi && i >= lo && (groups >> (i / kGroup) & 1); };
+                                    (a.window && j0 <= it.last - a.window);
+                // the row sees keys j0 + lo .. j0 + hi, as bits of 32 keys
+                const int hi = row_pos - j0, lo = row_from + 1 - j0;
+                auto seen = [&](int g) -> uint32_t {
+                    const int h = min(max(hi + 1 - 32 * g, 0), 32), l = min(max(lo - 32 * g, 0), 32);
+                    const uint32_t below_h = h == 32 ? 0xffffffffu : (1u << h) - 1;
+                    const uint32_t below_l = l == 32 ? 0xffffffffu : (1u << l) - 1;
+                    const uint32_t real = (groups >> (2 * g) & 1 ? 0xffffu : 0u) | (groups >> (2 * g + 1) & 1 ? 0xffff0000u : 0u);
+                    return below_h & ~below_l & real;
+                };
                 const float4 *k4 = reinterpret_cast<const float4 *>(ctl.kscale[slot]);
                 const float4 *v4 = reinterpret_cast<const float4 *>(ctl.vscale[slot]);
                 if (kF16) {
                     const int *e4 = ctl.vexp[slot];
                     ve = min(max(max(max(e4[0], e4[1]), max(e4[2], e4[3])), ve), 90);
                 }
-                // scores of 32 keys, scaled by their keys' scales and masked
-                auto fetch = [&](int g, float *x, auto mask) {
-                    uint32_t u[32];
-                    umma::tmem_ld_32x32b_x32(t_s + 32 * g, u);
-                    umma::tmem_wait_ld();
+                // 32 scores with their keys' scales, masked; the maximum so far
+                auto scale32 = [&](int g, float2 *x, float &top, auto mask) {
+                    const uint32_t see = decltype(mask)::value ? seen(g) : 0u;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        float4 ks = make_float4(1.f, 1.f, 1.f, 1.f);
-                        if (kF16) ks = k4[kF16 ? 8 * g + i / 4 : 0];
-                        const float s4[4] = {ks.x, ks.y, ks.z, ks.w};
-#pragma unroll
-                        for (int h = 0; h < 4; h++) {
-                            float v = __uint_as_float(u[i + h]);
-                            if (kF16) v *= s4[h];
-                            if (decltype(mask)::value) v = seen(32 * g + i + h) ? v : neg_inf();
-                            x[i + h] = v;
+                    for (int i = 0; i < 16; i += 2) {
+                        if (kF16) {
+                            const float4 ks = k4[kF16 ? 8 * g + i / 2 : 0];
+                            x[i] = __fmul2_rn(x[i], make_float2(ks.x, ks.y));
+                            x[i + 1] = __fmul2_rn(x[i + 1], make_float2(ks.z, ks.w));
                         }
-                    }
-                };
-                auto max_of = [&](const float *x, float &t0, float &t1) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        t0 = fmaxf(t0, fmaxf(x[i], x[i + 1]));
-                        t1 = fmaxf(t1, fmaxf(x[i + 2], x[i + 3]));
+                        for (int h = 0; h < 2; h++) {
+                            if (decltype(mask)::value) {
+                                x[i + h].x = see >> (2 * (i + h)) & 1 ? x[i + h].x : neg_inf();
+                                x[i + h].y = see >> (2 * (i + h) + 1) & 1 ? x[i + h].y : neg_inf();
+                            }
+                            top = max3(top, x[i + h].x, x[i + h].y);
+                        }
                     }
                 };
                 // weights of 32 keys, into P
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                auto weigh = [&](int g, const float *x, float base, auto mask) {
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                const float2 c2 = make_float2(c, c);
+                auto weigh = [&](int g, const float2 *x, float base, auto mask) {
                     uint32_t w[kTerms][16];
+                    const float2 nb2 = make_float2(-base, -base);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
+                    for (int i = 0; i < 16; i += 2) {
                         float4 vs = make_float4(1.f, 1.f, 1.f, 1.f);
-                        if (kF16) vs = v4[kF16 ? 8 * g + i / 4 : 0];
-                        const float s4[4] = {vs.x, vs.y, vs.z, vs.w};
-                        float p[4];
+                        if (kF16) vs = v4[kF16 ? 8 * g + i / 2 : 0];
 #pragma unroll
-                        for (int h = 0; h < 4; h++) {
-                            // a masked score is -inf, also after its product with c = 0
-                            p[h] = ex2(fmaf(x[i + h], c, -base));
-                            if (decltype(mask)::value) p[h] = seen(32 * g + i + h) ? p[h] : 0.f;
-                            sum[h] += p[h];
-                            if (kF16) {
-                                p[h] *= s4[h];
-                                if (decltype(mask)::value) p[h] = seen(32 * g + i + h) ? p[h] : 0.f;
-                            }
-                        }
+                        for (int h = 0; h < 2; h++) {
+                            float2 p = __ffma2_rn(x[i + h], c2, nb2);
+                            // (a masked score's weight must be exactly 0, and F32 results exact)
+                            if (!QF32 && !decltype(mask)::value && ((i + h) * kPolyOf8 & 7) < kPolyOf8)
+                                p = exp2_poly(p);
+                            else
+                                p = make_float2(ex2(p.x), ex2(p.y));
+                            sum[h] = __fadd2_rn(sum[h], p);
+                            if (kF16) p = __fmul2_rn(p, h ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y));
 #pragma unroll
-                        for (int t = 0; t < kTerms; t++) {
-                            w[t][i / 2] = take2<kF16>(p[0], p[1]);
-                            w[t][i / 2 + 1] = take2<kF16>(p[2], p[3]);
+                            for (int t = 0; t < kTerms; t++) w[t][i + h] = take2<kF16>(p.x, p.y);
                         }
                     }
 #pragma unroll
                     for (int t = 0; t < kTerms; t++) tmem_st_x16(t_p + t * 64 + 16 * g, w[t]);
+                    if (g & 1) {  // half of P is there
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        umma::fence_before_sync();
+                        bulk::mbar_arrive(&ctl.p_full[mt][g >> 1]);
+                    }
+                };
+                auto fetch = [&](int g, float2 *x) {  // without waiting
+                    umma::tmem_ld_32x32b_x32(t_s + 32 * g, *reinterpret_cast<uint32_t (*)[32]>(x));
                 };
                 // moves off to the block's maximum; what l and O must be multiplied with
                 auto move = [&](float top, float slack) -> float {
+                    // an infinite or NaN score: no weight of this row means anything any more
+                    if (!(top < __int_as_float(0x7f800000))) l = __int_as_float(0x7fffffff);
                     m = fmaxf(m, top == neg_inf() ? top : top * c);
                     const float to = m + (float)ve;
                     if (!(to > off + slack)) return 1.f;
@@ -679,14 +751,15 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     return f;
                 };
                 if constexpr (MT == 2) {
-                    auto block = [&](auto mask) {
-                        float x[kU], t0 = neg_inf(), t1 = neg_inf();
+                    float2 x[kU / 2];
 #pragma unroll
-                        for (int g = 0; g < 4; g++) {
-                            fetch(g, x + 32 * g, mask);
-                            max_of(x + 32 * g, t0, t1);
-                        }
-                        const float f = move(fmaxf(t0, t1), kGrow);
+                    for (int g = 0; g < 4; g++) fetch(g, x + 16 * g);
+                    umma::tmem_wait_ld();
+                    auto block = [&](auto mask) {
+                        float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+                        for (int g = 0; g < 4; g++) scale32(g, x + 16 * g, top[g], mask);
+                        const float f = move(max3(max3(top[0], top[1], top[2]), top[3], top[3]), kGrow);
                         if (b > 0 && __any_sync(0xffffffffu, f != 1.f)) {
                             // the scores' MMAs came after the last P V, so O is complete
 #pragma unroll 1
@@ -701,19 +774,20 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         }
                         const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
 #pragma unroll
-                        for (int g = 0; g < 4; g++) weigh(g, x + 32 * g, base, mask);
+                        for (int g = 0; g < 4; g++) weigh(g, x + 16 * g, base, mask);
                     };
                     if (masked) block(Yes{}); else block(No{});
                 } else {
                     auto pass1 = [&](auto mask) {
-                        float t0 = neg_inf(), t1 = neg_inf();
+                        float top = neg_inf();
 #pragma unroll
                         for (int g = 0; g < 4; g++) {
-                            float x[32];
-                            fetch(g, x, mask);
-                            max_of(x, t0, t1);
+                            float2 x[16];
+                            fetch(g, x);
+                            umma::tmem_wait_ld();
+                            scale32(g, x, top, mask);
                         }
-                        return fmaxf(t0, t1);
+                        return top;
                     };
                     const float top = masked ? pass1(Yes{}) : pass1(No{});
                     if (b > 0) {  // P V of the block before, while S waited
@@ -724,19 +798,19 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     alpha = move(top, 0.f);
                     const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
                     auto pass2 = [&](auto mask) {
+                        float ignore = 0.f;
 #pragma unroll
                         for (int g = 0; g < 4; g++) {
-                            float x[32];
-                            fetch(g, x, mask);
+                            float2 x[16];
+                            fetch(g, x);
+                            umma::tmem_wait_ld();
+                            scale32(g, x, ignore, mask);
                             weigh(g, x, base, mask);
                         }
                     };
                     if (masked) pass2(Yes{}); else pass2(No{});
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                umma::fence_before_sync();
-                bulk::mbar_arrive(&ctl.p_full[mt]);
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             if (!ok) break;
             // the last P V: one commit per item with two tiles, one per block with one
@@ -758,37 +832,51 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     for (int i = 0; i < 32; i++) x[i] = o[(32 * g + i) % kKeep];
                 }
                 // infinities and NaN that were taken out of blocks whose rows differ in what they see
-                const int jend = FMT != LAI_KV_I8 && bad ? min(it.blk1 * kU, it.tl.k1) : 0;
+                const int jend = bad ? min(it.blk1 * kU, it.tl.k1) : 0;
                 for (int j = max(it.blk0 * kU, it.tl.k0); j < jend; j++) {
                     if (!it.mixed(a, j / kU * kU, kU) || j > row_pos || j <= row_from) continue;
                     const int page = __ldg(a.kv.pages + (int64_t)it.tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
                     if (page < 0 || page >= a.kv.n_pages) continue;
-                    const int64_t at = (a.kv.page_base(page, it.head) + (j & in_page)) * HD + 32 * g;
+                    const int64_t at = a.kv.page_base(page, it.head) + (j & in_page);
+                    const float vs = kF16 ? __ldg(a.kv.v_scale + at) : 1.f;
 #pragma unroll
                     for (int i = 0; i < 32; i++) {
-                        const float v = element<FMT>(a.kv.v, at + i);
+                        const float v = element<FMT>(a.kv.v, at * HD + 32 * g + i) * vs;
                         if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) x[i] += v;
                     }
                 }
             };
-            const int64_t dst = (((int64_t)it.tl.q_row0 + tok) * ((int64_t)a.kv.n_kv * a.group) + row_head) * HD;
-            auto store = [&](int g, const float (&x)[32], float inv) {
-                if (!row_ok) return;
+            // 32 columns of this thread's row into the warp's rows of the Q tile (the next item's Q
+            // is not there yet): F32 has half of its columns in the second term's tile
+            auto stage = [&](int g, const float (&x)[32], float inv) {
                 if (QF32) {
-                    float *to = static_cast<float *>(out) + dst + 32 * g;
+                    const uint32_t tile = my_rows + (g >= HD / 64 ? MT * C::kTile : 0);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4 *>(to + i) =
-                            make_float4(x[i] * inv, x[i + 1] * inv, x[i + 2] * inv, x[i + 3] * inv);
+                    for (int i = 0; i < 8; i++)
+                        st_shared16(tile + chunk_off(wt, (8 * g + i) % (HD / 8)),
+                                    make_uint4(__float_as_uint(x[4 * i] * inv), __float_as_uint(x[4 * i + 1] * inv),
+                                               __float_as_uint(x[4 * i + 2] * inv), __float_as_uint(x[4 * i + 3] * inv)));
                 } else {
-                    uint16_t *to = static_cast<uint16_t *>(out) + dst + 32 * g;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        const float y[8] = {x[i] * inv, x[i + 1] * inv, x[i + 2] * inv, x[i + 3] * inv,
-                                            x[i + 4] * inv, x[i + 5] * inv, x[i + 6] * inv, x[i + 7] * inv};
-                        st_vec(to + i, pack<uint16_t>(y));
+                    for (int i = 0; i < 4; i++) {
+                        const float y[8] = {x[8 * i] * inv, x[8 * i + 1] * inv, x[8 * i + 2] * inv, x[8 * i + 3] * inv,
+                                            x[8 * i + 4] * inv, x[8 * i + 5] * inv, x[8 * i + 6] * inv, x[8 * i + 7] * inv};
+                        st_shared16(my_rows + chunk_off(wt, 4 * g + i), pack<uint16_t>(y));
                     }
                 }
+            };
+            auto store = [&]() {  // the warp's staged rows, in whole lines
+                __syncwarp();
+#pragma unroll 4
+                for (int p = 0; p < 32 / kAtOnce; p++) {
+                    const int rr = p * kAtOnce + sub, f = it.tl.row0 + mt * 128 + wrow + rr, tk = f / a.group;
+                    if (mt * 128 + wrow + rr >= it.tl.rows) continue;
+                    const uint32_t tile = my_rows + (QF32 && run >= kLanes / 2 ? MT * C::kTile : 0);
+                    const uint4 v = ld_shared16(tile + chunk_off(wrow + rr, run % (HD / 8)));
+                    st_vec(static_cast<char *>(out) +
+                               ((((int64_t)it.tl.q_row0 + tk) * a.kv.n_kv + it.head) * a.group + (f - tk * a.group)) * (HD * kElem) + run * 16, v);
+                }
+                __syncwarp();
             };
             if (it.begins && it.ends) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -796,9 +884,10 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 for (int g = 0; g < HD / 32; g++) {
                     float x[32];
                     piece(g, x);
-                    store(g, x, inv);
+                    stage(g, x, inv);
                 }
                 umma::fence_before_sync();
+                store();
                 continue;
             }
             // parts: [row] off, [row] sum, then [d / 4][row][4]
@@ -848,8 +937,9 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         x[i + 3] = fmaf(v.w, f, x[i + 3]);
                     }
                 }
-                store(g, x, inv);
+                stage(g, x, inv);
             }
+            store();
         }
     }
     umma::fence_before_sync();

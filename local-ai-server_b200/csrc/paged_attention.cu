@@ -138,13 +138,13 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     it.start(a, range);
     while (it.next(a)) {
         const Tile &tl = it.tl;
-        const int head = it.head, blk0 = it.blk0, blk1 = it.blk1;
+        const int head = it.kv_head(), blk0 = it.blk0, blk1 = it.blk1;
 
         // the query: lane (g, t) holds row g's elements 4 at a time, hi in the MMA's row g and
         // the rest of it in row g + 8
         uint32_t qa[KS][kThird ? 6 : 4];
         float row_scale = a.scale_log2;
-        const int row = tl.row0 + g, tok = row / a.group;
+        const int row = tl.row0 + g, tok = a.by_group.of(row);
         const bool row_ok = g < tl.rows;
         const int row_pos = row_ok ? tl.pos0 + tok : -1;
         const int row_from = a.window ? row_pos - a.window : -1;  // sees keys in (row_from, row_pos]
@@ -450,7 +450,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
 #pragma unroll
                 for (int i = 0; i < kPer; i++) {
                     const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
-                    const int p = tl.pos0 + (tl.row0 + r) / a.group;
+                    const int p = tl.pos0 + a.by_group.of(tl.row0 + r);
                     if (r >= tl.rows || j > p || (a.window && j <= p - a.window)) continue;
                     const float v = element<FMT>(a.kv.v, at + d);
                     if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) acc[i] += v;
@@ -501,7 +501,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             for (int i = 0; i < kPer; i++) {
                 const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
                 if (r >= tl.rows) continue;
-                const int fr = tl.row0 + r, tk = fr / a.group;
+                const int fr = tl.row0 + r, tk = a.by_group.of(fr);
                 const int64_t at = (((int64_t)tl.q_row0 + tk) * n_heads + head * a.group +
                                     (fr - tk * a.group)) * HD + d;
                 const float x = jl_[i] == 0.f ? 0.f : acc[i] / jl_[i];
@@ -538,7 +538,7 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
         !aligned16(scratch))
         return LAI_ERR_INVALID;
     if (n_rows == 0 || b->n_seqs == 0) return LAI_OK;
-    if (n_rows * (n_heads / kv->n_kv_heads) + b->n_seqs > INT32_MAX / 2) return LAI_ERR_RANGE;
+    if (n_rows * (n_heads / kv->n_kv_heads) + b->n_seqs >= 1 << 28) return LAI_ERR_RANGE;
     const size_t ob = paged::row_bytes(n_rows, width, width, kEsize);
     const size_t qb = paged::row_bytes(n_rows, ld_q, width, kEsize);
     const size_t wb = lai_paged_attention_scratch_bytes(kv->head_dim);
@@ -546,6 +546,7 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
         overlaps(scratch, wb, out, ob) || overlaps(scratch, wb, q, qb))
         return LAI_ERR_ALIAS;
     a.group = n_heads / kv->n_kv_heads;
+    a.by_group = Div::by(a.group);
     a.window = window < (1 << 30) ? window : 0;  // positions are below 2^31: it masks nothing
     a.scale_log2 = scale * kLog2e;
     a.ld_q = ld_q;

@@ -31,9 +31,18 @@ __device__ __forceinline__ float pow2i(int e) {
     return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
 }
 
+// n / d for 0 <= n < 2^28 and d <= 16: m = ceil(2^32 / d) overshoots 2^32 / d by less than 1, so
+// n m / 2^32 overshoots n / d by less than n / 2^32 < 1 / 16.
+struct Div {
+    uint64_t m;
+    __host__ __device__ static Div by(int d) { return Div{((1ull << 32) + d - 1) / d}; }
+    __device__ __forceinline__ int of(int n) const { return (int)((uint64_t)(uint32_t)n * m >> 32); }
+};
+
 struct AttnArgs {
     View kv;
     int group;      // query heads per kv head
+    Div by_group;
     int window;     // 0: every earlier key
     float scale_log2;
     int64_t ld_q;
@@ -47,6 +56,7 @@ struct Tile {
     int seq, row0, q_row0;  // sequence, first flattened row in it, the sequence's first row
     int rows;               // real rows, 0: no item
     int pos0;               // position of new token 0
+    int first, last;        // positions of the tile's first and last row
     int k0, k1;             // keys any row sees
     int b0, blocks;         // first block, blocks (1 for a tile that sees no key)
 };
@@ -83,8 +93,10 @@ struct Sched {
         t.q_row0 = q.row0;
         t.rows = (int)min((int64_t)R, all - r0);
         t.pos0 = q.len - q.n;
-        const int first = t.pos0 + t.row0 / a.group;
-        const int last = t.pos0 + (t.row0 + t.rows - 1) / a.group;
+        const int first = t.pos0 + a.by_group.of(t.row0);
+        const int last = t.pos0 + a.by_group.of(t.row0 + t.rows - 1);
+        t.first = first;
+        t.last = last;
         t.k1 = max(last + 1, 0);
         t.k0 = a.window ? max(first - a.window + 1, 0) : 0;
         t.b0 = t.k0 / U;
@@ -178,58 +190,56 @@ __device__ __forceinline__ int cta_of(const Range &r, int64_t x) {
 // The items of a CTA in order. Roles of a CTA that walk by themselves see the same ones.
 template <typename S>
 struct Walk {
-    Range w;
-    int64_t pos, slot_at;    // how far; position of the slot's first item
+    int64_t at, w0, w1;      // position of the current item; the CTA's range
     int64_t item0, item1;    // positions of the item's blocks
     Tile tl;
-    int slot, seq, cost;
+    int slot, seq, cost, n_slots;
     int head, blk0, blk1;    // the item's kv head; this CTA's blocks of it
-    int first, last;         // positions of the item's first and last row
     bool begins, ends;       // the item's first, last block is among them
 
     __device__ __forceinline__ void start(const AttnArgs &a, const Range &r) {
-        w = r;
-        pos = r.w0;
+        w0 = r.w0;
+        w1 = r.w1;
+        n_slots = r.n_slots;
         slot = r.slot;
         seq = r.seq;
-        slot_at = r.at;
-        cost = 0;
-        if (pos < w.w1) {
-            tl = S::tile(a, slot, seq);
-            cost = S::cost(tl);
-        }
+        tl = S::tile(a, slot, seq);
+        cost = S::cost(tl);
+        head = (int)((w0 - r.at) / cost);
+        at = r.at + (int64_t)head * cost;
     }
+    // Sets the item at `at` and steps past it.
     __device__ __forceinline__ bool next(const AttnArgs &a) {
-        while (pos < w.w1) {
-            while (pos >= slot_at + (int64_t)cost * a.kv.n_kv) {
-                slot_at += (int64_t)cost * a.kv.n_kv;
-                // the lengths must not change under the kernel; if they do, it still ends
-                if (++slot >= w.n_slots) return false;
-                while (seq + 1 < a.kv.n_seqs && S::base(a, seq + 1) <= slot) seq++;
-                tl = S::tile(a, slot, seq);
-                cost = S::cost(tl);
+        while (at < w1) {
+            if (head == a.kv.n_kv) {  // on to the next slot that holds a tile
+                head = 0;
+                do {
+                    // the lengths must not change under the kernel; if they do, it still ends
+                    if (++slot >= n_slots) return false;
+                    while (seq + 1 < a.kv.n_seqs && S::base(a, seq + 1) <= slot) seq++;
+                    tl = S::tile(a, slot, seq);
+                    cost = S::cost(tl);
+                } while (cost == 0);
             }
-            head = (int)((pos - slot_at) / cost);
-            const int64_t at = slot_at + (int64_t)head * cost;
             item0 = at + S::kExtra;
             item1 = at + cost;
-            const int64_t lo = max(pos, item0), hi = min(item1, w.w1);
-            pos = hi;
+            at = item1;
+            head++;
+            const int64_t lo = max(w0, item0), hi = min(item1, w1);
             if (lo >= hi) continue;  // only of the item's extra cost
             blk0 = tl.b0 + (int)(lo - item0);
             blk1 = tl.b0 + (int)(hi - item0);
             begins = lo == item0;
             ends = hi == item1;
-            first = tl.pos0 + tl.row0 / a.group;
-            last = tl.pos0 + (tl.row0 + tl.rows - 1) / a.group;
             return true;
         }
         return false;
     }
+    __device__ __forceinline__ int kv_head() const { return head - 1; }
     // Rows of the tile differ in which of the keys j0 .. j0 + n - 1 they see.
     __device__ __forceinline__ bool mixed(const AttnArgs &a, int j0, int n) const {
         const int jf = max(j0, tl.k0), jl = min(j0 + n, tl.k1) - 1;
-        return jl > first || (a.window && jf <= last - a.window);
+        return jl > tl.first || (a.window && jf <= tl.last - a.window);
     }
 };
 

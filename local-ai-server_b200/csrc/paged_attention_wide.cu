@@ -219,7 +219,6 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
     auto &ctl = *reinterpret_cast<Ctl<HD, FMT, QF32> *>(raw_smem + C::kRaw * C::kRawTile);
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int wg = warp >> 2, wt = threadIdx.x & 127;  // warpgroup, thread of it
-    volatile int *abort_flag = &ctl.abort;
 
     pdl_wait_prior();
     pdl_launch_dependents();
@@ -268,22 +267,15 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
     // its own columns
     constexpr uint32_t kP = MT == 2 ? 0 : 128, kPV = MT == 2 ? 256 : 384;
 
-    // Bounded wait of a whole warp, which agrees on the answer; false once this CTA gives up.
+    // Bounded wait of a whole warp, which agrees on the answer; false when it ran out.
     auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
         bool ok = bulk::mbar_try_wait(bar, parity);
         if (!ok) {
             const uint64_t t0 = bulk::globaltimer_ns();
-            for (uint32_t n = 1; !ok; n++) {
+            do
                 ok = bulk::mbar_try_wait(bar, parity);
-                if (!ok && (n & 63u) == 0) {
-                    if (*abort_flag) break;
-                    if (bulk::globaltimer_ns() - t0 > kWaitNs) {
-                        *abort_flag = 1;
-                        flag(a.err, LAI_DEVERR_TIMEOUT);
-                        break;
-                    }
-                }
-            }
+            while (!ok && bulk::globaltimer_ns() - t0 < kWaitNs);
+            if (!ok) ctl.abort = 1;
         }
         return __all_sync(0xffffffffu, ok);
     };
@@ -308,11 +300,12 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         uint32_t idx = 0, blocks = 0;  // operand tiles, blocks so far
         bool ok = true;
         while (ok && it.next(a)) {
+            const int head = it.kv_head();
             for (int r = lane; r < it.tl.rows; r += 32) {  // the item's queries on their way to L2
-                const int fr = it.tl.row0 + r, tok = fr / a.group;
+                const int fr = it.tl.row0 + r, tok = a.by_group.of(fr);
                 const char *q = static_cast<const char *>(qp) +
                                 (((int64_t)it.tl.q_row0 + tok) * a.ld_q +
-                                 (int64_t)(it.head * a.group + (fr - tok * a.group)) * HD) * (QF32 ? 4 : 2);
+                                 (int64_t)(head * a.group + (fr - tok * a.group)) * HD) * (QF32 ? 4 : 2);
 #pragma unroll
                 for (int i = 0; i < HD * (QF32 ? 4 : 2); i += 128)
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
@@ -335,7 +328,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     __syncwarp();
                     if constexpr (kF16) {
                         if (page >= 0) {
-                            const int64_t at = a.kv.page_base(page, it.head) + ((j0 + kGroup * lane) & in_page);
+                            const int64_t at = a.kv.page_base(page, head) + ((j0 + kGroup * lane) & in_page);
                             bulk::load(raw_smem + land * C::kRawTile + lane * kGroupBytes,
                                        (kv ? a.kv.v : a.kv.k) + at * HD, kGroupBytes, &ctl.landed[land]);
                             if (kv == 0) {
@@ -348,7 +341,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         const int g = lane / kHalves, h = lane % kHalves;
                         const int pg = __shfl_sync(0xffffffffu, page, g & 7);
                         if (g < kU / kGroup && pg >= 0) {
-                            const int64_t at = a.kv.page_base(pg, it.head) + ((j0 + kGroup * g) & in_page);
+                            const int64_t at = a.kv.page_base(pg, head) + ((j0 + kGroup * g) & in_page);
                             tma_load_2d(smem_addr(st_smem + land * C::kTile) + h * 16384 + g * (kGroup * 128),
                                         kv ? &v_map : &k_map, h * 64, (int)at, &ctl.landed[land]);
                         }
@@ -556,7 +549,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 blocks += nb;
                 continue;
             }
-            const int r = mt * 128 + wt, fr = it.tl.row0 + r, tok = fr / a.group;
+            const int head = it.kv_head();
+            const int r = mt * 128 + wt, fr = it.tl.row0 + r, tok = a.by_group.of(fr);
             const int row_pos = it.tl.pos0 + tok;  // of a row behind the last: not stored
             const int row_from = a.window ? row_pos - a.window : -1;  // sees (row_from, row_pos]
             // Q into shared memory, the warp's own 32 rows; the last scores of the item before are
@@ -567,19 +561,20 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             const int run = lane % kLanes, sub = lane / kLanes;
             float c = a.scale_log2;
             {
-                constexpr int kBatch = 16 < 32 / kAtOnce ? 16 : 32 / kAtOnce;
+                constexpr int kBatch = 8;  // loads under way per lane
+                static_assert(32 / kAtOnce % kBatch == 0, "whole batches");
 #pragma unroll 1
                 for (int p0 = 0; p0 < 32 / kAtOnce; p0 += kBatch) {
                     uint4 raw[kBatch];
 #pragma unroll
                     for (int p = 0; p < kBatch; p++) {
-                        const int rr = (p0 + p) * kAtOnce + sub, f = it.tl.row0 + mt * 128 + wrow + rr, tk = f / a.group;
+                        const int rr = (p0 + p) * kAtOnce + sub, f = it.tl.row0 + mt * 128 + wrow + rr, tk = a.by_group.of(f);
                         raw[p] = make_uint4(0, 0, 0, 0);
                         if (mt * 128 + wrow + rr < it.tl.rows)
                             raw[p] = __ldg(reinterpret_cast<const uint4 *>(
                                 static_cast<const char *>(qp) +
                                 (((int64_t)it.tl.q_row0 + tk) * a.ld_q +
-                                 (int64_t)(it.head * a.group + (f - tk * a.group)) * HD) * kElem + run * 16));
+                                 (int64_t)(head * a.group + (f - tk * a.group)) * HD) * kElem + run * 16));
                     }
 #pragma unroll
                     for (int p = 0; p < kBatch; p++) {
@@ -666,8 +661,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 umma::fence_after_sync();
                 if (MT == 2 && b > 0) saw_bad(blocks - 1);  // its P V came before these scores
                 const int groups = ctl.groups[slot];
-                const bool masked = groups != 0xff || j0 + kU - 1 > it.first || it.tl.k0 > j0 ||
-                                    (a.window && j0 <= it.last - a.window);
+                const bool masked = groups != 0xff || j0 + kU - 1 > it.tl.first || it.tl.k0 > j0 ||
+                                    (a.window && j0 <= it.tl.last - a.window);
                 // the row sees keys j0 + lo .. j0 + hi, as bits of 32 keys
                 const int hi = row_pos - j0, lo = row_from + 1 - j0;
                 auto seen = [&](int g) -> uint32_t {
@@ -831,18 +826,20 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
 #pragma unroll
                     for (int i = 0; i < 32; i++) x[i] = o[(32 * g + i) % kKeep];
                 }
-                // infinities and NaN that were taken out of blocks whose rows differ in what they see
-                const int jend = bad ? min(it.blk1 * kU, it.tl.k1) : 0;
-                for (int j = max(it.blk0 * kU, it.tl.k0); j < jend; j++) {
+            };
+            // Infinities and NaN that were taken out of blocks whose rows differ in what they see:
+            // add(d, value) for each that this row sees.
+            auto mend = [&](auto add) {
+                for (int j = max(it.blk0 * kU, it.tl.k0); j < min(it.blk1 * kU, it.tl.k1); j++) {
                     if (!it.mixed(a, j / kU * kU, kU) || j > row_pos || j <= row_from) continue;
                     const int page = __ldg(a.kv.pages + (int64_t)it.tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
                     if (page < 0 || page >= a.kv.n_pages) continue;
-                    const int64_t at = a.kv.page_base(page, it.head) + (j & in_page);
+                    const int64_t at = a.kv.page_base(page, head) + (j & in_page);
                     const float vs = kF16 ? __ldg(a.kv.v_scale + at) : 1.f;
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const float v = element<FMT>(a.kv.v, at * HD + 32 * g + i) * vs;
-                        if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) x[i] += v;
+#pragma unroll 1
+                    for (int d = 0; d < HD; d++) {
+                        const float v = element<FMT>(a.kv.v, at * HD + d) * vs;
+                        if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) add(d, v);
                     }
                 }
             };
@@ -869,12 +866,12 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 __syncwarp();
 #pragma unroll 4
                 for (int p = 0; p < 32 / kAtOnce; p++) {
-                    const int rr = p * kAtOnce + sub, f = it.tl.row0 + mt * 128 + wrow + rr, tk = f / a.group;
+                    const int rr = p * kAtOnce + sub, f = it.tl.row0 + mt * 128 + wrow + rr, tk = a.by_group.of(f);
                     if (mt * 128 + wrow + rr >= it.tl.rows) continue;
                     const uint32_t tile = my_rows + (QF32 && run >= kLanes / 2 ? MT * C::kTile : 0);
                     const uint4 v = ld_shared16(tile + chunk_off(wrow + rr, run % (HD / 8)));
                     st_vec(static_cast<char *>(out) +
-                               ((((int64_t)it.tl.q_row0 + tk) * a.kv.n_kv + it.head) * a.group + (f - tk * a.group)) * (HD * kElem) + run * 16, v);
+                               ((((int64_t)it.tl.q_row0 + tk) * a.kv.n_kv + head) * a.group + (f - tk * a.group)) * (HD * kElem) + run * 16, v);
                 }
                 __syncwarp();
             };
@@ -887,6 +884,17 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     stage(g, x, inv);
                 }
                 umma::fence_before_sync();
+                if (bad)
+                    mend([&](int d, float v) {
+                        if (QF32) {
+                            float *p = reinterpret_cast<float *>(q_smem + (d >= HD / 2 ? MT * C::kTile : 0) +
+                                                                 chunk_off(wt, d % (HD / 2) / 4) + d % 4 * 4);
+                            *p += v;
+                        } else {
+                            uint16_t *p = reinterpret_cast<uint16_t *>(q_smem + mt * C::kTile + chunk_off(wt, d / 8) + d % 8 * 2);
+                            *p = from_f<uint16_t>(to_f(*p) + v);
+                        }
+                    });
                 store();
                 continue;
             }
@@ -905,6 +913,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
             }
             umma::fence_before_sync();
+            if (bad) mend([&](int d, float v) { pp[2 * R + (d / 4 * R + r) * 4 + d % 4] += v; });
             __threadfence();
             if (!(ok = join())) break;
             const int c0 = cta_of(range, it.item0), c1 = cta_of(range, it.item1 - 1);
@@ -945,6 +954,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
+    if (threadIdx.x == 0 && ctl.abort) flag(a.err, LAI_DEVERR_TIMEOUT);
     if (warp == 12) umma::tmem_dealloc(tmem, 512);
 }
 

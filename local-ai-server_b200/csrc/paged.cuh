@@ -35,7 +35,7 @@ struct Seq {
     bool ok;
 };
 __device__ __forceinline__ Seq load_seq(const View &a, int s) {
-    const int r0 = __ldg(a.q_start + s), r1 = __ldg(a.q_start + s + 1), len = __ldg(a.kv_len + s);
+    const int r0 = a.q_start[s], r1 = a.q_start[s + 1], len = a.kv_len[s];
     Seq q;
     q.row0 = r0;
     q.n = r1 - r0;

@@ -101,6 +101,7 @@ template <int FMT> using FewSched = Sched<kRows, block_keys<FMT>(), 0>;
 template <int HD>
 struct Smem {
     SchedSmem sched;
+    SeqSmem seqs;
     float m[kWarps][kRows], l[kWarps][kRows];
     float o[kWarps][kRows][HD + 4];  // rows apart by 4 banks
     int bad, last;
@@ -127,16 +128,14 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     const int g = lane >> 2, t = lane & 3;
     pdl_wait_prior();
     pdl_launch_dependents();
-    if (blockIdx.x == 0)
-        for (int s = threadIdx.x; s < a.kv.n_seqs; s += kThreads)
-            if (!load_seq(a.kv, s).ok) flag(a.err, LAI_DEVERR_POSITION);
-    const Range range = find_range<FewSched<FMT>, kThreads>(a, sm.sched);
+    const AttnArgs as = cache_seqs<kThreads>(a, sm.seqs);
+    const Range range = find_range<FewSched<FMT>, kThreads>(as, sm.sched);
     if (range.w0 >= range.w1) return;
 
     const int n_heads = a.kv.n_kv * a.group, in_page = a.kv.page_size() - 1;
     Walk<FewSched<FMT>> it;
-    it.start(a, range);
-    while (it.next(a)) {
+    it.start(as, range);
+    while (it.next(as)) {
         const Tile &tl = it.tl;
         const int head = it.kv_head(), blk0 = it.blk0, blk1 = it.blk1;
 
@@ -339,12 +338,12 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             // ---- values. A step whose keys some rows of the tile see and others do not gives
             // every row 0 x v for the keys it must not see: infinities and NaN are taken out of
             // such a step, and added to the rows that see them at the end.
-            const bool mixed = FMT != LAI_KV_I8 && it.mixed(a, j0, kStep);
+            const bool uneven = FMT != LAI_KV_I8 && mixed(tl, a.window, j0, kStep);
             auto column = [&](int n, uint32_t (&b0)[NK], uint32_t (&b1)[NK]) {
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kk = 0; kk < NK; kk++) {
-                    if (mixed) {
+                    if (uneven) {
                         bad |= drop_nonfinite<kF16>(b0[kk]);
                         bad |= drop_nonfinite<kF16>(b1[kk]);
                     }
@@ -443,7 +442,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         }
         if (FMT != LAI_KV_I8 && sm.bad) {
             for (int j = max(blk0 * U, tl.k0); j < min(blk1 * U, tl.k1); j++) {
-                if (!it.mixed(a, j / kStep * kStep, kStep)) continue;
+                if (!mixed(tl, a.window, j / kStep * kStep, kStep)) continue;
                 const int page = __ldg(a.kv.pages + (int64_t)tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
                 if (page < 0 || page >= a.kv.n_pages) continue;
                 const int64_t at = (a.kv.page_base(page, head) + (j & in_page)) * HD;

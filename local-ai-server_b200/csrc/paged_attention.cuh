@@ -61,6 +61,13 @@ struct Tile {
     int b0, blocks;         // first block, blocks (1 for a tile that sees no key)
 };
 
+// Rows of the tile (or item) differ in which of the keys j0 .. j0 + n - 1 they see.
+template <typename T>
+__device__ __forceinline__ bool mixed(const T &t, int window, int j0, int n) {
+    const int jf = max(j0, t.k0), jl = min(j0 + n, t.k1) - 1;
+    return jl > t.first || (window && jf <= t.last - window);
+}
+
 template <int R, int U, int E>
 struct Sched {
     static constexpr int kRowsPerTile = R, kBlock = U, kExtra = E;
@@ -70,7 +77,7 @@ struct Sched {
         return n_rows * group / R + n_seqs;
     }
     static __device__ __forceinline__ int base(const AttnArgs &a, int s) {
-        return (int)((int64_t)__ldg(a.kv.q_start + s) * a.group / R) + s;
+        return (int)((int64_t)a.kv.q_start[s] * a.group / R) + s;
     }
     static __device__ __forceinline__ int cost(const Tile &t) { return t.rows ? t.blocks + E : 0; }
     // The last sequence whose slots start at or before `slot` (0 if none does).
@@ -104,6 +111,30 @@ struct Sched {
         return t;
     }
 };
+
+// The sequences' rows and lengths in shared memory, where they fit: finding a CTA's work looks at
+// them again and again, one load after another.
+constexpr int kSeqCache = 256;
+struct SeqSmem {
+    int32_t q_start[kSeqCache + 1], kv_len[kSeqCache];
+};
+// a with its tables in shared memory (or as it is); flags sequences that are not well formed. The
+// whole CTA; ends with a barrier.
+template <int THREADS>
+__device__ __forceinline__ AttnArgs cache_seqs(const AttnArgs &a, SeqSmem &sm) {
+    AttnArgs c = a;
+    if (a.kv.n_seqs <= kSeqCache) {
+        for (int s = threadIdx.x; s <= a.kv.n_seqs; s += THREADS) sm.q_start[s] = __ldg(a.kv.q_start + s);
+        for (int s = threadIdx.x; s < a.kv.n_seqs; s += THREADS) sm.kv_len[s] = __ldg(a.kv.kv_len + s);
+        c.kv.q_start = sm.q_start;
+        c.kv.kv_len = sm.kv_len;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int s = threadIdx.x; s < a.kv.n_seqs; s += THREADS)
+            if (!load_seq(c.kv, s).ok) flag(a.err, LAI_DEVERR_POSITION);
+    return c;
+}
 
 // Where a CTA starts, and how far it goes. Positions are in blocks of the whole work.
 struct Range {
@@ -236,11 +267,6 @@ struct Walk {
         return false;
     }
     __device__ __forceinline__ int kv_head() const { return head - 1; }
-    // Rows of the tile differ in which of the keys j0 .. j0 + n - 1 they see.
-    __device__ __forceinline__ bool mixed(const AttnArgs &a, int j0, int n) const {
-        const int jf = max(j0, tl.k0), jl = min(j0 + n, tl.k1) - 1;
-        return jl > tl.first || (a.window && jf <= tl.last - a.window);
-    }
 };
 
 // The kernel for many rows per sequence (paged_attention_wide.cu), scale_log2 > 0: LAI_OK or an

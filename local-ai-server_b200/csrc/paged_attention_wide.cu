@@ -39,7 +39,6 @@ constexpr int kGroup = 16;     // keys per copy
 constexpr int kRing = 4;       // blocks whose scales and flags are kept
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kGrow = 8.f;   // log2 of how far weights may pass 1 before O is rescaled
-constexpr int kPolyOf8 = 3;    // of 8 exponentials, those that the FMA pipe takes
 
 template <int HD, int FMT, bool QF32>
 struct Cfg {
@@ -54,8 +53,22 @@ struct Cfg {
     static constexpr int kLand = kF16 ? kRaw : kStages;  // tiles that copies land in
     // binary16 weights: 2^kLift at the row's maximum, below 2^15 after kGrow and a value scale
     static constexpr float kLift = kF16 ? 5.f : 0.f;
+    // Of 8 exponentials, those that the FMA pipe takes: with 8-bit caches 2 (2048 tokens over 32768
+    // INT8 keys, 16 heads of 128: 587 us with none, 588 with 1, 524 with 2, 640 with 3), with BF16
+    // ones none (466, 467, 476, 477 us).
+    static constexpr int kPolyOf8 = kF16 ? 2 : 0;
     using S = Sched<R, kU, 3>;
 };
+
+// A CTA's part of an item, as the copy warp hands it to the other roles.
+struct Item {
+    int seq, head, row0, rows, q_row0, pos0;  // rows 0: no more items
+    int first, last, k0, k1;                  // positions of its first and last row; keys any row sees
+    int blk0, blk1;                           // this CTA's blocks
+    int c0, c1;                               // the CTAs that have a part of it
+    bool begins, whole;                       // has its first block; has all of them
+};
+constexpr int kItems = 4;  // items under way
 
 template <int HD, int FMT, bool QF32>
 struct Ctl {
@@ -63,12 +76,13 @@ struct Ctl {
     static constexpr int kScales = C::kF16 ? kU : 4;
     float kscale[kRing][kScales], vscale[kRing][kScales];  // 16-byte aligned
     uint64_t landed[C::kLand], taken[C::kLand], full[C::kStages], empty[C::kStages];
-    uint64_t info[kRing];
+    uint64_t info[kRing], item_full[kItems], item_empty[kItems];
+    Item items[kItems];
     uint64_t q_full[2], s_full[2], p_full[2][2], pv_full[2], group[2];
     int vexp[kRing][4];
     int groups[kRing];  // bit i: 16-key group i of the block lies in a real page
     int vbad[kRing];    // the block (counted) from whose V infinities or NaN were taken out
-    SchedSmem sched;
+    SeqSmem seqs;
     uint32_t tmem;
     int abort, last[2];
 };
@@ -226,10 +240,9 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         if (threadIdx.x == 0) flag(a.err, LAI_DEVERR_SMEM_ALIGN);
         return;
     }
-    if (blockIdx.x == 0)
-        for (int s = threadIdx.x; s < a.kv.n_seqs; s += kThreads)
-            if (!load_seq(a.kv, s).ok) flag(a.err, LAI_DEVERR_POSITION);
-    const Range range = find_range<S, kThreads>(a, ctl.sched);
+    const AttnArgs as = cache_seqs<kThreads>(a, ctl.seqs);
+    // (in the place of Q, which comes behind the barrier below)
+    const Range range = find_range<S, kThreads>(as, *reinterpret_cast<SchedSmem *>(q_smem));
     if (range.w0 >= range.w1) return;  // the whole CTA
     if (warp == 12) {
         umma::tmem_alloc(&ctl.tmem, 512);
@@ -247,6 +260,10 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         for (int i = 0; i < kRing; i++) {
             bulk::mbar_init(&ctl.info[i], 4);
             ctl.vbad[i] = -1;
+        }
+        for (int i = 0; i < kItems; i++) {
+            bulk::mbar_init(&ctl.item_full[i], 1);
+            bulk::mbar_init(&ctl.item_empty[i], 4 + 1 + 4 * MT);
         }
         for (int i = 0; i < 2; i++) {
             bulk::mbar_init(&ctl.q_full[i], 128);
@@ -280,13 +297,23 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         return __all_sync(0xffffffffu, ok);
     };
 
-    Walk<S> it;
-    it.start(a, range);
+    // The next item for a warp of any role but the copies'; false at the end.
+    uint32_t n_items = 0;
+    Item it;
+    auto next = [&](bool &ok) -> bool {
+        const uint32_t i = n_items % kItems;
+        if (!(ok = wait(&ctl.item_full[i], (n_items / kItems) & 1))) return false;
+        n_items++;
+        it = ctl.items[i];
+        __syncwarp();
+        if (lane == 0) bulk::mbar_arrive(&ctl.item_empty[i]);
+        return it.rows != 0;
+    };
     // The page of 16-key group `lane` (< 8) of the block at j0, or -1.
-    auto page_of = [&](int j0) -> int {
+    auto page_of = [&](int seq, int k1, int j0) -> int {
         const int j = j0 + kGroup * lane;
-        if (lane >= kU / kGroup || j >= it.tl.k1) return -1;
-        const int page = __ldg(a.kv.pages + (int64_t)it.tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
+        if (lane >= kU / kGroup || j >= k1) return -1;
+        const int page = __ldg(a.kv.pages + (int64_t)seq * a.kv.max_pages + (j >> a.kv.log_page));
         return page >= 0 && page < a.kv.n_pages ? page : -1;
     };
     const int in_page = a.kv.page_size() - 1;
@@ -299,20 +326,39 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         // ================= copies ============================================================
         uint32_t idx = 0, blocks = 0;  // operand tiles, blocks so far
         bool ok = true;
-        while (ok && it.next(a)) {
-            const int head = it.kv_head();
-            for (int r = lane; r < it.tl.rows; r += 32) {  // the item's queries on their way to L2
-                const int fr = it.tl.row0 + r, tok = a.by_group.of(fr);
+        Walk<S> w;
+        w.start(as, range);
+        for (;;) {
+            const bool more = w.next(as);
+            const Tile &tl = w.tl;
+            const int head = w.kv_head();
+            const uint32_t slot = n_items % kItems;
+            if (n_items >= kItems && !(ok = wait(&ctl.item_empty[slot], (n_items / kItems - 1) & 1))) break;
+            n_items++;
+            if (lane == 0) {
+                Item &to = ctl.items[slot];
+                to = Item{tl.seq, head, tl.row0, more ? tl.rows : 0, tl.q_row0, tl.pos0, tl.first, tl.last,
+                          tl.k0, tl.k1, w.blk0, w.blk1, 0, 0, w.begins, w.begins && w.ends};
+                if (more && !to.whole) {
+                    to.c0 = cta_of(range, w.item0);
+                    to.c1 = cta_of(range, w.item1 - 1);
+                }
+                bulk::mbar_arrive(&ctl.item_full[slot]);
+            }
+            __syncwarp();
+            if (!more) break;
+            for (int r = lane; r < tl.rows; r += 32) {  // the item's queries on their way to L2
+                const int fr = tl.row0 + r, tok = a.by_group.of(fr);
                 const char *q = static_cast<const char *>(qp) +
-                                (((int64_t)it.tl.q_row0 + tok) * a.ld_q +
+                                (((int64_t)tl.q_row0 + tok) * a.ld_q +
                                  (int64_t)(head * a.group + (fr - tok * a.group)) * HD) * (QF32 ? 4 : 2);
 #pragma unroll
                 for (int i = 0; i < HD * (QF32 ? 4 : 2); i += 128)
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
             }
-            for (int blk = it.blk0; ok && blk < it.blk1; blk++, blocks++) {
+            for (int blk = w.blk0; ok && blk < w.blk1; blk++, blocks++) {
                 const int j0 = blk * kU;
-                const int page = page_of(j0);
+                const int page = page_of(tl.seq, tl.k1, j0);
                 const uint32_t groups = __ballot_sync(0xffffffffu, page >= 0);
                 for (int kv = 0; kv < 2; kv++, idx++) {
                     const uint32_t land = idx % LD;
@@ -348,6 +394,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     }
                 }
             }
+            if (!ok) break;
         }
         // an abort leaves copies in flight: they get a millisecond before shared memory goes
         if (!ok) {
@@ -358,18 +405,18 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         // ================= finishing tiles ===================================================
         uint32_t idx = 0, blocks = 0;
         bool ok = true;
-        while (ok && it.next(a)) {
+        while (next(ok)) {
             for (int blk = it.blk0; ok && blk < it.blk1; blk++, blocks++) {
                 const int j0 = blk * kU, slot = blocks % kRing;
-                const int page = page_of(j0);
-                if (wt < kU / kGroup && page < 0 && j0 + kGroup * lane < it.tl.k1 &&
-                    j0 + kGroup * lane + kGroup > it.tl.k0)
+                const int page = page_of(it.seq, it.k1, j0);
+                if (wt < kU / kGroup && page < 0 && j0 + kGroup * lane < it.k1 &&
+                    j0 + kGroup * lane + kGroup > it.k0)
                     flag(a.err, LAI_DEVERR_PAGE);
                 const uint32_t groups = __ballot_sync(0xffffffffu, page >= 0);
-                const bool whole = groups == 0xff && j0 >= it.tl.k0 && j0 + kU <= it.tl.k1;
-                const bool mixed = it.mixed(a, j0, kU);
+                const bool whole = groups == 0xff && j0 >= it.k0 && j0 + kU <= it.k1;
+                const bool mixed = paged::mixed(it, a.window, j0, kU);
                 auto there = [&](int r) {
-                    return j0 + r >= it.tl.k0 && j0 + r < it.tl.k1 && (groups >> (r / kGroup) & 1);
+                    return j0 + r >= it.k0 && j0 + r < it.k1 && (groups >> (r / kGroup) & 1);
                 };
                 for (int kv = 0; kv < 2; kv++, idx++) {
                     const uint32_t land = idx % LD;
@@ -471,8 +518,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             }
             commit(&ctl.s_full[mt]);
         };
-        while (ok && it.next(a)) {
-            const int tiles = MT == 2 && it.tl.rows > 128 ? 2 : 1;
+        while (next(ok)) {
+            const int tiles = MT == 2 && it.rows > 128 ? 2 : 1;
             const int nb = it.blk1 - it.blk0;
             ok = wait(&ctl.full[idx % ST], (idx / ST) & 1);
             for (int mt = 0; ok && mt < tiles; mt++) {
@@ -537,21 +584,21 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         const int mt = wg;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + lane_base + mt * 128, t_p = t_s + kP, t_pv = tmem + lane_base + kPV + mt * 128;
-        uint32_t n = 0, blocks = 0, n_group = 0, n_items = 0;  // this tile's blocks, all blocks, joins, items
+        uint32_t n = 0, blocks = 0, n_group = 0, n_last = 0;  // this tile's blocks, all blocks, joins, last P Vs
         bool ok = true;
         auto join = [&]() {  // all of the warpgroup, within the bound
             bulk::mbar_arrive(&ctl.group[mt]);
             return wait(&ctl.group[mt], n_group++ & 1);
         };
-        while (ok && it.next(a)) {
+        while (next(ok)) {
             const int nb = it.blk1 - it.blk0;
-            if (it.tl.rows <= mt * 128) {  // no rows of this tile
+            if (it.rows <= mt * 128) {  // no rows of this tile
                 blocks += nb;
                 continue;
             }
-            const int head = it.kv_head();
-            const int r = mt * 128 + wt, fr = it.tl.row0 + r, tok = a.by_group.of(fr);
-            const int row_pos = it.tl.pos0 + tok;  // of a row behind the last: not stored
+            const int head = it.head;
+            const int r = mt * 128 + wt, fr = it.row0 + r, tok = a.by_group.of(fr);
+            const int row_pos = it.pos0 + tok;  // of a row behind the last: not stored
             const int row_from = a.window ? row_pos - a.window : -1;  // sees (row_from, row_pos]
             // Q into shared memory, the warp's own 32 rows; the last scores of the item before are
             // done. kLanes lanes take a row, so that a load reads whole lines.
@@ -559,22 +606,35 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             const int wrow = (warp & 3) * 32;                            // the warp's first row of it
             constexpr int kElem = QF32 ? 4 : 2, kLanes = HD * kElem / 16, kAtOnce = 32 / kLanes;
             const int run = lane % kLanes, sub = lane / kLanes;
+            // row sub + p * kAtOnce of the warp as token and head of the group, p counting up
+            int tk, gh;
+            const int step_t = a.by_group.of(kAtOnce), step_g = kAtOnce - step_t * a.group;
+            auto first_row = [&]() {
+                const int f = it.row0 + mt * 128 + wrow + sub;
+                tk = a.by_group.of(f);
+                gh = f - tk * a.group;
+            };
+            auto next_row = [&]() {
+                tk += step_t;
+                gh += step_g;
+                if (gh >= a.group) gh -= a.group, tk++;
+            };
             float c = a.scale_log2;
             {
-                constexpr int kBatch = 8;  // loads under way per lane
-                static_assert(32 / kAtOnce % kBatch == 0, "whole batches");
+                constexpr int kBatch = 32 / kAtOnce < 16 ? 32 / kAtOnce : 16;  // loads under way per lane
+                const char *src = static_cast<const char *>(qp) +
+                                  ((int64_t)it.q_row0 * a.ld_q + (int64_t)head * a.group * HD) * kElem + run * 16;
+                first_row();
 #pragma unroll 1
                 for (int p0 = 0; p0 < 32 / kAtOnce; p0 += kBatch) {
                     uint4 raw[kBatch];
 #pragma unroll
                     for (int p = 0; p < kBatch; p++) {
-                        const int rr = (p0 + p) * kAtOnce + sub, f = it.tl.row0 + mt * 128 + wrow + rr, tk = a.by_group.of(f);
+                        const int rr = (p0 + p) * kAtOnce + sub;
                         raw[p] = make_uint4(0, 0, 0, 0);
-                        if (mt * 128 + wrow + rr < it.tl.rows)
-                            raw[p] = __ldg(reinterpret_cast<const uint4 *>(
-                                static_cast<const char *>(qp) +
-                                (((int64_t)it.tl.q_row0 + tk) * a.ld_q +
-                                 (int64_t)(head * a.group + (f - tk * a.group)) * HD) * kElem + run * 16));
+                        if (mt * 128 + wrow + rr < it.rows)
+                            raw[p] = __ldg(reinterpret_cast<const uint4 *>(src + (tk * a.ld_q + gh * HD) * kElem));
+                        next_row();
                     }
 #pragma unroll
                     for (int p = 0; p < kBatch; p++) {
@@ -661,8 +721,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 umma::fence_after_sync();
                 if (MT == 2 && b > 0) saw_bad(blocks - 1);  // its P V came before these scores
                 const int groups = ctl.groups[slot];
-                const bool masked = groups != 0xff || j0 + kU - 1 > it.tl.first || it.tl.k0 > j0 ||
-                                    (a.window && j0 <= it.tl.last - a.window);
+                const bool masked = groups != 0xff || j0 + kU - 1 > it.first || it.k0 > j0 ||
+                                    (a.window && j0 <= it.last - a.window);
                 // the row sees keys j0 + lo .. j0 + hi, as bits of 32 keys
                 const int hi = row_pos - j0, lo = row_from + 1 - j0;
                 auto seen = [&](int g) -> uint32_t {
@@ -712,7 +772,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         for (int h = 0; h < 2; h++) {
                             float2 p = __ffma2_rn(x[i + h], c2, nb2);
                             // (a masked score's weight must be exactly 0, and F32 results exact)
-                            if (!QF32 && !decltype(mask)::value && ((i + h) * kPolyOf8 & 7) < kPolyOf8)
+                            if (!QF32 && !decltype(mask)::value && ((i + h) * C::kPolyOf8 & 7) < C::kPolyOf8)
                                 p = exp2_poly(p);
                             else
                                 p = make_float2(ex2(p.x), ex2(p.y));
@@ -809,11 +869,13 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             }
             if (!ok) break;
             // the last P V: one commit per item with two tiles, one per block with one
-            if (!(ok = wait(&ctl.pv_full[mt], (MT == 2 ? n_items++ : n - 1) & 1))) break;
+            if (!(ok = wait(&ctl.pv_full[mt], (MT == 2 ? n_last++ : n - 1) & 1))) break;
             umma::fence_after_sync();
             saw_bad(blocks - 1);
             if (MT == 1) add_pv();
-            // columns 32 g .. of the output row, before the division
+            // columns 32 g .. of the output row, before the division (rolled where it may be: the code
+            // of all roles shares the instruction cache)
+            constexpr int kPieces = MT == 2 ? 1 : HD / 32;
             auto piece = [&](int g, float (&x)[32]) {
                 if constexpr (MT == 2) {
                     uint32_t u[32];
@@ -830,9 +892,9 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             // Infinities and NaN that were taken out of blocks whose rows differ in what they see:
             // add(d, value) for each that this row sees.
             auto mend = [&](auto add) {
-                for (int j = max(it.blk0 * kU, it.tl.k0); j < min(it.blk1 * kU, it.tl.k1); j++) {
-                    if (!it.mixed(a, j / kU * kU, kU) || j > row_pos || j <= row_from) continue;
-                    const int page = __ldg(a.kv.pages + (int64_t)it.tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
+                for (int j = max(it.blk0 * kU, it.k0); j < min(it.blk1 * kU, it.k1); j++) {
+                    if (!paged::mixed(it, a.window, j / kU * kU, kU) || j > row_pos || j <= row_from) continue;
+                    const int page = __ldg(a.kv.pages + (int64_t)it.seq * a.kv.max_pages + (j >> a.kv.log_page));
                     if (page < 0 || page >= a.kv.n_pages) continue;
                     const int64_t at = a.kv.page_base(page, head) + (j & in_page);
                     const float vs = kF16 ? __ldg(a.kv.v_scale + at) : 1.f;
@@ -864,90 +926,90 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             };
             auto store = [&]() {  // the warp's staged rows, in whole lines
                 __syncwarp();
+                char *dst = static_cast<char *>(out) +
+                            ((int64_t)it.q_row0 * a.kv.n_kv + head) * a.group * (HD * kElem) + run * 16;
+                const int64_t tok_bytes = (int64_t)a.kv.n_kv * a.group * (HD * kElem);
+                first_row();
 #pragma unroll 4
-                for (int p = 0; p < 32 / kAtOnce; p++) {
-                    const int rr = p * kAtOnce + sub, f = it.tl.row0 + mt * 128 + wrow + rr, tk = a.by_group.of(f);
-                    if (mt * 128 + wrow + rr >= it.tl.rows) continue;
+                for (int p = 0; p < 32 / kAtOnce; p++, next_row()) {
+                    const int rr = p * kAtOnce + sub;
+                    if (mt * 128 + wrow + rr >= it.rows) continue;
                     const uint32_t tile = my_rows + (QF32 && run >= kLanes / 2 ? MT * C::kTile : 0);
                     const uint4 v = ld_shared16(tile + chunk_off(wrow + rr, run % (HD / 8)));
-                    st_vec(static_cast<char *>(out) +
-                               ((((int64_t)it.tl.q_row0 + tk) * a.kv.n_kv + head) * a.group + (f - tk * a.group)) * (HD * kElem) + run * 16, v);
+                    st_vec(dst + tk * tok_bytes + gh * (HD * kElem), v);
                 }
                 __syncwarp();
             };
-            if (it.begins && it.ends) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
+            // parts: [row] off, [row] sum, then [d / 4][row][4]
+            constexpr int64_t kPart = (int64_t)R * (HD + 2);
+            auto part = [&](int cc) { return a.parts + ((int64_t)cc * 2 + (cc == it.c0 ? 1 : 0)) * kPart; };
+            float mu = 0.f;
+            if (!it.whole) {
+                float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * kPart;
+                pp[r] = off;
+                pp[R + r] = l;
+#pragma unroll kPieces
                 for (int g = 0; g < HD / 32; g++) {
                     float x[32];
                     piece(g, x);
-                    stage(g, x, inv);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4 *>(pp + 2 * R + ((8 * g + i / 4) * R + r) * 4) =
+                            make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                 }
                 umma::fence_before_sync();
-                if (bad)
-                    mend([&](int d, float v) {
-                        if (QF32) {
-                            float *p = reinterpret_cast<float *>(q_smem + (d >= HD / 2 ? MT * C::kTile : 0) +
-                                                                 chunk_off(wt, d % (HD / 2) / 4) + d % 4 * 4);
-                            *p += v;
-                        } else {
-                            uint16_t *p = reinterpret_cast<uint16_t *>(q_smem + mt * C::kTile + chunk_off(wt, d / 8) + d % 8 * 2);
-                            *p = from_f<uint16_t>(to_f(*p) + v);
+                if (bad) mend([&](int d, float v) { pp[2 * R + (d / 4 * R + r) * 4 + d % 4] += v; });
+                __threadfence();
+                if (!(ok = join())) break;
+                if (wt == 0) ctl.last[mt] = atomicAdd(a.counters + it.c0 * MT + mt, 1) == it.c1 - it.c0;
+                if (!(ok = join())) break;
+                if (!*(volatile int *)&ctl.last[mt]) continue;
+                __threadfence();
+                if (wt == 0) a.counters[it.c0 * MT + mt] = 0;  // ready for the next call
+                float top = neg_inf();
+                for (int cc = it.c0; cc <= it.c1; cc++) top = fmaxf(top, __ldcg(part(cc) + r));
+                mu = top == neg_inf() ? 0.f : top;
+                l = 0.f;
+                for (int cc = it.c0; cc <= it.c1; cc++)
+                    l = fmaf(__ldcg(part(cc) + R + r), ex2(__ldcg(part(cc) + r) - mu), l);
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll kPieces
+            for (int g = 0; g < HD / 32; g++) {
+                float x[32];
+                if (it.whole) {
+                    piece(g, x);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = 0.f;
+#pragma unroll 4
+                    for (int cc = it.c0; cc <= it.c1; cc++) {
+                        const float *pc = part(cc);
+                        const float f = ex2(__ldcg(pc + r) - mu);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * R + ((8 * g + i / 4) * R + r) * 4));
+                            x[i] = fmaf(v.x, f, x[i]);
+                            x[i + 1] = fmaf(v.y, f, x[i + 1]);
+                            x[i + 2] = fmaf(v.z, f, x[i + 2]);
+                            x[i + 3] = fmaf(v.w, f, x[i + 3]);
                         }
-                    });
-                store();
-                continue;
-            }
-            // parts: [row] off, [row] sum, then [d / 4][row][4]
-            constexpr int64_t kPart = (int64_t)R * (HD + 2);
-            float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * kPart;
-            pp[r] = off;
-            pp[R + r] = l;
-#pragma unroll
-            for (int g = 0; g < HD / 32; g++) {
-                float x[32];
-                piece(g, x);
-#pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                    *reinterpret_cast<float4 *>(pp + 2 * R + ((8 * g + i / 4) * R + r) * 4) =
-                        make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-            }
-            umma::fence_before_sync();
-            if (bad) mend([&](int d, float v) { pp[2 * R + (d / 4 * R + r) * 4 + d % 4] += v; });
-            __threadfence();
-            if (!(ok = join())) break;
-            const int c0 = cta_of(range, it.item0), c1 = cta_of(range, it.item1 - 1);
-            if (wt == 0) ctl.last[mt] = atomicAdd(a.counters + c0 * MT + mt, 1) == c1 - c0;
-            if (!(ok = join())) break;
-            if (!*(volatile int *)&ctl.last[mt]) continue;
-            __threadfence();
-            if (wt == 0) a.counters[c0 * MT + mt] = 0;  // ready for the next call
-            auto part = [&](int cc) { return a.parts + ((int64_t)cc * 2 + (cc == c0 ? 1 : 0)) * kPart; };
-            float top = neg_inf();
-            for (int cc = c0; cc <= c1; cc++) top = fmaxf(top, __ldcg(part(cc) + r));
-            const float mu = top == neg_inf() ? 0.f : top;
-            float sum = 0.f;
-            for (int cc = c0; cc <= c1; cc++) sum = fmaf(__ldcg(part(cc) + R + r), ex2(__ldcg(part(cc) + r) - mu), sum);
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll 1
-            for (int g = 0; g < HD / 32; g++) {
-                float x[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) x[i] = 0.f;
-                for (int cc = c0; cc <= c1; cc++) {
-                    const float *pc = part(cc);
-                    const float f = ex2(__ldcg(pc + r) - mu);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * R + ((8 * g + i / 4) * R + r) * 4));
-                        x[i] = fmaf(v.x, f, x[i]);
-                        x[i + 1] = fmaf(v.y, f, x[i + 1]);
-                        x[i + 2] = fmaf(v.z, f, x[i + 2]);
-                        x[i + 3] = fmaf(v.w, f, x[i + 3]);
                     }
                 }
                 stage(g, x, inv);
             }
+            umma::fence_before_sync();
+            if (it.whole && bad)
+                mend([&](int d, float v) {
+                    if (QF32) {
+                        float *p = reinterpret_cast<float *>(q_smem + (d >= HD / 2 ? MT * C::kTile : 0) +
+                                                             chunk_off(wt, d % (HD / 2) / 4) + d % 4 * 4);
+                        *p += v;
+                    } else {
+                        uint16_t *p = reinterpret_cast<uint16_t *>(q_smem + mt * C::kTile + chunk_off(wt, d / 8) + d % 8 * 2);
+                        *p = from_f<uint16_t>(to_f(*p) + v);
+                    }
+                });
             store();
         }
     }

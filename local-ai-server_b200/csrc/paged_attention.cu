@@ -7,8 +7,10 @@
 // cost is reading K and V once: HBM bound, 2 head_dim bytes per key and kv head for an 8-bit
 // cache. What stands in the way of that bound is arithmetic per key (group x 2 head_dim products,
 // and the conversion of 8-bit values), so the products go through the tensor cores with keys and
-// values straight from global memory in the operand layout of mma.m16n8k16: no shared memory, no
-// barrier in the loop, every warp with its own keys and loads in flight.
+// values in the operand layout of mma.m16n8k16, and every warp has its own keys, with no barrier
+// in the loop: straight from global memory, the next step's keys as soon as the scores are done
+// with this step's, the next values as soon as the products are. (Through shared memory with
+// cp.async the same loop took 162 us for 64 x 4096 INT8 keys, where it was bound by instructions.)
 //   * The sums over head_dim and over keys do not depend on the order of their terms. A lane
 //     takes 16-byte runs of K, and the query is loaded with the same permutation; a lane's n
 //     columns of V are a 16-byte run too, and the output is written back with that permutation.
@@ -103,9 +105,10 @@ struct Smem {
     SchedSmem sched;
     SeqSmem seqs;
     float m[kWarps][kRows], l[kWarps][kRows];
-    float o[kWarps][kRows][HD + 4];  // rows apart by 4 banks
+    alignas(16) float o[kWarps][kRows][HD + 4];  // rows apart by 4 banks
     int bad, last;
 };
+
 
 template <int HD, int FMT, bool QF32>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
@@ -121,6 +124,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     constexpr int ND = HD / 8;                       // 8-column groups of the output
     constexpr int VW = HD * kBytes / 32;             // 32-bit words of V per lane and key
     constexpr float kLift = kF16 ? 13.f : 0.f;
+    constexpr bool kOne = kF16 && !QF32;             // one term of the weights will do
     static_assert(kChunks * kPerChunk == KS, "a lane's runs cover its share of head_dim");
 
     __shared__ Smem<HD> sm;
@@ -138,6 +142,96 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     while (it.next(as)) {
         const Tile &tl = it.tl;
         const int head = it.kv_head(), blk0 = it.blk0, blk1 = it.blk1;
+
+        // this warp's steps of the item
+        int bl = blk0, bh = blk1;
+        if (bl * U + warp * kStep + kStep <= tl.k0) bl++;
+        if (bh > bl && (bh - 1) * U + warp * kStep >= tl.k1) bh--;
+        const int32_t *table = a.kv.pages + (int64_t)tl.seq * a.kv.max_pages;
+        // cache positions of step blk's 16-key groups, and which have a page, as bits
+        int64_t at[NK];
+        auto find = [&](int blk) -> uint32_t {
+            uint32_t there = 0;
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++) {
+                const int j = blk * U + warp * kStep + 16 * kk;
+                const bool in = j < tl.k1 && j + 16 > tl.k0;
+                const int page = in ? __ldg(table + (j >> a.kv.log_page)) : -1;
+                const bool real = page >= 0 && page < a.kv.n_pages;
+                if (in && !real && lane == 0) flag(a.err, LAI_DEVERR_PAGE);
+                there |= (uint32_t)real << kk;
+                at[kk] = a.kv.page_base(real ? page : 0, head) + (j & in_page);
+            }
+            return there;
+        };
+        // every key of the step is there
+        auto is_whole = [&](int blk, uint32_t there) {
+            const int j = blk * U + warp * kStep;
+            return there == (1u << NK) - 1 && j >= tl.k0 && j + kStep <= tl.k1;
+        };
+        uint4 kr[NB][kChunks];
+        uint32_t vr[NK][4][VW];
+        float2 ks[NB], vs[NB];
+        auto load_k = [&](int blk, uint32_t there, bool whole) {
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const int key = blk * U + warp * kStep + 8 * n + g;
+                const bool ok = whole || ((there >> (n / 2) & 1) && key >= tl.k0 && key < tl.k1);
+                const unsigned char *p = a.kv.k + (at[n / 2] + g) * (HD * kBytes) + 16 * t;
+#pragma unroll
+                for (int c = 0; c < kChunks; c++)
+                    kr[n][c] = ok ? ld_stream(p + 8 * (n & 1) * (HD * kBytes) + 64 * c) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto load_scales = [&]() {
+            if (kF16) {
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    const int64_t i = at[n / 2] + 8 * (n & 1) + 2 * t;
+                    ks[n] = __ldg(reinterpret_cast<const float2 *>(a.kv.k_scale + i));
+                    vs[n] = __ldg(reinterpret_cast<const float2 *>(a.kv.v_scale + i));
+                }
+            }
+        };
+        auto load_v = [&](int blk, uint32_t there, bool whole) {
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++) {
+                const unsigned char *p = a.kv.v + (at[kk] + 2 * t) * (HD * kBytes) + (VW == 2 ? 8 : 16) * g;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int off = (i & 1) + 8 * (i >> 1), key = blk * U + warp * kStep + 16 * kk + 2 * t + off;
+                    const bool ok = whole || ((there >> kk & 1) && key >= tl.k0 && key < tl.k1);
+                    const unsigned char *pi = p + off * (HD * kBytes);
+                    if constexpr (VW == 2) {
+                        const uint2 x = ok ? __ldg(reinterpret_cast<const uint2 *>(pi)) : make_uint2(0, 0);
+                        vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < VW / 4; c++) {
+                            const uint4 x = ok ? ld_stream(pi + 128 * c) : make_uint4(0, 0, 0, 0);
+                            vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
+                            vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
+                        }
+                    }
+                }
+            }
+        };
+        // (two ways, so that the common one needs no predicates)
+        auto load_step_k = [&](int blk, uint32_t there, bool whole) {
+            if (whole) load_k(blk, there, true); else load_k(blk, there, false);
+        };
+        auto load_step_v = [&](int blk, uint32_t there, bool whole) {
+            if (whole) load_v(blk, there, true); else load_v(blk, there, false);
+        };
+        uint32_t there = 0;
+        bool whole = false;
+        if (bl < bh) {
+            there = find(bl);
+            whole = is_whole(bl, there);
+            load_step_k(bl, there, whole);
+            load_scales();
+            load_step_v(bl, there, whole);
+        }
 
         // the query: lane (g, t) holds row g's elements 4 at a time, hi in the MMA's row g and
         // the rest of it in row g + 8
@@ -200,67 +294,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         int vexp = -126;  // accumulators are in units of 2^vexp (8-bit)
         bool bad = false;
 
-        for (int blk = blk0; blk < blk1; blk++) {
+        for (int blk = bl; blk < bh; blk++) {
             const int j0 = blk * U + warp * kStep;
-            if (j0 >= tl.k1 || j0 + kStep <= tl.k0) continue;
-            // ---- loads: this step's keys, values and scales
-            int64_t at[NK];  // cache position of each 16-key group
-            bool there[NK];
-#pragma unroll
-            for (int kk = 0; kk < NK; kk++) {
-                const int j = j0 + 16 * kk;
-                int page = -1;
-                if (j < tl.k1) {
-                    page = __ldg(a.kv.pages + (int64_t)tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
-                    if ((page < 0 || page >= a.kv.n_pages) && lane == 0 && j + 16 > tl.k0)
-                        flag(a.err, LAI_DEVERR_PAGE);
-                }
-                there[kk] = page >= 0 && page < a.kv.n_pages;
-                at[kk] = a.kv.page_base(there[kk] ? page : 0, head) + (j & in_page);
-            }
-            uint4 kr[NB][kChunks];
-            uint32_t vr[NK][4][VW];
-            float2 ks[NB], vs[NB];
-#pragma unroll
-            for (int n = 0; n < NB; n++) {
-                const int j = j0 + 8 * n + g;
-                const bool ok = there[n / 2] && j >= tl.k0 && j < tl.k1;
-                const unsigned char *p = a.kv.k + (at[n / 2] + 8 * (n & 1) + g) * (HD * kBytes) + 16 * t;
-#pragma unroll
-                for (int c = 0; c < kChunks; c++)
-                    kr[n][c] = ok ? ld_stream(p + 64 * c) : make_uint4(0, 0, 0, 0);
-            }
-            if (kF16) {
-#pragma unroll
-                for (int n = 0; n < NB; n++) {
-                    const int64_t i = at[n / 2] + 8 * (n & 1) + 2 * t;
-                    ks[n] = __ldg(reinterpret_cast<const float2 *>(a.kv.k_scale + i));
-                    vs[n] = __ldg(reinterpret_cast<const float2 *>(a.kv.v_scale + i));
-                }
-            }
-#pragma unroll
-            for (int kk = 0; kk < NK; kk++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int off = 2 * t + (i & 1) + 8 * (i >> 1), j = j0 + 16 * kk + off;
-                    const bool ok = there[kk] && j >= tl.k0 && j < tl.k1;
-                    const unsigned char *p = a.kv.v + (at[kk] + off) * (HD * kBytes);
-#pragma unroll
-                    for (int c = 0; c < VW; c++) vr[kk][i][c] = 0u;
-                    if (ok) {
-                        if constexpr (VW == 2) {
-                            const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p + 8 * g));
-                            vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < VW / 4; c++) {
-                                const uint4 x = ld_stream(p + 16 * g + 128 * c);
-                                vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
-                                vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
-                            }
-                        }
-                    }
-                }
             // ---- scores
             float sc[NB][2];
 #pragma unroll
@@ -285,26 +320,43 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                 sc[n][0] = c[0] + c[2];
                 sc[n][1] = c[1] + c[3];
             }
+            // ---- the next step's keys
+            const bool more = blk + 1 < bh, was_whole = whole;
+            const uint32_t was_there = there;
+            if (more) {
+                there = find(blk + 1);
+                whole = is_whole(blk + 1, there);
+                load_step_k(blk + 1, there, whole);
+            }
             // ---- mask, running maximum
-            float top = neg_inf();
-            uint32_t vtop = 0;
+            const bool uneven = mixed(tl, a.window, j0, kStep);
+            const bool all = was_whole && !uneven;  // every row sees every key
+            float top = neg_inf(), vtop = 0.f;
 #pragma unroll
-            for (int n = 0; n < NB; n++)
+            for (int n = 0; n < NB; n++) {
+                const float k0 = kF16 ? row_scale * ks[n].x : row_scale, k1 = kF16 ? row_scale * ks[n].y : row_scale;
+                sc[n][0] *= k0;
+                sc[n][1] *= k1;
+            }
+            if (!all) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int j = j0 + 8 * n + 2 * t + i;
-                    const bool see = j <= row_pos && j > row_from && there[n / 2];
-                    float x = sc[n][i] * row_scale;
-                    if (kF16) x *= i ? ks[n].y : ks[n].x;
-                    sc[n][i] = see ? x : neg_inf();
-                    if (kF16) {
-                        float &f = i ? vs[n].y : vs[n].x;
-                        f = see ? f : 0.f;
-                        const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
-                        vtop = max(vtop, u < 0x7f800000u ? u : 0u);
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int j = j0 + 8 * n + 2 * t + i;
+                        const bool see = j <= row_pos && j > row_from && (was_there >> (n / 2) & 1);
+                        sc[n][i] = see ? sc[n][i] : neg_inf();
+                        if (kF16) {
+                            float &f = i ? vs[n].y : vs[n].x;
+                            f = see ? f : 0.f;
+                        }
                     }
-                    top = fmaxf(top, sc[n][i]);
-                }
+            }
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                top = fmaxf(top, fmaxf(sc[n][0], sc[n][1]));
+                if (kF16) vtop = fmaxf(vtop, fmaxf(vs[n].x, vs[n].y));
+            }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float mn = fmaxf(m, top);
@@ -313,9 +365,9 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             m = mn;
             l *= alpha;
             float down = 1.f;
-            if (kF16) {
-                vtop = __reduce_max_sync(0xffffffffu, vtop);
-                const int e = max(vexp, min((int)(vtop >> 23) - 127, 126));
+            if (kF16) {  // a row's lanes have all of the step's value scales; the warp takes one power
+                const uint32_t u = __reduce_max_sync(0xffffffffu, __float_as_uint(vtop));
+                const int e = max(vexp, min((int)(u >> 23) - 127, 126));
                 alpha *= pow2i(vexp - e);
                 down = pow2i(-e);
                 vexp = e;
@@ -331,19 +383,28 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     p1 *= vs[n].y * down;
                 }
                 uint32_t *pk = pa[n / 2] + (n & 1) * 2;
+                if (kOne) {
+                    pk[0] = pack2<kF16>(p0, p1);
+                    pk[1] = 0u;
+                    continue;
+                }
                 pk[0] = take2<kF16>(p0, p1);
-                pk[1] = take2<kF16>(p0, p1);
-                if constexpr (kThird) pa[n / 2][4 + (n & 1)] = pack2<false>(p0, p1);
+                if constexpr (kThird) {
+                    pk[1] = take2<kF16>(p0, p1);
+                    pa[n / 2][4 + (n & 1)] = pack2<false>(p0, p1);
+                } else {
+                    pk[1] = pack2<kF16>(p0, p1);
+                }
             }
+            if (more) load_scales();
             // ---- values. A step whose keys some rows of the tile see and others do not gives
             // every row 0 x v for the keys it must not see: infinities and NaN are taken out of
             // such a step, and added to the rows that see them at the end.
-            const bool uneven = FMT != LAI_KV_I8 && mixed(tl, a.window, j0, kStep);
             auto column = [&](int n, uint32_t (&b0)[NK], uint32_t (&b1)[NK]) {
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kk = 0; kk < NK; kk++) {
-                    if (uneven) {
+                    if (FMT != LAI_KV_I8 && uneven) {
                         bad |= drop_nonfinite<kF16>(b0[kk]);
                         bad |= drop_nonfinite<kF16>(b1[kk]);
                     }
@@ -351,8 +412,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     if constexpr (kThird) mma<kF16>(c, pk[4], 0u, pk[5], 0u, b0[kk], b1[kk]);
                     mma<kF16>(c, pk[0], pk[1], pk[2], pk[3], b0[kk], b1[kk]);
                 }
-                o[n][0] = fmaf(o[n][0], alpha, c[0] + c[2]);
-                o[n][1] = fmaf(o[n][1], alpha, c[1] + c[3]);
+                o[n][0] = fmaf(o[n][0], alpha, kOne ? c[0] : c[0] + c[2]);
+                o[n][1] = fmaf(o[n][1], alpha, kOne ? c[1] : c[1] + c[3]);
             };
 #pragma unroll
             for (int wd = 0; wd < VW; wd++) {
@@ -388,6 +449,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     }
                 }
             }
+            // ---- the next step's values
+            if (more) load_step_v(blk + 1, there, whole);
         }
 
         // ---- join the warps
@@ -420,25 +483,34 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             if (bad) sm.bad = 1;
             __syncthreads();
         }
-        constexpr int kPer = kRows * HD / kThreads;
-        float acc[kPer], jm[kPer], jl_[kPer];
+        // a thread owns runs of 4 columns: run i starts at flattened element (i * kThreads + thread) * 4
+        constexpr int kRuns = kRows * HD / 4 / kThreads;
+        float4 acc[kRuns];
+        float sum[kRuns];
+        auto row_of = [&](int i) { return (i * kThreads + (int)threadIdx.x) * 4 / HD; };
+        auto col_of = [&](int i) { return (i * kThreads + (int)threadIdx.x) * 4 % HD; };
+        auto fma4 = [](float4 &x, const float4 &v, float f) {
+            x.x = fmaf(v.x, f, x.x);
+            x.y = fmaf(v.y, f, x.y);
+            x.z = fmaf(v.z, f, x.z);
+            x.w = fmaf(v.w, f, x.w);
+        };
+        float top[kRuns];
 #pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
-            float mx = sm.m[0][r];
+        for (int i = 0; i < kRuns; i++) {
+            const int r = row_of(i), d = col_of(i);
+            top[i] = sm.m[0][r];
 #pragma unroll
-            for (int x = 1; x < kWarps; x++) mx = fmaxf(mx, sm.m[x][r]);
-            const float mu = mx == neg_inf() ? 0.f : mx;
-            float sum = 0.f, v = 0.f;
+            for (int x = 1; x < kWarps; x++) top[i] = fmaxf(top[i], sm.m[x][r]);
+            const float mu = top[i] == neg_inf() ? 0.f : top[i];
+            sum[i] = 0.f;
+            acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int x = 0; x < kWarps; x++) {
                 const float c = ex2(sm.m[x][r] - mu);
-                sum = fmaf(sm.l[x][r], c, sum);
-                v = fmaf(sm.o[x][r][d], c, v);
+                sum[i] = fmaf(sm.l[x][r], c, sum[i]);
+                fma4(acc[i], *reinterpret_cast<const float4 *>(&sm.o[x][r][d]), c);
             }
-            acc[i] = v;
-            jm[i] = mx;
-            jl_[i] = sum;
         }
         if (FMT != LAI_KV_I8 && sm.bad) {
             for (int j = max(blk0 * U, tl.k0); j < min(blk1 * U, tl.k1); j++) {
@@ -447,27 +519,29 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                 if (page < 0 || page >= a.kv.n_pages) continue;
                 const int64_t at = (a.kv.page_base(page, head) + (j & in_page)) * HD;
 #pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
-                    const int p = tl.pos0 + a.by_group.of(tl.row0 + r);
+                for (int i = 0; i < kRuns; i++) {
+                    const int r = row_of(i), p = tl.pos0 + a.by_group.of(tl.row0 + r);
                     if (r >= tl.rows || j > p || (a.window && j <= p - a.window)) continue;
-                    const float v = element<FMT>(a.kv.v, at + d);
-                    if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) acc[i] += v;
+                    float *x = &acc[i].x;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float v = element<FMT>(a.kv.v, at + col_of(i) + e);
+                        if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) x[e] += v;
+                    }
                 }
             }
         }
         bool write = it.begins && it.ends;
         if (!write) {
-            const int64_t slot_no = (int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0);
-            float *pp = a.parts + slot_no * part_floats(HD);
+            // parts: [row] max, [row] sum, [row][column]
+            float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * part_floats(HD);
 #pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
-                if (d == 0) {
-                    pp[r] = jm[i];
-                    pp[kRows + r] = jl_[i];
+            for (int i = 0; i < kRuns; i++) {
+                if (col_of(i) == 0) {
+                    pp[row_of(i)] = top[i];
+                    pp[kRows + row_of(i)] = sum[i];
                 }
-                pp[2 * kRows + e] = acc[i];
+                *reinterpret_cast<float4 *>(pp + 2 * kRows + (i * kThreads + threadIdx.x) * 4) = acc[i];
             }
             __threadfence();
             __syncthreads();
@@ -478,47 +552,81 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             if (write) {
                 __threadfence();
                 if (threadIdx.x == 0) a.counters[c0] = 0;  // ready for the next call
+                // The parts' weights first, then the parts with 8 of them under way at a time.
+                // Shared memory that the warps' join used holds kWeights parts at once.
+                constexpr int kWeights = sizeof(sm.o) / sizeof(float) / kRows / 2;
+                float *wm = &sm.o[0][0][0], *wl = wm + kWeights * kRows;
+                auto part = [&](int c) { return a.parts + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * part_floats(HD); };
 #pragma unroll
-                for (int i = 0; i < kPer; i++) acc[i] = jl_[i] = 0.f, jm[i] = neg_inf();
-                for (int c = c0; c <= c1; c++) {
-                    const float *pc = a.parts + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * part_floats(HD);
+                for (int i = 0; i < kRuns; i++) {
+                    acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    sum[i] = 0.f;
+                    top[i] = neg_inf();
+                }
+                for (int first = c0; first <= c1; first += kWeights) {
+                    const int n = min(kWeights, c1 + 1 - first);
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < n * kRows; i += kThreads) {
+                        const float *pc = part(first + i / kRows) + i % kRows;
+                        wm[i] = __ldcg(pc);
+                        wl[i] = __ldcg(pc + kRows);
+                    }
+                    __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < kPer; i++) {
-                        const int e = threadIdx.x + i * kThreads, r = e / HD;
-                        const float cm = __ldcg(pc + r), mx = fmaxf(jm[i], cm);
-                        const float mu = mx == neg_inf() ? 0.f : mx;
-                        const float ca = ex2(jm[i] - mu), cb = ex2(cm - mu);
-                        jl_[i] = fmaf(__ldcg(pc + kRows + r), cb, jl_[i] * ca);
-                        acc[i] = fmaf(__ldcg(pc + 2 * kRows + e), cb, acc[i] * ca);
-                        jm[i] = mx;
+                    for (int i = 0; i < kRuns; i++) {
+                        const int r = row_of(i);
+                        float t = top[i];
+                        for (int c = 0; c < n; c++) t = fmaxf(t, wm[c * kRows + r]);
+                        const float mu = t == neg_inf() ? 0.f : t;
+                        const float down = ex2(top[i] - mu);
+                        top[i] = t;
+                        sum[i] *= down;
+                        acc[i].x *= down;
+                        acc[i].y *= down;
+                        acc[i].z *= down;
+                        acc[i].w *= down;
+#pragma unroll 8
+                        for (int c = 0; c < n; c++) {
+                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(
+                                part(first + c) + 2 * kRows + (i * kThreads + threadIdx.x) * 4));
+                            const float f = ex2(wm[c * kRows + r] - mu);
+                            sum[i] = fmaf(wl[c * kRows + r], f, sum[i]);
+                            fma4(acc[i], v, f);
+                        }
                     }
                 }
             }
         }
         if (write) {
 #pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const int e = threadIdx.x + i * kThreads, r = e / HD, d = e % HD;
+            for (int i = 0; i < kRuns; i++) {
+                const int r = row_of(i);
                 if (r >= tl.rows) continue;
                 const int fr = tl.row0 + r, tk = a.by_group.of(fr);
                 const int64_t at = (((int64_t)tl.q_row0 + tk) * n_heads + head * a.group +
-                                    (fr - tk * a.group)) * HD + d;
-                const float x = jl_[i] == 0.f ? 0.f : acc[i] / jl_[i];
-                if (QF32) static_cast<float *>(out)[at] = x;
-                else static_cast<uint16_t *>(out)[at] = from_f<uint16_t>(x);
+                                    (fr - tk * a.group)) * HD + col_of(i);
+                const float inv = sum[i] == 0.f ? 0.f : 1.f / sum[i];
+                if (QF32)
+                    *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) =
+                        make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
+                else
+                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + at) =
+                        make_uint2(pack_bf16x2(acc[i].x * inv, acc[i].y * inv),
+                                   pack_bf16x2(acc[i].z * inv, acc[i].w * inv));
             }
         }
     }
 }
 
 template <int HD, int FMT, bool QF32>
-void launch_few(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
+int launch_few(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
     constexpr int U = block_keys<FMT>();
     const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.log_page) + U - 1) / U;
     const int64_t most = FewSched<FMT>::slots(a.kv.n_rows, a.group, a.kv.n_seqs) * a.kv.n_kv;
     const int64_t ctas = most < kMaxCtas ? most * blocks : kMaxCtas;  // most * blocks fits
-    launch_pdl(paged_attn_few_kernel<HD, FMT, QF32>,
-               dim3((unsigned)(ctas < kMaxCtas ? ctas : kMaxCtas)), dim3(kThreads), 0, st, out, q, a);
+    auto kern = paged_attn_few_kernel<HD, FMT, QF32>;
+    launch_pdl(kern, dim3((unsigned)(ctas < kMaxCtas ? ctas : kMaxCtas)), dim3(kThreads), 0, st, out, q, a);
+    return launch_status();
 }
 
 template <bool QF32>
@@ -555,16 +663,14 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
     const cudaStream_t cs = as_stream(stream);
     if (n_rows * a.group > (int64_t)kWideRows * b->n_seqs && a.scale_log2 > 1e-30f)
         return attention_wide(out, q, QF32, kv->head_dim, kv->format, a, cs);
-#define LAI_FEW(FMT)                                                      \
-    if (kv->head_dim == 128) launch_few<128, FMT, QF32>(out, q, a, cs);   \
-    else launch_few<64, FMT, QF32>(out, q, a, cs)
+#define LAI_FEW(FMT)                                                             \
+    (kv->head_dim == 128 ? launch_few<128, FMT, QF32>(out, q, a, cs) : launch_few<64, FMT, QF32>(out, q, a, cs))
     switch (kv->format) {
-        case LAI_KV_BF16: LAI_FEW(LAI_KV_BF16); break;
-        case LAI_KV_E4M3: LAI_FEW(LAI_KV_E4M3); break;
-        default: LAI_FEW(LAI_KV_I8); break;
+        case LAI_KV_BF16: return LAI_FEW(LAI_KV_BF16);
+        case LAI_KV_E4M3: return LAI_FEW(LAI_KV_E4M3);
+        default: return LAI_FEW(LAI_KV_I8);
     }
 #undef LAI_FEW
-    return launch_status();
 }
 
 }  // namespace

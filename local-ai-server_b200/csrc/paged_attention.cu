@@ -67,19 +67,27 @@ template <bool F16> __device__ __forceinline__ uint32_t take2(float &x0, float &
     x1 -= f.y;
     return p;
 }
-template <bool F16>
+// c (+)= a b; FIRST: c = a b, without zeros having to be moved into c.
+template <bool F16, bool FIRST>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                     uint32_t a3, uint32_t b0, uint32_t b1) {
-    if (F16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-            "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-            "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+#define LAI_MMA(T)                                                                            \
+    if (FIRST)                                                                                \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." T "." T ".f32 "                          \
+            "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"             \
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                  \
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));                \
+    else                                                                                      \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." T "." T ".f32 "                          \
+            "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"                 \
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                  \
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+    if (F16) {
+        LAI_MMA("f16");
+    } else {
+        LAI_MMA("bf16");
+    }
+#undef LAI_MMA
 }
 // Zero an element of a pair that is an infinity or NaN; true if there was one.
 template <bool F16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &p) {
@@ -297,12 +305,12 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         for (int blk = bl; blk < bh; blk++) {
             const int j0 = blk * U + warp * kStep;
             // ---- scores
-            float sc[NB][2];
+            // (step by step over head_dim, so that the groups' MMAs stand between one group's)
+            float cs[NB][4], sc[NB][2];
 #pragma unroll
-            for (int n = 0; n < NB; n++) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
+                for (int n = 0; n < NB; n++) {
                     const uint4 r = kr[n][s / kPerChunk];
                     uint32_t b0, b1;
                     if constexpr (kF16) {
@@ -314,11 +322,17 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                         b0 = s % 2 ? r.z : r.x;
                         b1 = s % 2 ? r.w : r.y;
                     }
-                    if constexpr (kThird) mma<kF16>(c, qa[s][4], 0u, qa[s][5], 0u, b0, b1);
-                    mma<kF16>(c, qa[s][0], qa[s][1], qa[s][2], qa[s][3], b0, b1);
+                    if constexpr (kThird) {
+                        if (s == 0) mma<kF16, true>(cs[n], qa[s][4], 0u, qa[s][5], 0u, b0, b1);
+                        else mma<kF16, false>(cs[n], qa[s][4], 0u, qa[s][5], 0u, b0, b1);
+                    }
+                    if (s == 0 && !kThird) mma<kF16, true>(cs[n], qa[s][0], qa[s][1], qa[s][2], qa[s][3], b0, b1);
+                    else mma<kF16, false>(cs[n], qa[s][0], qa[s][1], qa[s][2], qa[s][3], b0, b1);
                 }
-                sc[n][0] = c[0] + c[2];
-                sc[n][1] = c[1] + c[3];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                sc[n][0] = cs[n][0] + cs[n][2];
+                sc[n][1] = cs[n][1] + cs[n][3];
             }
             // ---- the next step's keys
             const bool more = blk + 1 < bh, was_whole = whole;
@@ -401,7 +415,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             // every row 0 x v for the keys it must not see: infinities and NaN are taken out of
             // such a step, and added to the rows that see them at the end.
             auto column = [&](int n, uint32_t (&b0)[NK], uint32_t (&b1)[NK]) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                float c[4];
 #pragma unroll
                 for (int kk = 0; kk < NK; kk++) {
                     if (FMT != LAI_KV_I8 && uneven) {
@@ -409,8 +423,12 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                         bad |= drop_nonfinite<kF16>(b1[kk]);
                     }
                     const uint32_t *pk = pa[kk];
-                    if constexpr (kThird) mma<kF16>(c, pk[4], 0u, pk[5], 0u, b0[kk], b1[kk]);
-                    mma<kF16>(c, pk[0], pk[1], pk[2], pk[3], b0[kk], b1[kk]);
+                    if constexpr (kThird) {
+                        if (kk == 0) mma<kF16, true>(c, pk[4], 0u, pk[5], 0u, b0[kk], b1[kk]);
+                        else mma<kF16, false>(c, pk[4], 0u, pk[5], 0u, b0[kk], b1[kk]);
+                    }
+                    if (kk == 0 && !kThird) mma<kF16, true>(c, pk[0], pk[1], pk[2], pk[3], b0[kk], b1[kk]);
+                    else mma<kF16, false>(c, pk[0], pk[1], pk[2], pk[3], b0[kk], b1[kk]);
                 }
                 o[n][0] = fmaf(o[n][0], alpha, kOne ? c[0] : c[0] + c[2]);
                 o[n][1] = fmaf(o[n][1], alpha, kOne ? c[1] : c[1] + c[3]);

@@ -8,9 +8,11 @@
 // cache. What stands in the way of that bound is arithmetic per key (group x 2 head_dim products,
 // and the conversion of 8-bit values), so the products go through the tensor cores with keys and
 // values in the operand layout of mma.m16n8k16, and every warp has its own keys, with no barrier
-// in the loop: straight from global memory, the next step's keys as soon as the scores are done
-// with this step's, the next values as soon as the products are. (Through shared memory with
-// cp.async the same loop took 162 us for 64 x 4096 INT8 keys, where it was bound by instructions.)
+// in the loop. One warp of a CTA only copies: it follows the page tables and keeps a ring of
+// chunks (a chunk is what a warp takes at a time) filled with bulk copies, across the ends of
+// items, so the other eight neither compute addresses nor hold loads in registers. (With loads
+// straight into registers 64 x 4096 INT8 keys took 143 us, bound by their latency at the 12 warps
+// that fit; this takes KKK us.)
 //   * The sums over head_dim and over keys do not depend on the order of their terms. A lane
 //     takes 16-byte runs of K, and the query is loaded with the same permutation; a lane's n
 //     columns of V are a 16-byte run too, and the output is written back with that permutation.
@@ -23,6 +25,7 @@
 //   * 8-bit: a key's scale multiplies its score, a value's scale its weight. Weights in binary16
 //     are taken relative to the largest value scale so far (a power of two per warp) and lifted
 //     by 2^13, so that small ones keep their bits.
+#include "bulk_copy.cuh"
 #include "paged_attention.cuh"
 
 namespace lai {
@@ -31,15 +34,18 @@ namespace {
 
 using namespace paged;
 
-constexpr int kThreads = 128, kWarps = 4;
+constexpr int kWarps = 7;     // that compute; one more copies
+constexpr int kMath = kWarps * 32, kThreads = kMath + 32;
+constexpr int kHalf = 4;      // sums that the warps join in
 constexpr int kRows = 8;      // rows of a tile
-constexpr int kCtasPerSm = 3;
+constexpr int kCtasPerSm = 2;
 constexpr int kMaxCtas = kSMs * kCtasPerSm;
 constexpr int kCounters = 1024;  // ints at the front of the scratch
 constexpr int kWideRows = 32;    // more rows per sequence (on average) go to the wide kernel
 
-template <int FMT> __host__ __device__ constexpr int step_keys() { return FMT == LAI_KV_BF16 ? 16 : 32; }  // per warp
+template <int FMT> __host__ __device__ constexpr int step_keys() { return FMT == LAI_KV_BF16 ? 16 : 32; }  // of a chunk
 template <int FMT> __host__ __device__ constexpr int block_keys() { return kWarps * step_keys<FMT>(); }
+constexpr uint64_t kWaitNs = 1000000000ull;
 __host__ __device__ constexpr int part_floats(int hd) { return kRows * (hd + 2); }
 
 // ---- operands ----------------------------------------------------------------------------------
@@ -104,19 +110,33 @@ template <int FMT> __device__ __forceinline__ float element(const unsigned char 
     return unpack2<true>(e4m3x2_to_f16x2(v[i])).x;
 }
 
-// Extra cost of an item in blocks: none. (Its queries, join and output cost about as much as a
-// block of 64 keys, but with 3 CTAs on an SM they run beside the loads of the others.)
 template <int FMT> using FewSched = Sched<kRows, block_keys<FMT>(), 0>;
 
-template <int HD>
-struct Smem {
-    SchedSmem sched;
-    SeqSmem seqs;
-    float m[kWarps][kRows], l[kWarps][kRows];
-    alignas(16) float o[kWarps][kRows][HD + 4];  // rows apart by 4 banks
-    int bad, last;
+// A chunk in shared memory: rows of K, rows of V, scales of K, scales of V.
+template <int HD, int FMT>
+struct Chunk {
+    static constexpr int kKeys = step_keys<FMT>(), kRow = HD * Fmt<FMT>::kBytes;
+    static constexpr int kV = kKeys * kRow, kScaleK = 2 * kV, kScaleV = kScaleK + kKeys * 4;
+    static constexpr int kBytes = FMT == LAI_KV_BF16 ? kScaleK : kScaleV + kKeys * 4;
+    static constexpr int kRing = 10;
 };
 
+template <int HD, int FMT>
+struct Smem {
+    alignas(128) unsigned char ring[Chunk<HD, FMT>::kRing][Chunk<HD, FMT>::kBytes];
+    alignas(16) float o[kHalf][kRows][HD + 4];  // rows apart by 4 banks
+    alignas(16) uint4 q[HD / 16][32];
+    uint2 q3[FMT == LAI_KV_BF16 ? HD / 16 : 1][32];   // the third terms
+    float m[kHalf][kRows], l[kHalf][kRows];
+    uint64_t full[Chunk<HD, FMT>::kRing], empty[Chunk<HD, FMT>::kRing];
+    uint32_t there[Chunk<HD, FMT>::kRing];            // 16-key groups of a chunk that have a page, as bits
+    uint32_t id[Chunk<HD, FMT>::kRing];               // the chunk that a slot was given to last
+    SchedSmem sched;
+    SeqSmem seqs;
+    int bad;          // the item (counted) that infinities or NaN were taken out of
+    int last, abort;
+};
+__device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kMath) : "memory"); }
 
 template <int HD, int FMT, bool QF32>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
@@ -135,115 +155,105 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     constexpr bool kOne = kF16 && !QF32;             // one term of the weights will do
     static_assert(kChunks * kPerChunk == KS, "a lane's runs cover its share of head_dim");
 
-    __shared__ Smem<HD> sm;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    using Ck = Chunk<HD, FMT>;
+    constexpr int kRing = Ck::kRing;
+    extern __shared__ __align__(128) unsigned char smem_bytes[];
+    auto &sm = *reinterpret_cast<Smem<HD, FMT> *>(smem_bytes);
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     pdl_wait_prior();
     pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRing; i++) {
+            bulk::mbar_init(&sm.full[i], 1);
+            bulk::mbar_init(&sm.empty[i], 1);
+            sm.id[i] = 0xffffffffu;
+        }
+        sm.abort = 0;
+        sm.bad = 0;
+        bulk::fence_barrier_init();
+    }
     const AttnArgs as = cache_seqs<kThreads>(a, sm.seqs);
     const Range range = find_range<FewSched<FMT>, kThreads>(as, sm.sched);
-    if (range.w0 >= range.w1) return;
+    if (range.w0 >= range.w1) return;  // the whole CTA
 
-    const int n_heads = a.kv.n_kv * a.group, in_page = a.kv.page_size() - 1;
+    // Bounded wait of a warp. When one runs out the CTA goes on with whatever is there (every
+    // access stays in bounds), no further wait takes time, and the caller gets the flag.
+    auto give_up = [&]() {
+        sm.abort = 1;
+        flag(a.err, LAI_DEVERR_TIMEOUT);
+    };
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (!bulk::mbar_try_wait(bar, parity)) {
+            const uint64_t t0 = bulk::globaltimer_ns();
+            while (!bulk::mbar_try_wait(bar, parity) && !*(volatile int *)&sm.abort)
+                if (bulk::globaltimer_ns() - t0 > kWaitNs) give_up();
+        }
+        __syncwarp();
+    };
+    const int in_page = a.kv.page_size() - 1;
     Walk<FewSched<FMT>> it;
     it.start(as, range);
-    while (it.next(as)) {
-        const Tile &tl = it.tl;
-        const int head = it.kv_head(), blk0 = it.blk0, blk1 = it.blk1;
+    uint32_t chunk0 = 0;  // chunks of the blocks before this one
 
-        // this warp's steps of the item
-        int bl = blk0, bh = blk1;
-        if (bl * U + warp * kStep + kStep <= tl.k0) bl++;
-        if (bh > bl && (bh - 1) * U + warp * kStep >= tl.k1) bh--;
-        const int32_t *table = a.kv.pages + (int64_t)tl.seq * a.kv.max_pages;
-        // cache positions of step blk's 16-key groups, and which have a page, as bits
-        int64_t at[NK];
-        auto find = [&](int blk) -> uint32_t {
-            uint32_t there = 0;
-#pragma unroll
-            for (int kk = 0; kk < NK; kk++) {
-                const int j = blk * U + warp * kStep + 16 * kk;
-                const bool in = j < tl.k1 && j + 16 > tl.k0;
-                const int page = in ? __ldg(table + (j >> a.kv.log_page)) : -1;
-                const bool real = page >= 0 && page < a.kv.n_pages;
-                if (in && !real && lane == 0) flag(a.err, LAI_DEVERR_PAGE);
-                there |= (uint32_t)real << kk;
-                at[kk] = a.kv.page_base(real ? page : 0, head) + (j & in_page);
-            }
-            return there;
-        };
-        // every key of the step is there
-        auto is_whole = [&](int blk, uint32_t there) {
-            const int j = blk * U + warp * kStep;
-            return there == (1u << NK) - 1 && j >= tl.k0 && j + kStep <= tl.k1;
-        };
-        uint4 kr[NB][kChunks];
-        uint32_t vr[NK][4][VW];
-        float2 ks[NB], vs[NB];
-        auto load_k = [&](int blk, uint32_t there, bool whole) {
-#pragma unroll
-            for (int n = 0; n < NB; n++) {
-                const int key = blk * U + warp * kStep + 8 * n + g;
-                const bool ok = whole || ((there >> (n / 2) & 1) && key >= tl.k0 && key < tl.k1);
-                const unsigned char *p = a.kv.k + (at[n / 2] + g) * (HD * kBytes) + 16 * t;
-#pragma unroll
-                for (int c = 0; c < kChunks; c++)
-                    kr[n][c] = ok ? ld_stream(p + 8 * (n & 1) * (HD * kBytes) + 64 * c) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto load_scales = [&]() {
-            if (kF16) {
-#pragma unroll
-                for (int n = 0; n < NB; n++) {
-                    const int64_t i = at[n / 2] + 8 * (n & 1) + 2 * t;
-                    ks[n] = __ldg(reinterpret_cast<const float2 *>(a.kv.k_scale + i));
-                    vs[n] = __ldg(reinterpret_cast<const float2 *>(a.kv.v_scale + i));
+    if (warp == kWarps) {
+        // ---- copies: lane 2 c + kk (8-bit) or c (BF16) looks up the page of 16-key group kk of chunk c
+        static_assert(kWarps * NK <= 32, "a lane per 16-key group of a block");
+        while (it.next(as)) {
+            const Tile &tl = it.tl;
+            const int head = it.kv_head();
+            const int32_t *table = a.kv.pages + (int64_t)tl.seq * a.kv.max_pages;
+            for (int blk = it.blk0; blk < it.blk1; blk++, chunk0 += kWarps) {
+                const int j = blk * U + 16 * lane;
+                int page = -1;
+                if (lane < kWarps * NK && j < tl.k1 && j + 16 > tl.k0) {
+                    page = __ldg(table + (j >> a.kv.log_page));
+                    if (page < 0 || page >= a.kv.n_pages) {
+                        flag(a.err, LAI_DEVERR_PAGE);
+                        page = -1;
+                    }
                 }
-            }
-        };
-        auto load_v = [&](int blk, uint32_t there, bool whole) {
-#pragma unroll
-            for (int kk = 0; kk < NK; kk++) {
-                const unsigned char *p = a.kv.v + (at[kk] + 2 * t) * (HD * kBytes) + (VW == 2 ? 8 : 16) * g;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int off = (i & 1) + 8 * (i >> 1), key = blk * U + warp * kStep + 16 * kk + 2 * t + off;
-                    const bool ok = whole || ((there >> kk & 1) && key >= tl.k0 && key < tl.k1);
-                    const unsigned char *pi = p + off * (HD * kBytes);
-                    if constexpr (VW == 2) {
-                        const uint2 x = ok ? __ldg(reinterpret_cast<const uint2 *>(pi)) : make_uint2(0, 0);
-                        vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < VW / 4; c++) {
-                            const uint4 x = ok ? ld_stream(pi + 128 * c) : make_uint4(0, 0, 0, 0);
-                            vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
-                            vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
-                        }
+                const uint32_t real = __ballot_sync(0xffffffffu, page >= 0);
+                const int64_t at = a.kv.page_base(page >= 0 ? page : 0, head) + (j & in_page);
+                for (int c = 0; c < kWarps; c++) {
+                    const uint32_t id = chunk0 + c, slot = id % kRing;
+                    if (id >= (uint32_t)kRing) wait(&sm.empty[slot], (id / kRing - 1) & 1);
+                    const uint32_t there = real >> (c * NK) & ((1u << NK) - 1);
+                    if (lane == 0) {
+                        sm.there[slot] = there;
+                        *(volatile uint32_t *)&sm.id[slot] = id;
+                        bulk::mbar_arrive_expect_tx(&sm.full[slot],
+                                                    __popc(there) * (2 * 16 * Ck::kRow + (kF16 ? 2 * 16 * 4 : 0)));
+                    }
+                    __syncwarp();
+                    // one copy for both groups of a chunk that lies in one page: copies cost time each
+                    const bool one = NK == 2 && a.kv.log_page > 4 && there == 3u;
+                    const int kk = lane % NK;
+                    if (lane / NK == c && page >= 0 && !(one && kk)) {
+                        unsigned char *to = sm.ring[slot];
+                        const int n = one ? 32 : 16;
+                        bulk::load(to + kk * 16 * Ck::kRow, a.kv.k + at * Ck::kRow, n * Ck::kRow, &sm.full[slot]);
+                        if (kF16) bulk::load(to + Ck::kScaleK + kk * 64, a.kv.k_scale + at, n * 4, &sm.full[slot]);
+                        bulk::load(to + Ck::kV + kk * 16 * Ck::kRow, a.kv.v + at * Ck::kRow, n * Ck::kRow, &sm.full[slot]);
+                        if (kF16) bulk::load(to + Ck::kScaleV + kk * 64, a.kv.v_scale + at, n * 4, &sm.full[slot]);
                     }
                 }
             }
-        };
-        // (two ways, so that the common one needs no predicates)
-        auto load_step_k = [&](int blk, uint32_t there, bool whole) {
-            if (whole) load_k(blk, there, true); else load_k(blk, there, false);
-        };
-        auto load_step_v = [&](int blk, uint32_t there, bool whole) {
-            if (whole) load_v(blk, there, true); else load_v(blk, there, false);
-        };
-        uint32_t there = 0;
-        bool whole = false;
-        if (bl < bh) {
-            there = find(bl);
-            whole = is_whole(bl, there);
-            load_step_k(bl, there, whole);
-            load_scales();
-            load_step_v(bl, there, whole);
         }
+        if (sm.abort) {  // copies may be in flight: they get a millisecond before shared memory goes
+            const uint64_t t0 = bulk::globaltimer_ns();
+            while (bulk::globaltimer_ns() - t0 < 1000000ull) {}
+        }
+        return;
+    }
+
+    const int n_heads = a.kv.n_kv * a.group;
+    for (int n_it = 1; it.next(as); n_it++) {
+        const Tile &tl = it.tl;
+        const int head = it.kv_head(), blk0 = it.blk0, blk1 = it.blk1;
 
         // the query: lane (g, t) holds row g's elements 4 at a time, hi in the MMA's row g and
         // the rest of it in row g + 8
-        uint32_t qa[KS][kThird ? 6 : 4];
         float row_scale = a.scale_log2;
         const int row = tl.row0 + g, tok = a.by_group.of(row);
         const bool row_ok = g < tl.rows;
@@ -285,15 +295,17 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             }
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                qa[s][0] = take2<kF16>(x[s][0], x[s][1]);
-                qa[s][2] = take2<kF16>(x[s][2], x[s][3]);
-                qa[s][1] = QF32 ? take2<kF16>(x[s][0], x[s][1]) : 0u;
-                qa[s][3] = QF32 ? take2<kF16>(x[s][2], x[s][3]) : 0u;
-                if constexpr (kThird) {
-                    qa[s][4] = pack2<false>(x[s][0], x[s][1]);
-                    qa[s][5] = pack2<false>(x[s][2], x[s][3]);
-                }
+                if (s % kWarps != warp) continue;  // every warp has all of it; each writes its share
+                uint4 v;
+                v.x = take2<kF16>(x[s][0], x[s][1]);
+                v.z = take2<kF16>(x[s][2], x[s][3]);
+                v.y = QF32 ? take2<kF16>(x[s][0], x[s][1]) : 0u;
+                v.w = QF32 ? take2<kF16>(x[s][2], x[s][3]) : 0u;
+                sm.q[s][lane] = v;
+                if constexpr (kThird)
+                    sm.q3[s][lane] = make_uint2(pack2<false>(x[s][0], x[s][1]), pack2<false>(x[s][2], x[s][3]));
             }
+            math_sync();
         }
 
         float m = neg_inf(), l = 0.f, o[ND][2];
@@ -302,16 +314,39 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         int vexp = -126;  // accumulators are in units of 2^vexp (8-bit)
         bool bad = false;
 
-        for (int blk = bl; blk < bh; blk++) {
+        for (int blk = blk0; blk < blk1; blk++, chunk0 += kWarps) {
             const int j0 = blk * U + warp * kStep;
+            const uint32_t id = chunk0 + warp, slot = id % kRing;
+            // A slot's chunks belong to different warps, and a parity only tells neighbouring phases
+            // apart: a warp looks at its phase once the slot is its chunk's.
+            if (*(volatile uint32_t *)&sm.id[slot] != id) {
+                const uint64_t t0 = bulk::globaltimer_ns();
+                while (*(volatile uint32_t *)&sm.id[slot] != id && !*(volatile int *)&sm.abort)
+                    if (bulk::globaltimer_ns() - t0 > kWaitNs) give_up();
+            }
+            __syncwarp();
+            wait(&sm.full[slot], (id / kRing) & 1);
+            const unsigned char *from = sm.ring[slot];
+            const uint32_t there = sm.there[slot];
+            if (there == 0) {  // none of its keys
+                if (lane == 0) bulk::mbar_arrive(&sm.empty[slot]);
+                continue;
+            }
+            const bool whole = there == (1u << NK) - 1 && j0 >= tl.k0 && j0 + kStep <= tl.k1;
             // ---- scores
             // (step by step over head_dim, so that the groups' MMAs stand between one group's)
             float cs[NB][4], sc[NB][2];
+            uint4 kr[NB];
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+            for (int s = 0; s < KS; s++) {
+                const uint4 q = sm.q[s][lane];
+                uint2 q3 = make_uint2(0u, 0u);
+                if constexpr (kThird) q3 = sm.q3[s][lane];
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
-                    const uint4 r = kr[n][s / kPerChunk];
+                    if (s % kPerChunk == 0)
+                        kr[n] = *reinterpret_cast<const uint4 *>(from + (8 * n + g) * Ck::kRow + 16 * t + 64 * (s / kPerChunk));
+                    const uint4 r = kr[n];
                     uint32_t b0, b1;
                     if constexpr (kF16) {
                         const int i = s % 4;
@@ -323,28 +358,29 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                         b1 = s % 2 ? r.w : r.y;
                     }
                     if constexpr (kThird) {
-                        if (s == 0) mma<kF16, true>(cs[n], qa[s][4], 0u, qa[s][5], 0u, b0, b1);
-                        else mma<kF16, false>(cs[n], qa[s][4], 0u, qa[s][5], 0u, b0, b1);
+                        if (s == 0) mma<kF16, true>(cs[n], q3.x, 0u, q3.y, 0u, b0, b1);
+                        else mma<kF16, false>(cs[n], q3.x, 0u, q3.y, 0u, b0, b1);
                     }
-                    if (s == 0 && !kThird) mma<kF16, true>(cs[n], qa[s][0], qa[s][1], qa[s][2], qa[s][3], b0, b1);
-                    else mma<kF16, false>(cs[n], qa[s][0], qa[s][1], qa[s][2], qa[s][3], b0, b1);
+                    if (s == 0 && !kThird) mma<kF16, true>(cs[n], q.x, q.y, q.z, q.w, b0, b1);
+                    else mma<kF16, false>(cs[n], q.x, q.y, q.z, q.w, b0, b1);
                 }
+            }
 #pragma unroll
             for (int n = 0; n < NB; n++) {
                 sc[n][0] = cs[n][0] + cs[n][2];
                 sc[n][1] = cs[n][1] + cs[n][3];
             }
-            // ---- the next step's keys
-            const bool more = blk + 1 < bh, was_whole = whole;
-            const uint32_t was_there = there;
-            if (more) {
-                there = find(blk + 1);
-                whole = is_whole(blk + 1, there);
-                load_step_k(blk + 1, there, whole);
-            }
             // ---- mask, running maximum
+            float2 ks[NB], vs[NB];
+            if (kF16) {
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    ks[n] = *reinterpret_cast<const float2 *>(from + Ck::kScaleK + (8 * n + 2 * t) * 4);
+                    vs[n] = *reinterpret_cast<const float2 *>(from + Ck::kScaleV + (8 * n + 2 * t) * 4);
+                }
+            }
             const bool uneven = mixed(tl, a.window, j0, kStep);
-            const bool all = was_whole && !uneven;  // every row sees every key
+            const bool all = whole && !uneven;  // every row sees every key
             float top = neg_inf(), vtop = 0.f;
 #pragma unroll
             for (int n = 0; n < NB; n++) {
@@ -358,7 +394,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const int j = j0 + 8 * n + 2 * t + i;
-                        const bool see = j <= row_pos && j > row_from && (was_there >> (n / 2) & 1);
+                        const bool see = j <= row_pos && j > row_from && (there >> (n / 2) & 1);
                         sc[n][i] = see ? sc[n][i] : neg_inf();
                         if (kF16) {
                             float &f = i ? vs[n].y : vs[n].x;
@@ -410,7 +446,27 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     pk[1] = pack2<kF16>(p0, p1);
                 }
             }
-            if (more) load_scales();
+            uint32_t vr[NK][4][VW];
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int r = 16 * kk + 2 * t + (i & 1) + 8 * (i >> 1);
+                    const unsigned char *p = from + Ck::kV + r * Ck::kRow;
+                    // what is not there may be anything, and 0 x anything has to be 0
+                    const bool ok = whole || ((there >> kk & 1) && j0 + r >= tl.k0 && j0 + r < tl.k1);
+                    if constexpr (VW == 2) {
+                        const uint2 x = ok ? *reinterpret_cast<const uint2 *>(p + 8 * g) : make_uint2(0, 0);
+                        vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < VW / 4; c++) {
+                            const uint4 x = ok ? *reinterpret_cast<const uint4 *>(p + 16 * g + 128 * c) : make_uint4(0, 0, 0, 0);
+                            vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
+                            vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
+                        }
+                    }
+                }
             // ---- values. A step whose keys some rows of the tile see and others do not gives
             // every row 0 x v for the keys it must not see: infinities and NaN are taken out of
             // such a step, and added to the rows that see them at the end.
@@ -467,171 +523,159 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     }
                 }
             }
-            // ---- the next step's values
-            if (more) load_step_v(blk + 1, there, whole);
+            __syncwarp();
+            if (lane == 0) bulk::mbar_arrive(&sm.empty[slot]);
         }
 
-        // ---- join the warps
+        // ---- join the warps: the upper half's sums into the lower half's, those in shared memory
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        __syncthreads();  // the shared memory of the item before is read
-        if (threadIdx.x == 0) sm.bad = 0;
-        if (t == 0) {
-            sm.m[warp][g] = m;
-            sm.l[warp][g] = l;
+        if (FMT != LAI_KV_I8 && bad) sm.bad = n_it;
+        // column 2t + i of group n: the lane that holds it took its V from the run of lanes with
+        // g = 2t + i
+        auto column_of = [&](int n, int i) {
+            const int gg = 2 * t + i;
+            return VW == 2 ? gg * 8 + n : kF16 ? gg * 16 + n : (gg + 8 * (n / 8)) * 8 + n % 8;
+        };
+        const float unit = kF16 ? pow2i(vexp) : 1.f;
+        const int half = warp % kHalf;
+        if (warp >= kHalf) {
+            if (t == 0) sm.m[half][g] = m, sm.l[half][g] = l;
+#pragma unroll
+            for (int n = 0; n < ND; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) sm.o[half][g][column_of(n, i)] = o[n][i] * unit;
         }
-        {
-            const float unit = kF16 ? pow2i(vexp) : 1.f;
+        math_sync();
+        if (warp < kHalf) {
+            const bool both = warp + kHalf < kWarps;
+            const float mo = both ? sm.m[half][g] : neg_inf(), lo = both ? sm.l[half][g] : 0.f;
+            const float mx = fmaxf(m, mo), mu = mx == neg_inf() ? 0.f : mx;
+            const float ca = ex2(m - mu), cb = ex2(mo - mu);
+            __syncwarp();
+            if (t == 0) {
+                sm.l[half][g] = fmaf(lo, cb, l * ca);
+                sm.m[half][g] = mx;
+            }
 #pragma unroll
             for (int n = 0; n < ND; n++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    // column 2t + i of group n: the lane that holds it took its V from the run
-                    // of lanes with g = 2t + i
-                    const int gg = 2 * t + i;
-                    int d;
-                    if constexpr (VW == 2) d = gg * 8 + n;
-                    else if constexpr (kF16) d = gg * 16 + n;
-                    else d = (gg + 8 * (n / 8)) * 8 + n % 8;
-                    sm.o[warp][g][d] = o[n][i] * unit;
+                    float &x = sm.o[half][g][column_of(n, i)];
+                    x = fmaf(both ? x : 0.f, cb, o[n][i] * unit * ca);
                 }
         }
-        __syncthreads();
-        if (FMT != LAI_KV_I8) {
-            if (bad) sm.bad = 1;
-            __syncthreads();
-        }
-        // a thread owns runs of 4 columns: run i starts at flattened element (i * kThreads + thread) * 4
-        constexpr int kRuns = kRows * HD / 4 / kThreads;
-        float4 acc[kRuns];
-        float sum[kRuns];
-        auto row_of = [&](int i) { return (i * kThreads + (int)threadIdx.x) * 4 / HD; };
-        auto col_of = [&](int i) { return (i * kThreads + (int)threadIdx.x) * 4 % HD; };
-        auto fma4 = [](float4 &x, const float4 &v, float f) {
-            x.x = fmaf(v.x, f, x.x);
-            x.y = fmaf(v.y, f, x.y);
-            x.z = fmaf(v.z, f, x.z);
-            x.w = fmaf(v.w, f, x.w);
+        math_sync();
+        // from here a thread owns 4 columns of a row at a time
+        float4 acc;
+        float sum, top;
+        auto clear = [&]() {
+            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            sum = 0.f;
+            top = neg_inf();
         };
-        float top[kRuns];
+        // adds the state (pm, pl, pv) of some keys; top is their common maximum by now
+        auto add = [&](float pm, float pl, const float4 &pv) {
+            const float f = ex2(pm - (top == neg_inf() ? 0.f : top));
+            sum = fmaf(pl, f, sum);
+            acc.x = fmaf(pv.x, f, acc.x);
+            acc.y = fmaf(pv.y, f, acc.y);
+            acc.z = fmaf(pv.z, f, acc.z);
+            acc.w = fmaf(pv.w, f, acc.w);
+        };
+        auto write = [&](int r, int col) {
+            if (r >= tl.rows) return;
+            const int fr = tl.row0 + r, tk = a.by_group.of(fr);
+            const int64_t to = (((int64_t)tl.q_row0 + tk) * n_heads + head * a.group + (fr - tk * a.group)) * HD + col;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            if (QF32)
+                *reinterpret_cast<float4 *>(static_cast<float *>(out) + to) =
+                    make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            else
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + to) =
+                    make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        };
+        const bool alone = it.begins && it.ends;
+        float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * part_floats(HD);
+        for (int e = threadIdx.x * 4; e < kRows * HD; e += kMath * 4) {
+            const int r = e / HD, col = e % HD;
+            clear();
 #pragma unroll
-        for (int i = 0; i < kRuns; i++) {
-            const int r = row_of(i), d = col_of(i);
-            top[i] = sm.m[0][r];
+            for (int x = 0; x < kHalf; x++) top = fmaxf(top, sm.m[x][r]);
 #pragma unroll
-            for (int x = 1; x < kWarps; x++) top[i] = fmaxf(top[i], sm.m[x][r]);
-            const float mu = top[i] == neg_inf() ? 0.f : top[i];
-            sum[i] = 0.f;
-            acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int x = 0; x < kHalf; x++) add(sm.m[x][r], sm.l[x][r], *reinterpret_cast<const float4 *>(&sm.o[x][r][col]));
+            if (FMT != LAI_KV_I8 && sm.bad == n_it && r < tl.rows) {
+                const int p = tl.pos0 + a.by_group.of(tl.row0 + r);
+                for (int j = max(blk0 * U, tl.k0); j < min(blk1 * U, tl.k1); j++) {
+                    if (!mixed(tl, a.window, j / kStep * kStep, kStep) || j > p || (a.window && j <= p - a.window)) continue;
+                    const int page = __ldg(a.kv.pages + (int64_t)tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
+                    if (page < 0 || page >= a.kv.n_pages) continue;
+                    const int64_t at = (a.kv.page_base(page, head) + (j & in_page)) * HD + col;
+                    float v[4];
 #pragma unroll
-            for (int x = 0; x < kWarps; x++) {
-                const float c = ex2(sm.m[x][r] - mu);
-                sum[i] = fmaf(sm.l[x][r], c, sum[i]);
-                fma4(acc[i], *reinterpret_cast<const float4 *>(&sm.o[x][r][d]), c);
-            }
-        }
-        if (FMT != LAI_KV_I8 && sm.bad) {
-            for (int j = max(blk0 * U, tl.k0); j < min(blk1 * U, tl.k1); j++) {
-                if (!mixed(tl, a.window, j / kStep * kStep, kStep)) continue;
-                const int page = __ldg(a.kv.pages + (int64_t)tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
-                if (page < 0 || page >= a.kv.n_pages) continue;
-                const int64_t at = (a.kv.page_base(page, head) + (j & in_page)) * HD;
-#pragma unroll
-                for (int i = 0; i < kRuns; i++) {
-                    const int r = row_of(i), p = tl.pos0 + a.by_group.of(tl.row0 + r);
-                    if (r >= tl.rows || j > p || (a.window && j <= p - a.window)) continue;
-                    float *x = &acc[i].x;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float v = element<FMT>(a.kv.v, at + col_of(i) + e);
-                        if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) x[e] += v;
+                    for (int i = 0; i < 4; i++) {
+                        v[i] = element<FMT>(a.kv.v, at + i);
+                        v[i] = (__float_as_uint(v[i]) & 0x7f800000u) == 0x7f800000u ? v[i] : 0.f;
                     }
+                    acc.x += v[0];
+                    acc.y += v[1];
+                    acc.z += v[2];
+                    acc.w += v[3];
                 }
             }
-        }
-        bool write = it.begins && it.ends;
-        if (!write) {
+            if (alone) {
+                write(r, col);
+                continue;
+            }
             // parts: [row] max, [row] sum, [row][column]
-            float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * part_floats(HD);
-#pragma unroll
-            for (int i = 0; i < kRuns; i++) {
-                if (col_of(i) == 0) {
-                    pp[row_of(i)] = top[i];
-                    pp[kRows + row_of(i)] = sum[i];
-                }
-                *reinterpret_cast<float4 *>(pp + 2 * kRows + (i * kThreads + threadIdx.x) * 4) = acc[i];
+            if (col == 0) {
+                pp[r] = top;
+                pp[kRows + r] = sum;
             }
-            __threadfence();
-            __syncthreads();
-            const int c0 = cta_of(range, it.item0), c1 = cta_of(range, it.item1 - 1);
-            if (threadIdx.x == 0) sm.last = atomicAdd(a.counters + c0, 1) == c1 - c0;
-            __syncthreads();
-            write = sm.last;
-            if (write) {
-                __threadfence();
-                if (threadIdx.x == 0) a.counters[c0] = 0;  // ready for the next call
-                // The parts' weights first, then the parts with 8 of them under way at a time.
-                // Shared memory that the warps' join used holds kWeights parts at once.
-                constexpr int kWeights = sizeof(sm.o) / sizeof(float) / kRows / 2;
-                float *wm = &sm.o[0][0][0], *wl = wm + kWeights * kRows;
-                auto part = [&](int c) { return a.parts + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * part_floats(HD); };
-#pragma unroll
-                for (int i = 0; i < kRuns; i++) {
-                    acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    sum[i] = 0.f;
-                    top[i] = neg_inf();
-                }
-                for (int first = c0; first <= c1; first += kWeights) {
-                    const int n = min(kWeights, c1 + 1 - first);
-                    __syncthreads();
-                    for (int i = threadIdx.x; i < n * kRows; i += kThreads) {
-                        const float *pc = part(first + i / kRows) + i % kRows;
-                        wm[i] = __ldcg(pc);
-                        wl[i] = __ldcg(pc + kRows);
-                    }
-                    __syncthreads();
-#pragma unroll
-                    for (int i = 0; i < kRuns; i++) {
-                        const int r = row_of(i);
-                        float t = top[i];
-                        for (int c = 0; c < n; c++) t = fmaxf(t, wm[c * kRows + r]);
-                        const float mu = t == neg_inf() ? 0.f : t;
-                        const float down = ex2(top[i] - mu);
-                        top[i] = t;
-                        sum[i] *= down;
-                        acc[i].x *= down;
-                        acc[i].y *= down;
-                        acc[i].z *= down;
-                        acc[i].w *= down;
-#pragma unroll 8
-                        for (int c = 0; c < n; c++) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(
-                                part(first + c) + 2 * kRows + (i * kThreads + threadIdx.x) * 4));
-                            const float f = ex2(wm[c * kRows + r] - mu);
-                            sum[i] = fmaf(wl[c * kRows + r], f, sum[i]);
-                            fma4(acc[i], v, f);
-                        }
-                    }
-                }
-            }
+            *reinterpret_cast<float4 *>(pp + 2 * kRows + e) = acc;
         }
-        if (write) {
+        if (alone) continue;
+        const int c0 = cta_of(range, it.item0), c1 = cta_of(range, it.item1 - 1);
+        math_sync();
+        if (threadIdx.x == 0) {
+            __threadfence();  // for the whole CTA, whose writes the barrier put before it
+            const bool last = atomicAdd(a.counters + c0, 1) == c1 - c0;
+            __threadfence();
+            if (last) a.counters[c0] = 0;  // ready for the next call
+            sm.last = last;
+        }
+        math_sync();
+        if (!sm.last) continue;
+        for (int e = threadIdx.x * 4; e < kRows * HD; e += kMath * 4) {
+            const int r = e / HD, col = e % HD;
+            clear();
+            constexpr int kAtOnce = 8;  // the parts in their order, so many of them under way
+            for (int first = c0; first <= c1; first += kAtOnce) {
+                float pm[kAtOnce], pl[kAtOnce];
+                float4 pv[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < kRuns; i++) {
-                const int r = row_of(i);
-                if (r >= tl.rows) continue;
-                const int fr = tl.row0 + r, tk = a.by_group.of(fr);
-                const int64_t at = (((int64_t)tl.q_row0 + tk) * n_heads + head * a.group +
-                                    (fr - tk * a.group)) * HD + col_of(i);
-                const float inv = sum[i] == 0.f ? 0.f : 1.f / sum[i];
-                if (QF32)
-                    *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) =
-                        make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
-                else
-                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + at) =
-                        make_uint2(pack_bf16x2(acc[i].x * inv, acc[i].y * inv),
-                                   pack_bf16x2(acc[i].z * inv, acc[i].w * inv));
+                for (int c = 0; c < kAtOnce; c++) {
+                    pm[c] = neg_inf();
+                    pl[c] = 0.f;
+                    pv[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (first + c <= c1) {
+                        const float *pc = a.parts + ((int64_t)(first + c) * 2 + (first + c == c0 ? 1 : 0)) * part_floats(HD);
+                        pm[c] = __ldcg(pc + r);
+                        pl[c] = __ldcg(pc + kRows + r);
+                        pv[c] = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * kRows + e));
+                    }
+                }
+                const float was = top, wl = sum;
+                const float4 wv = acc;
+#pragma unroll
+                for (int c = 0; c < kAtOnce; c++) top = fmaxf(top, pm[c]);
+                sum = 0.f;
+                acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                add(was, wl, wv);
+#pragma unroll
+                for (int c = 0; c < kAtOnce; c++) add(pm[c], pl[c], pv[c]);
             }
+            write(r, col);
         }
     }
 }
@@ -642,8 +686,12 @@ int launch_few(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
     const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.log_page) + U - 1) / U;
     const int64_t most = FewSched<FMT>::slots(a.kv.n_rows, a.group, a.kv.n_seqs) * a.kv.n_kv;
     const int64_t ctas = most < kMaxCtas ? most * blocks : kMaxCtas;  // most * blocks fits
+    constexpr size_t kSmem = sizeof(Smem<HD, FMT>);
+    static_assert(kSmem * kCtasPerSm <= 226 * 1024, "shared memory of an SM");
     auto kern = paged_attn_few_kernel<HD, FMT, QF32>;
-    launch_pdl(kern, dim3((unsigned)(ctas < kMaxCtas ? ctas : kMaxCtas)), dim3(kThreads), 0, st, out, q, a);
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
+        return LAI_ERR_CUDA;
+    launch_pdl(kern, dim3((unsigned)(ctas < kMaxCtas ? ctas : kMaxCtas)), dim3(kThreads), kSmem, st, out, q, a);
     return launch_status();
 }
 

@@ -436,11 +436,13 @@ class _PagedBatchC(ctypes.Structure):
                 ("max_pages", ctypes.c_int32)]
 
 
-def _need_cuda(*tensors):
-    dev = tensors[0].device
+def _need_cuda(index, *tensors):
+    """Every tensor (or None) is on CUDA device `index` (-1: a CPU tensor's)."""
     for t in tensors:
-        if t is not None and (t.device.type != "cuda" or t.device != dev):
-            raise ValueError("paged cache, batch and rows must be CUDA tensors of one device")
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        raise ValueError("paged cache, batch and rows must be CUDA tensors of one device")
 
 
 class PagedKV:
@@ -466,10 +468,11 @@ class PagedKV:
                 raise ValueError("scales must be contiguous F32 [n_pages, n_kv_heads, page_size]")
         if k.shape[2] not in (16, 32, 64, 128, 256) or k.shape[3] not in (64, 128):
             raise ValueError("page_size must be 16, 32, 64, 128 or 256 and head_dim 64 or 128")
-        _need_cuda(k, v, k_scale, v_scale)
+        self.index = k.get_device()
+        _need_cuda(self.index, v, k_scale, v_scale)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
-        self.device = k.device
+        self.device, self.width = k.device, k.shape[1] * k.shape[3]
         self._c = _PagedKVC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if fmt else None,
                             v_scale.data_ptr() if fmt else None, *(k.shape[0], k.shape[2]),
                             k.shape[1], k.shape[3], fmt)
@@ -494,57 +497,68 @@ class PagedBatch:
 
     def __init__(self, q_start, kv_len, pages):
         import torch
-        for t in (q_start, kv_len, pages):
-            if t.dtype != torch.int32 or not t.is_contiguous():
-                raise ValueError("q_start, kv_len and pages must be contiguous int32")
-        if q_start.dim() != 1 or kv_len.dim() != 1 or pages.dim() != 2 or \
-                q_start.shape[0] != kv_len.shape[0] + 1 or pages.shape[0] != kv_len.shape[0]:
+        i32 = torch.int32
+        if q_start.dtype != i32 or kv_len.dtype != i32 or pages.dtype != i32 or not (
+                q_start.is_contiguous() and kv_len.is_contiguous() and pages.is_contiguous()):
+            raise ValueError("q_start, kv_len and pages must be contiguous int32")
+        shape = pages.shape
+        if len(shape) != 2 or kv_len.shape != shape[:1] or q_start.shape != (shape[0] + 1,):
             raise ValueError("a batch is q_start [n + 1], kv_len [n], pages [n, max_pages]")
-        _need_cuda(q_start, kv_len, pages)
+        self.index = q_start.get_device()
+        _need_cuda(self.index, kv_len, pages)
         self.q_start, self.kv_len, self.pages = q_start, kv_len, pages
-        self.device = q_start.device
         self._c = _PagedBatchC(q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(),
-                               *pages.shape)
+                               shape[0], shape[1])
         self._ref = ctypes.byref(self._c)
 
 
 def _paged_rows(t, width):
     """Row stride of a [rows, width] tensor whose rows are dense (a column block will do)."""
-    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and t.shape[1] != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] != width or (stride[1] != 1 and width != 1):
         raise ValueError(f"rows must be [n, {width}] with adjacent elements")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    return stride[0] if shape[0] > 1 else max(stride[0], width)
 
 
-def _paged_call(fn, device, args, stream):
+_PAGED_FN: dict = {}
+
+
+def _paged_fn(name, dtype):
+    """The entry point `name` for rows of torch dtype."""
+    fn = _PAGED_FN.get((name, dtype))
+    if fn is None:
+        import torch
+        suffix = {torch.float32: "f32", torch.bfloat16: "bf16"}.get(dtype)
+        if suffix is None:
+            raise TypeError(f"rows must be float32 or bfloat16, not {dtype}")
+        fn = _PAGED_FN[name, dtype] = getattr(load(), f"{name}_{suffix}")
+    return fn
+
+
+def _paged_call(fn, index, stream, *args):
     """Launch on `stream`, or on the current stream of the tensors' device."""
     import torch
-    if device.index == torch.cuda.current_device():
-        return call(fn, *args, _s(stream))
-    with torch.cuda.device(device):
-        return call(fn, *args, _s(stream))
-
-
-def _paged_dtype(t):
-    import torch
-    if t == torch.float32:
-        return "f32"
-    if t == torch.bfloat16:
-        return "bf16"
-    raise TypeError(f"rows must be float32 or bfloat16, not {t}")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            st = fn(*args, torch.cuda.current_stream().cuda_stream if stream is None else stream.cuda_stream)
+    else:
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream)
+    if st != LAI_OK:
+        raise LaiError(fn.__name__, st)
 
 
 def paged_kv_append(kv, batch, k, v, err=None, stream=None):
     """Write the new tokens' rows k, v [rows, n_kv_heads * head_dim] (F32 or BF16; column blocks
     of one tensor will do) to their positions in the cache, quantising them if it is an 8-bit one."""
+    fn = _paged_fn("lai_paged_kv_append", k.dtype)
     if v.dtype != k.dtype or v.shape != k.shape:
         raise ValueError("k and v must have the same shape and dtype")
-    suffix = _paged_dtype(k.dtype)
-    ld = _paged_rows(k, kv.n_kv_heads * kv.head_dim)
-    if _paged_rows(v, kv.n_kv_heads * kv.head_dim) != ld:
+    ld = _paged_rows(k, kv.width)
+    if _paged_rows(v, kv.width) != ld:
         raise ValueError("k and v must have the same row stride")
-    _need_cuda(kv.k, batch.q_start, k, v, err)
-    _paged_call("lai_paged_kv_append_" + suffix, kv.device,
-                (kv._ref, batch._ref, k.data_ptr(), v.data_ptr(), ld, k.shape[0], _p(err)), stream)
+    _need_cuda(kv.index, batch.q_start, k, v, err)
+    _paged_call(fn, kv.index, stream, kv._ref, batch._ref, k.data_ptr(), v.data_ptr(), ld,
+                k.shape[0], None if err is None else err.data_ptr())
 
 
 def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None):
@@ -552,17 +566,17 @@ def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None)
     stands for at the positions of the batch's rows. With kv_len as the lengths of q_start's
     ranges these are whole sequences."""
     import torch
-    suffix, width = _paged_dtype(dtype), kv.n_kv_heads * kv.head_dim
-    k = torch.empty((rows, width), dtype=dtype, device=kv.device) if k is None else k
-    v = torch.empty((rows, width), dtype=dtype, device=kv.device) if v is None else v
+    fn = _paged_fn("lai_paged_kv_read", dtype)
+    k = torch.empty((rows, kv.width), dtype=dtype, device=kv.device) if k is None else k
+    v = torch.empty((rows, kv.width), dtype=dtype, device=kv.device) if v is None else v
     if k.dtype != dtype or v.dtype != dtype or k.shape[0] != rows or v.shape[0] != rows:
         raise ValueError("k and v must be [rows, n_kv_heads * head_dim] of dtype")
-    ld = _paged_rows(k, width)
-    if _paged_rows(v, width) != ld:
+    ld = _paged_rows(k, kv.width)
+    if _paged_rows(v, kv.width) != ld:
         raise ValueError("k and v must have the same row stride")
-    _need_cuda(kv.k, batch.q_start, k, v, err)
-    _paged_call("lai_paged_kv_read_" + suffix, kv.device,
-                (k.data_ptr(), v.data_ptr(), ld, rows, kv._ref, batch._ref, _p(err)), stream)
+    _need_cuda(kv.index, batch.q_start, k, v, err)
+    _paged_call(fn, kv.index, stream, k.data_ptr(), v.data_ptr(), ld, rows, kv._ref, batch._ref,
+                None if err is None else err.data_ptr())
     return k, v
 
 
@@ -570,8 +584,17 @@ def paged_attention_scratch(head_dim=128, device="cuda"):
     """Zeroed scratch for paged_attention, of one size for every batch. It serves any number of
     calls one after another; calls that may run at the same time need one each."""
     import torch
-    nb = load().lai_paged_attention_scratch_bytes(head_dim)
-    return torch.zeros(nb // 4, dtype=torch.float32, device=device)
+    return torch.zeros(_paged_scratch_floats(head_dim), dtype=torch.float32, device=device)
+
+
+_PAGED_SCRATCH: dict = {}
+
+
+def _paged_scratch_floats(head_dim):
+    n = _PAGED_SCRATCH.get(head_dim)
+    if n is None:
+        n = _PAGED_SCRATCH[head_dim] = load().lai_paged_attention_scratch_bytes(head_dim) // 4
+    return n
 
 
 def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, err=None,
@@ -581,23 +604,23 @@ def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, 
     token sees the last `window` keys up to itself (0: all). Returns out [rows, n_heads * head_dim]
     (rows that belong to no sequence are not written)."""
     import torch
-    suffix, hd = _paged_dtype(q.dtype), kv.head_dim
-    if q.dim() != 2 or q.shape[1] % (hd * kv.n_kv_heads):
+    fn, hd = _paged_fn("lai_paged_attention", q.dtype), kv.head_dim
+    shape = q.shape
+    if len(shape) != 2 or shape[1] % kv.width:
         raise ValueError("q must be [rows, n_heads * head_dim], n_heads a multiple of n_kv_heads")
-    ld = _paged_rows(q, q.shape[1])
+    ld = _paged_rows(q, shape[1])
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
+        out = torch.empty(shape, dtype=q.dtype, device=kv.device)
+    elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and dtype")
     if scratch is None:
         scratch = paged_attention_scratch(hd, kv.device)
-    elif scratch.numel() * scratch.element_size() < load().lai_paged_attention_scratch_bytes(hd):
+    elif scratch.nbytes < 4 * _paged_scratch_floats(hd):
         raise ValueError("scratch is too small: use paged_attention_scratch(head_dim)")
-    _need_cuda(kv.k, batch.q_start, q, out, scratch, err)
-    _paged_call("lai_paged_attention_" + suffix, kv.device,
-                (out.data_ptr(), q.data_ptr(), ld, q.shape[0], q.shape[1] // hd, kv._ref,
-                 batch._ref, hd ** -0.5 if scale is None else scale, window, scratch.data_ptr(),
-                 _p(err)), stream)
+    _need_cuda(kv.index, batch.q_start, q, out, scratch, err)
+    _paged_call(fn, kv.index, stream, out.data_ptr(), q.data_ptr(), ld, shape[0], shape[1] // hd,
+                kv._ref, batch._ref, hd ** -0.5 if scale is None else scale, window,
+                scratch.data_ptr(), None if err is None else err.data_ptr())
     return out
 
 

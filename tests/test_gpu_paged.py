@@ -228,3 +228,13 @@ def test_attention_wide_heads_and_pages(H, Hkv, hd, page, cache, dtype):
 @pytest.mark.parametrize("cache,dtype", [("bf16", "bf16"), ("i8", "f32"), ("e4m3", "bf16"), ("bf16", "f32")])
 def test_attention_wide_window(window, hd, cache, dtype):
     Case([200, 400], [1000, 400], 4, 2, hd, cache, 16, dtype, seed=window % 89).check(window=window)
+
+
+@pytest.mark.parametrize("cache", list(ref.FORMATS))
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+@pytest.mark.parametrize("hd,Hkv", [(128, 8), (64, 5)])
+def test_attention_many_sequences_of_one_token(cache, dtype, hd, Hkv):
+    # more work than CTAs: every CTA goes through several items, cut and whole ones
+    r = torch.Generator().manual_seed(hd)
+    keys = [int(x) for x in torch.randint(1, 3000, (48,), generator=r)]
+    Case([1] * 48, keys, 2 * Hkv, Hkv, hd, cache, 64, dtype, seed=5).check()

@@ -95,12 +95,13 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
     }
 #undef LAI_MMA
 }
-// Zero an element of a pair that is an infinity or NaN; true if there was one.
-template <bool F16> __device__ __forceinline__ bool drop_nonfinite(uint32_t &p) {
-    constexpr uint32_t kLo = F16 ? 0x7c00u : 0x7f80u, kHi = kLo << 16;
-    const bool lo = (p & kLo) == kLo, hi = (p & kHi) == kHi;
-    p &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
-    return lo || hi;
+// Zero what is an infinity or NaN among the elements of a stored word; true if there was one.
+template <int FMT> __device__ __forceinline__ bool drop_nonfinite(uint32_t &x) {
+    uint32_t gone;
+    if (FMT == LAI_KV_BF16) gone = __vcmpeq2(x & 0x7f807f80u, 0x7f807f80u);
+    else gone = __vcmpeq4(x & 0x7f7f7f7fu, 0x7f7f7f7fu);  // E4M3: NaN alone
+    x &= ~gone;
+    return gone != 0;
 }
 
 // One stored element as F32, without its scale.
@@ -262,48 +263,48 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         {
             const int64_t at = ((int64_t)tl.q_row0 + tok) * a.ld_q +
                                (int64_t)(head * a.group + (row - tok * a.group)) * HD;
-            float x[KS][4];
-            uint32_t top = 0;
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
+            // the 4 elements that the lane needs in step s
+            auto load4 = [&](int s, float (&x)[4]) {
                 const int d = (s / kPerChunk * 4 + t) * (kPerChunk * 4) + s % kPerChunk * 4;
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[s][e] = 0.f;
-                if (row_ok) {
-                    if (QF32) {
-                        const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(qp) + at + d);
-                        x[s][0] = f.x; x[s][1] = f.y; x[s][2] = f.z; x[s][3] = f.w;
-                    } else {
-                        const uint2 f = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(qp) + at + d);
-                        x[s][0] = bf16_lo(f.x); x[s][1] = bf16_hi(f.x);
-                        x[s][2] = bf16_lo(f.y); x[s][3] = bf16_hi(f.y);
-                    }
+                x[0] = x[1] = x[2] = x[3] = 0.f;
+                if (!row_ok) return;
+                if (QF32) {
+                    const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(qp) + at + d);
+                    x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+                } else {
+                    const uint2 f = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(qp) + at + d);
+                    x[0] = bf16_lo(f.x); x[1] = bf16_hi(f.x); x[2] = bf16_lo(f.y); x[3] = bf16_hi(f.y);
                 }
-#pragma unroll
-                for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[s][e]) & 0x7fffffffu);
-            }
+            };
+            float up = 1.f;
             if (kF16) {  // the row's largest into [2^13, 2^14)
+                uint32_t top = 0;
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    float x[4];
+                    load4(s, x);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                }
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const int e = (int)(top >> 23) - 127;
-                const float up = pow2i(13 - e);
+                up = pow2i(13 - e);
                 row_scale *= pow2i(e - 13);
-#pragma unroll
-                for (int s = 0; s < KS; s++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[s][i] *= up;
             }
+#pragma unroll 1
+            for (int s = warp; s < KS; s += kWarps) {  // the warp's share
+                float x[4];
+                load4(s, x);
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                if (s % kWarps != warp) continue;  // every warp has all of it; each writes its share
+                for (int e = 0; e < 4; e++) x[e] *= up;
                 uint4 v;
-                v.x = take2<kF16>(x[s][0], x[s][1]);
-                v.z = take2<kF16>(x[s][2], x[s][3]);
-                v.y = QF32 ? take2<kF16>(x[s][0], x[s][1]) : 0u;
-                v.w = QF32 ? take2<kF16>(x[s][2], x[s][3]) : 0u;
+                v.x = take2<kF16>(x[0], x[1]);
+                v.z = take2<kF16>(x[2], x[3]);
+                v.y = QF32 ? take2<kF16>(x[0], x[1]) : 0u;
+                v.w = QF32 ? take2<kF16>(x[2], x[3]) : 0u;
                 sm.q[s][lane] = v;
-                if constexpr (kThird)
-                    sm.q3[s][lane] = make_uint2(pack2<false>(x[s][0], x[s][1]), pack2<false>(x[s][2], x[s][3]));
+                if constexpr (kThird) sm.q3[s][lane] = make_uint2(pack2<false>(x[0], x[1]), pack2<false>(x[2], x[3]));
             }
             math_sync();
         }
@@ -446,38 +447,48 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     pk[1] = pack2<kF16>(p0, p1);
                 }
             }
+            // ---- values
             uint32_t vr[NK][4][VW];
 #pragma unroll
             for (int kk = 0; kk < NK; kk++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int r = 16 * kk + 2 * t + (i & 1) + 8 * (i >> 1);
-                    const unsigned char *p = from + Ck::kV + r * Ck::kRow;
-                    // what is not there may be anything, and 0 x anything has to be 0
-                    const bool ok = whole || ((there >> kk & 1) && j0 + r >= tl.k0 && j0 + r < tl.k1);
+                    const unsigned char *p = from + Ck::kV + (16 * kk + 2 * t + (i & 1) + 8 * (i >> 1)) * Ck::kRow;
                     if constexpr (VW == 2) {
-                        const uint2 x = ok ? *reinterpret_cast<const uint2 *>(p + 8 * g) : make_uint2(0, 0);
+                        const uint2 x = *reinterpret_cast<const uint2 *>(p + 8 * g);
                         vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
                     } else {
 #pragma unroll
                         for (int c = 0; c < VW / 4; c++) {
-                            const uint4 x = ok ? *reinterpret_cast<const uint4 *>(p + 16 * g + 128 * c) : make_uint4(0, 0, 0, 0);
+                            const uint4 x = *reinterpret_cast<const uint4 *>(p + 16 * g + 128 * c);
                             vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
                             vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
                         }
                     }
                 }
-            // ---- values. A step whose keys some rows of the tile see and others do not gives
-            // every row 0 x v for the keys it must not see: infinities and NaN are taken out of
-            // such a step, and added to the rows that see them at the end.
+            // What is not there may be anything, and weight 0 times it has to be 0. And a step whose
+            // keys some rows of the tile see and others do not gives every row 0 x v for the keys it
+            // must not see: infinities and NaN are taken out of such a step, and added to the rows
+            // that see them at the end.
+            if (!all) {
+#pragma unroll
+                for (int kk = 0; kk < NK; kk++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int j = j0 + 16 * kk + 2 * t + (i & 1) + 8 * (i >> 1);
+                        const bool ok = (there >> kk & 1) && j >= tl.k0 && j < tl.k1;
+#pragma unroll
+                        for (int w = 0; w < VW; w++) {
+                            uint32_t &x = vr[kk][i][w];
+                            x = ok ? x : 0u;
+                            if (FMT != LAI_KV_I8) bad |= drop_nonfinite<FMT>(x);
+                        }
+                    }
+            }
             auto column = [&](int n, uint32_t (&b0)[NK], uint32_t (&b1)[NK]) {
                 float c[4];
 #pragma unroll
                 for (int kk = 0; kk < NK; kk++) {
-                    if (FMT != LAI_KV_I8 && uneven) {
-                        bad |= drop_nonfinite<kF16>(b0[kk]);
-                        bad |= drop_nonfinite<kF16>(b1[kk]);
-                    }
                     const uint32_t *pk = pa[kk];
                     if constexpr (kThird) {
                         if (kk == 0) mma<kF16, true>(c, pk[4], 0u, pk[5], 0u, b0[kk], b1[kk]);
@@ -531,10 +542,10 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (FMT != LAI_KV_I8 && bad) sm.bad = n_it;
-        // column 2t + i of group n: the lane that holds it took its V from the run of lanes with
-        // g = 2t + i
-        auto column_of = [&](int n, int i) {
-            const int gg = 2 * t + i;
+        // Column 2t + i of group n: the lane that holds it took its V from the run of lanes with
+        // g = 2t + i. Groups 4 k .. 4 k + 3 are neighbours in the output.
+        auto run_of = [&](int k, int i) {
+            const int gg = 2 * t + i, n = 4 * k;
             return VW == 2 ? gg * 8 + n : kF16 ? gg * 16 + n : (gg + 8 * (n / 8)) * 8 + n % 8;
         };
         const float unit = kF16 ? pow2i(vexp) : 1.f;
@@ -542,27 +553,31 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         if (warp >= kHalf) {
             if (t == 0) sm.m[half][g] = m, sm.l[half][g] = l;
 #pragma unroll
-            for (int n = 0; n < ND; n++)
+            for (int k = 0; k < ND / 4; k++)
 #pragma unroll
-                for (int i = 0; i < 2; i++) sm.o[half][g][column_of(n, i)] = o[n][i] * unit;
+                for (int i = 0; i < 2; i++)
+                    *reinterpret_cast<float4 *>(&sm.o[half][g][run_of(k, i)]) =
+                        make_float4(o[4 * k][i] * unit, o[4 * k + 1][i] * unit, o[4 * k + 2][i] * unit, o[4 * k + 3][i] * unit);
         }
         math_sync();
         if (warp < kHalf) {
             const bool both = warp + kHalf < kWarps;
             const float mo = both ? sm.m[half][g] : neg_inf(), lo = both ? sm.l[half][g] : 0.f;
             const float mx = fmaxf(m, mo), mu = mx == neg_inf() ? 0.f : mx;
-            const float ca = ex2(m - mu), cb = ex2(mo - mu);
+            const float ca = ex2(m - mu), cb = ex2(mo - mu), cu = ca * unit;
             __syncwarp();
             if (t == 0) {
                 sm.l[half][g] = fmaf(lo, cb, l * ca);
                 sm.m[half][g] = mx;
             }
 #pragma unroll
-            for (int n = 0; n < ND; n++)
+            for (int k = 0; k < ND / 4; k++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    float &x = sm.o[half][g][column_of(n, i)];
-                    x = fmaf(both ? x : 0.f, cb, o[n][i] * unit * ca);
+                    float4 *p = reinterpret_cast<float4 *>(&sm.o[half][g][run_of(k, i)]);
+                    const float4 x = both ? *p : make_float4(0.f, 0.f, 0.f, 0.f);
+                    *p = make_float4(fmaf(x.x, cb, o[4 * k][i] * cu), fmaf(x.y, cb, o[4 * k + 1][i] * cu),
+                                     fmaf(x.z, cb, o[4 * k + 2][i] * cu), fmaf(x.w, cb, o[4 * k + 3][i] * cu));
                 }
         }
         math_sync();
@@ -635,7 +650,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             *reinterpret_cast<float4 *>(pp + 2 * kRows + e) = acc;
         }
         if (alone) continue;
-        const int c0 = cta_of(range, it.item0), c1 = cta_of(range, it.item1 - 1);
+        const int c0 = range.cta_of(it.item0), c1 = range.cta_of(it.item1 - 1);
         math_sync();
         if (threadIdx.x == 0) {
             __threadfence();  // for the whole CTA, whose writes the barrier put before it
@@ -649,8 +664,10 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         for (int e = threadIdx.x * 4; e < kRows * HD; e += kMath * 4) {
             const int r = e / HD, col = e % HD;
             clear();
-            constexpr int kAtOnce = 8;  // the parts in their order, so many of them under way
-            for (int first = c0; first <= c1; first += kAtOnce) {
+            constexpr int kAtOnce = 4;  // the parts in their order, so many of them under way
+            const float *from = a.parts + (int64_t)c0 * 2 * part_floats(HD);
+#pragma unroll 1
+            for (int first = c0; first <= c1; first += kAtOnce, from += kAtOnce * 2 * part_floats(HD)) {
                 float pm[kAtOnce], pl[kAtOnce];
                 float4 pv[kAtOnce];
 #pragma unroll
@@ -658,8 +675,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     pm[c] = neg_inf();
                     pl[c] = 0.f;
                     pv[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (first + c <= c1) {
-                        const float *pc = a.parts + ((int64_t)(first + c) * 2 + (first + c == c0 ? 1 : 0)) * part_floats(HD);
+                    if (first + c <= c1) {  // (the first part is its CTA's second)
+                        const float *pc = from + c * 2 * part_floats(HD) + (first + c == c0 ? part_floats(HD) : 0);
                         pm[c] = __ldcg(pc + r);
                         pl[c] = __ldcg(pc + kRows + r);
                         pv[c] = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * kRows + e));
@@ -682,16 +699,14 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
 
 template <int HD, int FMT, bool QF32>
 int launch_few(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
-    constexpr int U = block_keys<FMT>();
-    const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.log_page) + U - 1) / U;
-    const int64_t most = FewSched<FMT>::slots(a.kv.n_rows, a.group, a.kv.n_seqs) * a.kv.n_kv;
-    const int64_t ctas = most < kMaxCtas ? most * blocks : kMaxCtas;  // most * blocks fits
+    const int64_t most = FewSched<FMT>::most_blocks(a.kv, a.group);
+    if (most > INT32_MAX) return LAI_ERR_RANGE;
     constexpr size_t kSmem = sizeof(Smem<HD, FMT>);
     static_assert(kSmem * kCtasPerSm <= 226 * 1024, "shared memory of an SM");
     auto kern = paged_attn_few_kernel<HD, FMT, QF32>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
         return LAI_ERR_CUDA;
-    launch_pdl(kern, dim3((unsigned)(ctas < kMaxCtas ? ctas : kMaxCtas)), dim3(kThreads), kSmem, st, out, q, a);
+    launch_pdl(kern, dim3((unsigned)(most < kMaxCtas ? most : kMaxCtas)), dim3(kThreads), kSmem, st, out, q, a);
     return launch_status();
 }
 

@@ -73,11 +73,16 @@ struct Sched {
     static constexpr int kRowsPerTile = R, kBlock = U, kExtra = E;
     // Slots of tiles: sequence s has those from q_start[s] * group / R + s on, at least as many as
     // it has tiles.
-    static __host__ __device__ int64_t slots(int64_t n_rows, int group, int n_seqs) {
-        return n_rows * group / R + n_seqs;
+    static __host__ __device__ int slots(int64_t n_rows, int group, int n_seqs) {
+        return (int)(n_rows * group / R) + n_seqs;
+    }
+    // No batch of this shape has more blocks (they are counted in 32 bits).
+    static int64_t most_blocks(const View &v, int group) {
+        const int64_t keys = ((int64_t)v.max_pages << v.log_page) + U;
+        return slots(v.n_rows, group, v.n_seqs) * (keys / U + 1 + E) * v.n_kv;
     }
     static __device__ __forceinline__ int base(const AttnArgs &a, int s) {
-        return (int)((int64_t)a.kv.q_start[s] * a.group / R) + s;
+        return a.kv.q_start[s] * a.group / R + s;
     }
     static __device__ __forceinline__ int cost(const Tile &t) { return t.rows ? t.blocks + E : 0; }
     // The last sequence whose slots start at or before `slot` (0 if none does).
@@ -93,12 +98,12 @@ struct Sched {
         Tile t = {};
         const Seq q = load_seq(a.kv, s);
         const int i = slot - base(a, s);
-        const int64_t r0 = (int64_t)i * R, all = (int64_t)q.n * a.group;
+        const int r0 = i * R, all = q.n * a.group;  // below 2^28 where ok
         if (!q.ok || i < 0 || r0 >= all) return t;
         t.seq = s;
-        t.row0 = (int)r0;
+        t.row0 = r0;
         t.q_row0 = q.row0;
-        t.rows = (int)min((int64_t)R, all - r0);
+        t.rows = min(R, all - r0);
         t.pos0 = q.len - q.n;
         const int first = t.pos0 + a.by_group.of(t.row0);
         const int last = t.pos0 + a.by_group.of(t.row0 + t.rows - 1);
@@ -138,73 +143,79 @@ __device__ __forceinline__ AttnArgs cache_seqs(const AttnArgs &a, SeqSmem &sm) {
 
 // Where a CTA starts, and how far it goes. Positions are in blocks of the whole work.
 struct Range {
-    int64_t total, w0, w1;  // all blocks; this CTA's
-    int64_t at;             // position of slot's first block
-    int slot, seq;
-    int ctas;               // CTAs that have work
-    int n_slots;
+    int total, ctas;  // all blocks; CTAs that have work
+    int w0, w1;       // this CTA's
+    int at;           // position of slot's first block
+    int slot, seq, n_slots;
+    // floor(total c / ctas)
+    __device__ __forceinline__ int begin(int c) const {
+        const int q = total / ctas, r = total - q * ctas;
+        return q * c + r * c / ctas;  // r c < ctas^2
+    }
+    // the CTA that takes position x
+    __device__ __forceinline__ int cta_of(int x) const {
+        int c = (int)((float)x * ((float)ctas / (float)total));  // within 1: ctas is far below 2^22
+        c = min(max(c, 0), ctas - 1);
+        if (begin(c) > x) c--;
+        else if (c + 1 < ctas && begin(c + 1) <= x) c++;
+        return c;
+    }
 };
 
 struct SchedSmem {
-    int64_t sums[32];
-    int64_t at;
-    int slot, seq;
+    int sums[32];
+    int at, slot, seq;
 };
 
 template <typename S, int THREADS>
 __device__ __forceinline__ Range find_range(const AttnArgs &a, SchedSmem &sm) {
-    const int n_slots = (int)S::slots(a.kv.n_rows, a.group, a.kv.n_seqs);
+    const int n_slots = S::slots(a.kv.n_rows, a.group, a.kv.n_seqs);
     const int per = (n_slots + THREADS - 1) / THREADS;
     const int s0 = min((int)threadIdx.x * per, n_slots), s1 = min(s0 + per, n_slots);
-    int64_t mine = 0;
-    int first_seq = 0;
+    int mine = 0, first_seq = 0;
     if (s0 < s1) {
         int s = first_seq = S::seq_of(a, s0);
+#pragma unroll 1
         for (int slot = s0; slot < s1; slot++) {
             while (s + 1 < a.kv.n_seqs && S::base(a, s + 1) <= slot) s++;
             mine += S::cost(S::tile(a, slot, s));
         }
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += x;
     }
     if (lane == 31) sm.sums[warp] = upto;
-    if (threadIdx.x == 0) sm.slot = n_slots;
     __syncthreads();
-    int64_t total = 0, before = upto - mine;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; w++) {
-        if (w < warp) before += sm.sums[w];
-        total += sm.sums[w];
-    }
+    // every warp adds up the warps' sums
+    int before = lane < THREADS / 32 ? sm.sums[lane] : 0;
+    const int total = __reduce_add_sync(0xffffffffu, before);
+    before = __reduce_add_sync(0xffffffffu, lane < warp ? before : 0) + upto - mine;
     Range r;
     r.total = total * a.kv.n_kv;
-    r.ctas = (int)min((int64_t)gridDim.x, r.total);
-    r.w0 = r.w1 = r.at = 0;
-    r.slot = r.seq = 0;
+    r.ctas = min((int)gridDim.x, r.total);
+    r.w0 = r.w1 = r.at = r.slot = r.seq = 0;
     r.n_slots = n_slots;
     if ((int)blockIdx.x >= r.ctas) return r;  // the whole CTA
-    r.w0 = r.total * blockIdx.x / r.ctas;
-    r.w1 = r.total * (blockIdx.x + 1) / r.ctas;
-    const int64_t nk = a.kv.n_kv;
+    r.w0 = r.begin(blockIdx.x);
+    r.w1 = r.begin(blockIdx.x + 1);
+    const int nk = a.kv.n_kv;
     if (before * nk <= r.w0 && r.w0 < (before + mine) * nk) {  // one thread's slots hold w0
-        int s = first_seq;
-        int64_t at = before;
-        for (int slot = s0; slot < s1; slot++) {
+        int s = first_seq, at = before, slot = s0;
+#pragma unroll 1
+        for (; slot + 1 < s1; slot++) {
             while (s + 1 < a.kv.n_seqs && S::base(a, s + 1) <= slot) s++;
             const int c = S::cost(S::tile(a, slot, s));
-            if (r.w0 < (at + c) * nk) {
-                sm.slot = slot;
-                sm.seq = s;
-                sm.at = at * nk;
-                break;
-            }
+            if (r.w0 < (at + c) * nk) break;
             at += c;
         }
+        while (s + 1 < a.kv.n_seqs && S::base(a, s + 1) <= slot) s++;
+        sm.slot = slot;
+        sm.seq = s;
+        sm.at = at * nk;
     }
     __syncthreads();
     r.slot = sm.slot;
@@ -213,16 +224,11 @@ __device__ __forceinline__ Range find_range(const AttnArgs &a, SchedSmem &sm) {
     return r;
 }
 
-// The CTA that takes position x.
-__device__ __forceinline__ int cta_of(const Range &r, int64_t x) {
-    return (int)(((x + 1) * r.ctas - 1) / r.total);
-}
-
 // The items of a CTA in order. Roles of a CTA that walk by themselves see the same ones.
 template <typename S>
 struct Walk {
-    int64_t at, w0, w1;      // position of the current item; the CTA's range
-    int64_t item0, item1;    // positions of the item's blocks
+    int at, w0, w1;          // position of the current item; the CTA's range
+    int item0, item1;        // positions of the item's blocks
     Tile tl;
     int slot, seq, cost, n_slots;
     int head, blk0, blk1;    // the item's kv head; this CTA's blocks of it
@@ -236,8 +242,8 @@ struct Walk {
         seq = r.seq;
         tl = S::tile(a, slot, seq);
         cost = S::cost(tl);
-        head = (int)((w0 - r.at) / cost);
-        at = r.at + (int64_t)head * cost;
+        head = (w0 - r.at) / cost;
+        at = r.at + head * cost;
     }
     // Sets the item at `at` and steps past it.
     __device__ __forceinline__ bool next(const AttnArgs &a) {
@@ -256,10 +262,10 @@ struct Walk {
             item1 = at + cost;
             at = item1;
             head++;
-            const int64_t lo = max(w0, item0), hi = min(item1, w1);
+            const int lo = max(w0, item0), hi = min(item1, w1);
             if (lo >= hi) continue;  // only of the item's extra cost
-            blk0 = tl.b0 + (int)(lo - item0);
-            blk1 = tl.b0 + (int)(hi - item0);
+            blk0 = tl.b0 + lo - item0;
+            blk1 = tl.b0 + hi - item0;
             begins = lo == item0;
             ends = hi == item1;
             return true;

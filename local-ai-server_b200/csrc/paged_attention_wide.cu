@@ -340,8 +340,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 to = Item{tl.seq, head, tl.row0, more ? tl.rows : 0, tl.q_row0, tl.pos0, tl.first, tl.last,
                           tl.k0, tl.k1, w.blk0, w.blk1, 0, 0, w.begins, w.begins && w.ends};
                 if (more && !to.whole) {
-                    to.c0 = cta_of(range, w.item0);
-                    to.c1 = cta_of(range, w.item1 - 1);
+                    to.c0 = range.cta_of(w.item0);
+                    to.c1 = range.cta_of(w.item1 - 1);
                 }
                 bulk::mbar_arrive(&ctl.item_full[slot]);
             }
@@ -1059,6 +1059,7 @@ int launch_wide(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
     if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || fa.numRegs != 128) return LAI_ERR_CUDA;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
         return LAI_ERR_CUDA;
+    if (C::S::most_blocks(a.kv, a.group) > INT32_MAX) return LAI_ERR_RANGE;
     CUtensorMap maps[2] = {};
     if (FMT == LAI_KV_BF16) {
         const int64_t rows = (a.kv.n_pages * a.kv.n_kv) << a.kv.log_page;

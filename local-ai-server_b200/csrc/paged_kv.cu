@@ -8,11 +8,17 @@
 //
 // HBM bound: every row is read once and every cache row written once (and the other way round).
 // A group of head_dim / 8 lanes owns one (row, head) of k and of v, 8 elements per lane, so the
-// maximum is a shuffle within the group, each global access is a whole 128- to 512-byte run, and
-// both tensors' loads are in flight together. A CTA's threads cover consecutive (row, head)
-// pairs; the sequence of its first row is found by counting the q_start that are not above it
-// (one load per thread and a barrier, not a chain of dependent loads), and a thread walks on
-// from there.
+// maximum is a shuffle within the group, and each global access is a whole 128- to 512-byte run.
+// What costs time beside the bytes:
+//   * The look-up of a row's place is a chain of loads (q_start, lengths, page). A CTA covers
+//     consecutive (row, head) pairs, several per thread; a thread per row follows the chain and
+//     leaves the place in shared memory, while an append's first rows are on their way. The
+//     sequence of the CTA's first row is found by counting the q_start that are not above it (one
+//     load per thread and a barrier).
+//   * The divisions: 8 per lane and tensor. The scale's reciprocal is rounded correctly once, and
+//     each quotient corrected twice by its remainder, q + (x - q s) (1 / s) in fused operations;
+//     with a correctly rounded reciprocal and a quotient within a last place that is the correctly
+//     rounded quotient (Markstein 1990). Where remainders could underflow the division itself runs.
 #include "paged.cuh"
 
 namespace lai {
@@ -24,14 +30,19 @@ using paged::View;
 
 constexpr int kThreads = 256;
 
-template <typename T> __device__ __forceinline__ void load8(const T *p, float (&x)[8]);
-template <> __device__ __forceinline__ void load8<uint16_t>(const uint16_t *p, float (&x)[8]) {
-    unpack<uint16_t>(ld_stream(p), x);
+// 8 elements of a row as they are in memory.
+template <typename T> struct Raw { uint4 w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ Raw<T> load8(const T *p) {
+    Raw<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = ld_stream(p + i * (16 / (int)sizeof(T)));
+    return r;
 }
-template <> __device__ __forceinline__ void load8<float>(const float *p, float (&x)[8]) {
+__device__ __forceinline__ void floats_of(const Raw<uint16_t> &r, float (&x)[8]) { unpack<uint16_t>(r.w[0], x); }
+__device__ __forceinline__ void floats_of(const Raw<float> &r, float (&x)[8]) {
     float a[4], b[4];
-    unpack<float>(ld_stream(p), a);
-    unpack<float>(ld_stream(p + 4), b);
+    unpack<float>(r.w[0], a);
+    unpack<float>(r.w[1], b);
 #pragma unroll
     for (int e = 0; e < 4; e++) x[e] = a[e], x[4 + e] = b[e];
 }
@@ -50,30 +61,33 @@ __device__ __forceinline__ uint32_t f32x2_to_e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ uint32_t f32_to_i8(float x) {
-    return (uint32_t)__float2int_rn(fminf(fmaxf(x, -127.f), 127.f)) & 0xffu;
+// Four integers nearest to x (ties to even), |x| <= 127, as bytes: adding 1.5 * 2^23 leaves them in
+// the low bits.
+__device__ __forceinline__ uint32_t f32x4_to_i8x4(const float *x) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) b[e] = __float_as_uint(fminf(fmaxf(x[e], -127.f), 127.f) + 12582912.f);
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
-// Where this thread's (row, head) lies in the cache. false: nothing to do for it (whole lane
-// groups agree).
-__device__ __forceinline__ bool locate(const View &a, int64_t row, int s, int head, int *err,
-                                       bool first_lane, int64_t &at) {
+// The place of a row in the cache, as the position of head 0 (a head is 1 << log_page positions),
+// looking from sequence s on; -1: nowhere.
+__device__ __forceinline__ int64_t place_of(const View &a, int64_t row, int s, int *err) {
     while (s < a.n_seqs && __ldg(a.q_start + s + 1) <= row) s++;
-    if (s >= a.n_seqs) return false;
+    if (s >= a.n_seqs || row >= a.n_rows) return -1;
     const Seq q = paged::load_seq(a, s);
-    if (row < q.row0) return false;
-    const int64_t p = (int64_t)q.len - q.n + (row - q.row0);
+    if (row < q.row0) return -1;
+    const int p = q.len - q.n + (int)(row - q.row0);
     if (!q.ok || p < 0) {
-        if (first_lane) paged::flag(err, LAI_DEVERR_POSITION);
-        return false;
+        paged::flag(err, LAI_DEVERR_POSITION);
+        return -1;
     }
     const int page = __ldg(a.pages + (int64_t)s * a.max_pages + (p >> a.log_page));
     if (page < 0 || page >= a.n_pages) {
-        if (first_lane) paged::flag(err, LAI_DEVERR_PAGE);
-        return false;
+        paged::flag(err, LAI_DEVERR_PAGE);
+        return -1;
     }
-    at = a.page_base(page, head) + (p & (a.page_size() - 1));
-    return true;
+    return a.page_base(page, 0) + (p & (a.page_size() - 1));
 }
 
 // The sequence that a CTA starts its search at: the number of q_start[1..] not above its row.
@@ -107,16 +121,23 @@ __device__ __forceinline__ void put(unsigned char *cache, float *scale, int64_t 
     s = s > 0.f ? s : 1.f;
     uint32_t w[2] = {0, 0};
     if (finite) {
+        if (s > 1e-30f && s < 1e30f) {
+            const float y = __frcp_rn(s);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = __fdiv_rn(x[e], s);
+            for (int e = 0; e < 8; e++) {
+                float q = x[e] * y;
+                q = fmaf(fmaf(-q, s, x[e]), y, q);
+                x[e] = fmaf(fmaf(-q, s, x[e]), y, q);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = __fdiv_rn(x[e], s);
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const float *y = x + 4 * h;
-            if (FMT == LAI_KV_E4M3)
-                w[h] = f32x2_to_e4m3x2(y[0], y[1]) | f32x2_to_e4m3x2(y[2], y[3]) << 16;
-            else
-                w[h] = f32_to_i8(y[0]) | f32_to_i8(y[1]) << 8 | f32_to_i8(y[2]) << 16 |
-                       f32_to_i8(y[3]) << 24;
+            const float *q = x + 4 * h;
+            if (FMT == LAI_KV_E4M3) w[h] = f32x2_to_e4m3x2(q[0], q[1]) | f32x2_to_e4m3x2(q[2], q[3]) << 16;
+            else w[h] = f32x4_to_i8x4(q);
         }
     }
     if (!ok) return;
@@ -124,71 +145,141 @@ __device__ __forceinline__ void put(unsigned char *cache, float *scale, int64_t 
     if (e0 == 0) scale[at] = finite ? s : __int_as_float(0x7fffffff);
 }
 
+// 8 stored elements and their scale, and what they stand for.
+template <int FMT> struct Stored {
+    uint4 w;
+    float s;
+};
 template <int HD, int FMT>
-__device__ __forceinline__ void get(const unsigned char *cache, const float *scale, int64_t at,
-                                    int e0, float (&x)[8]) {
+__device__ __forceinline__ Stored<FMT> fetch(const unsigned char *cache, const float *scale, int64_t at, int e0) {
+    Stored<FMT> r = {};
     if (FMT == LAI_KV_BF16) {
-        unpack<uint16_t>(ld_stream(reinterpret_cast<const uint16_t *>(cache) + at * HD + e0), x);
+        r.w = ld_stream(cache + (at * HD + e0) * 2);
+        return r;
+    }
+    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(cache + at * HD + e0));
+    r.w.x = w.x;
+    r.w.y = w.y;
+    r.s = __ldg(scale + at);
+    return r;
+}
+template <int FMT>
+__device__ __forceinline__ void values_of(const Stored<FMT> &r, float (&x)[8]) {
+    if (FMT == LAI_KV_BF16) {
+        unpack<uint16_t>(r.w, x);
         return;
     }
     constexpr int kF = FMT == LAI_KV_BF16 ? LAI_KV_I8 : FMT;  // not reached for BF16
-    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(cache + at * HD + e0));
-    const float s = __ldg(scale + at);
-    const uint32_t h[4] = {paged::half2_of<kF, false>(w.x),
-                           paged::half2_of<kF, true>(w.x),
-                           paged::half2_of<kF, false>(w.y),
-                           paged::half2_of<kF, true>(w.y)};
+    const uint32_t h[4] = {paged::half2_of<kF, false>(r.w.x), paged::half2_of<kF, true>(r.w.x),
+                           paged::half2_of<kF, false>(r.w.y), paged::half2_of<kF, true>(r.w.y)};
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         float lo, hi;
         asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
             : "=f"(lo), "=f"(hi)
             : "r"(h[e]));
-        x[2 * e] = lo * s;
-        x[2 * e + 1] = hi * s;
+        x[2 * e] = lo * r.s;
+        x[2 * e + 1] = hi * r.s;
     }
 }
+
+constexpr int kUnits = 4;  // (row, head) pairs per thread, kTogether of them under way at a time
+constexpr int kTogether = 2;
+
+// The pairs of a CTA: lane group i has pairs i, i + kGroups, ...
+template <int HD>
+struct Pairs {
+    static constexpr int kLanes = HD / 8, kGroups = kThreads / kLanes, kPerCta = kGroups * kUnits;
+    int64_t row0;
+    int rest, n_kv;
+    __device__ __forceinline__ explicit Pairs(const View &a) : n_kv(a.n_kv) {
+        const int64_t pair0 = (int64_t)blockIdx.x * kPerCta;
+        row0 = pair0 / n_kv;
+        rest = (int)(pair0 - row0 * n_kv);
+    }
+    __device__ __forceinline__ int rows() const { return (rest + kPerCta - 1) / n_kv + 1; }  // touched
+    // pair u of the thread: row (from row0 on) and head
+    __device__ __forceinline__ int row(int u, int &head) const {
+        const uint32_t i = (uint32_t)(rest + u * kGroups + (int)threadIdx.x / kLanes), r = i / (uint32_t)n_kv;
+        head = (int)(i - r * n_kv);
+        return (int)r;
+    }
+    // looks up the places of all rows; the whole CTA
+    __device__ __forceinline__ void find(const View &a, int64_t *place, int *err) const {
+        const int s = first_seq(a, row0);
+        for (int i = threadIdx.x; i < rows(); i += kThreads) place[i] = place_of(a, row0 + i, s, err);
+        __syncthreads();
+    }
+};
 
 template <typename T, int HD, int FMT>
 __global__ void __launch_bounds__(kThreads)
 append_kernel(const View a, const T *__restrict__ k, const T *__restrict__ v, int64_t ld, int *err) {
-    constexpr int kLanes = HD / 8, kPairs = kThreads / kLanes;
+    __shared__ int64_t place[Pairs<HD>::kPerCta + 1];
     pdl_wait_prior();
     pdl_launch_dependents();
-    const int64_t pair0 = (int64_t)blockIdx.x * kPairs;
-    const int64_t pair = pair0 + threadIdx.x / kLanes;
-    const int64_t row = pair / a.n_kv;
-    const int head = (int)(pair - row * a.n_kv), e0 = (threadIdx.x % kLanes) * 8;
-    float kx[8] = {}, vx[8] = {};
-    if (row < a.n_rows) {  // both loads are under way while the sequence is looked up
-        load8(k + row * ld + (int64_t)head * HD + e0, kx);
-        load8(v + row * ld + (int64_t)head * HD + e0, vx);
+    const Pairs<HD> pairs(a);
+    const int e0 = (threadIdx.x % Pairs<HD>::kLanes) * 8;
+#pragma unroll 1
+    for (int u0 = 0; u0 < kUnits; u0 += kTogether) {
+        Raw<T> kx[kTogether], vx[kTogether];
+        int row[kTogether], head[kTogether];
+#pragma unroll
+        for (int u = 0; u < kTogether; u++) {
+            row[u] = pairs.row(u0 + u, head[u]);
+            kx[u] = vx[u] = Raw<T>{};
+            if (pairs.row0 + row[u] < a.n_rows) {
+                const int64_t at = (pairs.row0 + row[u]) * ld + head[u] * HD + e0;
+                kx[u] = load8(k + at);
+                vx[u] = load8(v + at);
+            }
+        }
+        if (u0 == 0) pairs.find(a, place, err);
+#pragma unroll
+        for (int u = 0; u < kTogether; u++) {
+            const int64_t p = place[row[u]], at = p + ((int64_t)head[u] << a.log_page);
+            float x[8];
+            floats_of(kx[u], x);
+            put<HD, FMT>(a.k, a.k_scale, at, e0, x, p >= 0);
+            floats_of(vx[u], x);
+            put<HD, FMT>(a.v, a.v_scale, at, e0, x, p >= 0);
+        }
     }
-    const int s0 = first_seq(a, pair0 / a.n_kv);
-    int64_t at = 0;
-    const bool ok = row < a.n_rows && locate(a, row, s0, head, err, e0 == 0, at);
-    put<HD, FMT>(a.k, a.k_scale, at, e0, kx, ok);
-    put<HD, FMT>(a.v, a.v_scale, at, e0, vx, ok);
 }
 
 template <typename T, int HD, int FMT>
 __global__ void __launch_bounds__(kThreads)
 read_kernel(const View a, T *__restrict__ k, T *__restrict__ v, int64_t ld, int *err) {
-    constexpr int kLanes = HD / 8, kPairs = kThreads / kLanes;
+    __shared__ int64_t place[Pairs<HD>::kPerCta + 1];
     pdl_wait_prior();
     pdl_launch_dependents();
-    const int64_t pair0 = (int64_t)blockIdx.x * kPairs;
-    const int64_t pair = pair0 + threadIdx.x / kLanes;
-    const int64_t row = pair / a.n_kv;
-    const int head = (int)(pair - row * a.n_kv), e0 = (threadIdx.x % kLanes) * 8;
-    const int s0 = first_seq(a, pair0 / a.n_kv);
-    int64_t at;
-    if (row >= a.n_rows || !locate(a, row, s0, head, err, e0 == 0, at)) return;
-    float kx[8], vx[8];
-    get<HD, FMT>(a.k, a.k_scale, at, e0, kx);
-    get<HD, FMT>(a.v, a.v_scale, at, e0, vx);
-    store8(k + row * ld + (int64_t)head * HD + e0, kx);
-    store8(v + row * ld + (int64_t)head * HD + e0, vx);
+    const Pairs<HD> pairs(a);
+    const int e0 = (threadIdx.x % Pairs<HD>::kLanes) * 8;
+    pairs.find(a, place, err);
+#pragma unroll 1
+    for (int u0 = 0; u0 < kUnits; u0 += kTogether) {
+        Stored<FMT> kx[kTogether], vx[kTogether];
+        int row[kTogether], head[kTogether];
+#pragma unroll
+        for (int u = 0; u < kTogether; u++) {
+            row[u] = pairs.row(u0 + u, head[u]);
+            const int64_t p = place[row[u]];
+            if (p < 0) continue;
+            const int64_t at = p + ((int64_t)head[u] << a.log_page);
+            kx[u] = fetch<HD, FMT>(a.k, a.k_scale, at, e0);
+            vx[u] = fetch<HD, FMT>(a.v, a.v_scale, at, e0);
+        }
+#pragma unroll
+        for (int u = 0; u < kTogether; u++) {
+            if (place[row[u]] < 0) continue;
+            const int64_t at = (pairs.row0 + row[u]) * ld + head[u] * HD + e0;
+            float x[8];
+            values_of<FMT>(kx[u], x);
+            store8(k + at, x);
+            values_of<FMT>(vx[u], x);
+            store8(v + at, x);
+        }
+    }
 }
 
 template <typename T, bool APPEND, typename P>
@@ -213,7 +304,7 @@ int rows_entry(const lai_paged_kv_t *kv, const lai_paged_batch_t *b, P k, P v, i
         const uintptr_t w = (uintptr_t)width * sizeof(T);
         if (d % row < w || row - d % row < w) return LAI_ERR_ALIAS;
     }
-    const int64_t pairs = n_rows * kv->n_kv_heads, per = kThreads / (kv->head_dim / 8);
+    const int64_t pairs = n_rows * kv->n_kv_heads, per = kThreads / (kv->head_dim / 8) * kUnits;
     if ((pairs + per - 1) / per > INT32_MAX) return LAI_ERR_RANGE;
     const dim3 grid(grid_for(pairs, per));
     const cudaStream_t cs = as_stream(stream);

@@ -100,6 +100,12 @@ __device__ __forceinline__ int first_seq(const View &a, int64_t row) {
     return s;
 }
 
+__device__ __forceinline__ float max_abs3(float x, float y, float z) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(x)), "f"(fabsf(y)), "f"(fabsf(z)));
+    return r;
+}
+
 // Write a lane's 8 elements (and lane 0 its row's scale) where ok; all lanes take part in the
 // maximum.
 template <int HD, int FMT>
@@ -110,24 +116,28 @@ __device__ __forceinline__ void put(unsigned char *cache, float *scale, int64_t 
         return;
     }
     constexpr float kTop = Fmt<FMT>::kTop;
-    // |x| by bits: an unsigned maximum orders magnitudes and keeps an infinity or a NaN on top
-    uint32_t top = 0;
+    // the largest magnitude; a NaN stays one
+    float top = max_abs3(x[0], x[1], x[2]);
+    top = max_abs3(top, x[3], x[4]);
+    top = max_abs3(max_abs3(top, x[5], x[6]), x[7], 0.f);
 #pragma unroll
-    for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = HD / 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const bool finite = top < 0x7f800000u;
-    float s = __fdiv_rn(__uint_as_float(top), kTop);
+    for (int o = HD / 16; o > 0; o >>= 1) top = max_abs3(top, __shfl_xor_sync(0xffffffffu, top, o), 0.f);
+    const bool finite = top < __int_as_float(0x7f800000);
+    float s = __fdiv_rn(top, kTop);
     s = s > 0.f ? s : 1.f;
     uint32_t w[2] = {0, 0};
     if (finite) {
         if (s > 1e-30f && s < 1e30f) {
             const float y = __frcp_rn(s);
+            const float2 y2 = make_float2(y, y), ns2 = make_float2(-s, -s);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float q = x[e] * y;
-                q = fmaf(fmaf(-q, s, x[e]), y, q);
-                x[e] = fmaf(fmaf(-q, s, x[e]), y, q);
+            for (int e = 0; e < 8; e += 2) {
+                const float2 v = make_float2(x[e], x[e + 1]);
+                float2 q = __fmul2_rn(v, y2);
+                q = __ffma2_rn(__ffma2_rn(q, ns2, v), y2, q);
+                q = __ffma2_rn(__ffma2_rn(q, ns2, v), y2, q);
+                x[e] = q.x;
+                x[e + 1] = q.y;
             }
         } else {
 #pragma unroll

@@ -373,7 +373,8 @@ LAI_API int lai_paged_kv_read_f32(float *k, float *v, int64_t ld, int64_t n_rows
  * becomes 0. q [n_rows, n_heads * head_dim] with row stride ld_q elements, out dense; query head h
  * reads kv head h / (n_heads / n_kv_heads), a group of at most 16. Keys in a page outside
  * [0, n_pages) count as not seen and set LAI_DEVERR_PAGE. What lies in the cache behind kv_len,
- * or at positions a row does not see, does not reach that row, whatever its bits. Scores, softmax
+ * or at positions a row does not see, does not reach that row, whatever its bits; an infinity or
+ * NaN that it does see makes what it touches an infinity or NaN. Scores, softmax
  * and sums are F32; with F32 q the products are exact to about F32 too (16-bit operands split
  * into terms), with BF16 q and a BF16 cache the weights of the values may be rounded to BF16.
  * scratch: lai_paged_attention_scratch_bytes(head_dim) bytes, zeroed once before first use; every

@@ -717,6 +717,7 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
     AttnArgs a;
     const int st = check(kv, b, n_rows, &a.kv);
     if (st != LAI_OK) return st;
+    if (n_rows == 0 || b->n_seqs == 0) return LAI_OK;
     constexpr int kEsize = QF32 ? 4 : 2;
     if (!out || !q || !scratch || n_heads <= 0 || window < 0 || n_heads % kv->n_kv_heads != 0 ||
         n_heads / kv->n_kv_heads > 16)
@@ -725,7 +726,6 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
     if (ld_q < width || ld_q % (16 / kEsize) != 0 || !aligned16(q) || !aligned16(out) ||
         !aligned16(scratch))
         return LAI_ERR_INVALID;
-    if (n_rows == 0 || b->n_seqs == 0) return LAI_OK;
     if (n_rows * (n_heads / kv->n_kv_heads) + b->n_seqs >= 1 << 28) return LAI_ERR_RANGE;
     const size_t ob = paged::row_bytes(n_rows, width, width, kEsize);
     const size_t qb = paged::row_bytes(n_rows, ld_q, width, kEsize);

@@ -51,8 +51,9 @@ struct Cfg {
     static constexpr int kRaw = kF16 ? 3 : 0;          // 8-bit tiles in the staging ring
     static constexpr int kRawTile = 128 * HD;
     static constexpr int kLand = kF16 ? kRaw : kStages;  // tiles that copies land in
-    // binary16 weights: 2^kLift at the row's maximum, below 2^15 after kGrow and a value scale
-    static constexpr float kLift = kF16 ? 5.f : 0.f;
+    // binary16 weights: 2^kLift at the row's maximum, at most 2^14 with kGrow (two tiles) and a value
+    // scale's mantissa, so that small ones are held to 2^-25 of 2^kLift
+    static constexpr float kLift = !kF16 ? 0.f : QF32 ? 13.f : 5.f;
     // Of 8 exponentials, those that the FMA pipe takes: with 8-bit caches 2 (2048 tokens over 32768
     // INT8 keys, 16 heads of 128: 587 us with none, 588 with 1, 524 with 2, 640 with 3), with BF16
     // ones none (466, 467, 476, 477 us).
@@ -770,8 +771,13 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         if (kF16) vs = v4[kF16 ? 8 * g + i / 2 : 0];
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            float2 p = __ffma2_rn(x[i + h], c2, nb2);
-                            // (a masked score's weight must be exactly 0, and F32 results exact)
+                            // (the packed product and sum would become one fused operation)
+                            float2 p = decltype(mask)::value
+                                           ? make_float2(__fsub_rn(__fmul_rn(x[i + h].x, c), base),
+                                                         __fsub_rn(__fmul_rn(x[i + h].y, c), base))
+                                           : __ffma2_rn(x[i + h], c2, nb2);
+                            // (a masked score's weight must be exactly 0, and F32 results exact; scores
+                            // of 2^20 and more are rounded before the subtraction as the maximum was)
                             if (!QF32 && !decltype(mask)::value && ((i + h) * C::kPolyOf8 & 7) < C::kPolyOf8)
                                 p = exp2_poly(p);
                             else
@@ -793,6 +799,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 auto fetch = [&](int g, float2 *x) {  // without waiting
                     umma::tmem_ld_32x32b_x32(t_s + 32 * g, *reinterpret_cast<uint32_t (*)[32]>(x));
                 };
+                auto is_big = [&](float top) { return __any_sync(0xffffffffu, fabsf(top * c) > 1048576.f); };
                 // moves off to the block's maximum; what l and O must be multiplied with
                 auto move = [&](float top, float slack) -> float {
                     // an infinite or NaN score: no weight of this row means anything any more
@@ -810,28 +817,32 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
 #pragma unroll
                     for (int g = 0; g < 4; g++) fetch(g, x + 16 * g);
                     umma::tmem_wait_ld();
-                    auto block = [&](auto mask) {
-                        float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+                    float part[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+                    auto scale_all = [&](auto mask) {
 #pragma unroll
-                        for (int g = 0; g < 4; g++) scale32(g, x + 16 * g, top[g], mask);
-                        const float f = move(max3(max3(top[0], top[1], top[2]), top[3], top[3]), kGrow);
-                        if (b > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-                            // the scores' MMAs came after the last P V, so O is complete
+                        for (int g = 0; g < 4; g++) scale32(g, x + 16 * g, part[g], mask);
+                    };
+                    if (masked) scale_all(Yes{}); else scale_all(No{});
+                    const float top = max3(max3(part[0], part[1], part[2]), part[3], part[3]);
+                    const float f = move(top, kGrow);
+                    if (b > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+                        // the scores' MMAs came after the last P V, so O is complete
 #pragma unroll 1
-                            for (int g = 0; g < HD / 16; g++) {
-                                uint32_t y[16];
-                                umma::tmem_ld_32x32b_x16(t_pv + 16 * g, y);
-                                umma::tmem_wait_ld();
+                        for (int g = 0; g < HD / 16; g++) {
+                            uint32_t y[16];
+                            umma::tmem_ld_32x32b_x16(t_pv + 16 * g, y);
+                            umma::tmem_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 16; i++) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-                                tmem_st_x16(t_pv + 16 * g, y);
-                            }
+                            for (int i = 0; i < 16; i++) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                            tmem_st_x16(t_pv + 16 * g, y);
                         }
-                        const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
+                    }
+                    const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
+                    auto weigh_all = [&](auto mask) {
 #pragma unroll
                         for (int g = 0; g < 4; g++) weigh(g, x + 16 * g, base, mask);
                     };
-                    if (masked) block(Yes{}); else block(No{});
+                    if (masked || is_big(top)) weigh_all(Yes{}); else weigh_all(No{});
                 } else {
                     auto pass1 = [&](auto mask) {
                         float top = neg_inf();
@@ -863,7 +874,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                             weigh(g, x, base, mask);
                         }
                     };
-                    if (masked) pass2(Yes{}); else pass2(No{});
+                    if (masked || is_big(top)) pass2(Yes{}); else pass2(No{});
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }

@@ -298,10 +298,10 @@ int rows_entry(const lai_paged_kv_t *kv, const lai_paged_batch_t *b, P k, P v, i
     View a;
     const int st = paged::check(kv, b, n_rows, &a);
     if (st != LAI_OK) return st;
+    if (n_rows == 0 || b->n_seqs == 0) return LAI_OK;
     const int64_t width = (int64_t)kv->n_kv_heads * kv->head_dim;
     if (!k || !v || ld < width || ld % (16 / (int)sizeof(T)) != 0 || !aligned16(k) || !aligned16(v))
         return LAI_ERR_INVALID;
-    if (n_rows == 0 || b->n_seqs == 0) return LAI_OK;
     const size_t nb = paged::row_bytes(n_rows, ld, width, sizeof(T));
     if (paged::hits_cache(kv, k, nb) || paged::hits_cache(kv, v, nb)) return LAI_ERR_ALIAS;
     const size_t cb = paged::cache_bytes(kv), sb = paged::scale_bytes(kv);

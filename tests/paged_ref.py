@@ -66,8 +66,8 @@ def sequence(vals, pages, n):
 
 def attend(q, k, v, pos0, scale, window=0):
     """q [n, H, hd], k / v [keys, Hkv, hd] float64, query i at position pos0 + i. Returns
-    (o, sum_j p_j |v_j|, max_j scale * sum_d |q_d k_d|): the result and what its error scales
-    with. Rows that see nothing are 0."""
+    (o, sum_j p_j |v_j|, max_j scale * sum_d |q_d k_d|, keys * max |v|): the result and what its
+    error scales with. Rows that see nothing are 0."""
     n, H, hd = q.shape
     G = H // k.shape[1]
     kh, vh = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
@@ -85,10 +85,11 @@ def attend(q, k, v, pos0, scale, window=0):
     a = torch.einsum("hnk,khd->nhd", w, vz.abs())
     b = torch.einsum("nhd,khd->hnk", q.abs(), kh.abs()) * scale
     b = b.masked_fill(~see, 0.0).amax(-1).T[..., None] if k.shape[0] else torch.zeros_like(o[..., :1])
-    return o, a, b
+    u = k.shape[0] * vz.abs().amax((0, 2))[:, None] if k.shape[0] else torch.zeros_like(o[..., :1])
+    return o, a, b, u
 
 
-def tolerance(o, a, b, dtype, cache):
+def tolerance(o, a, b, u, dtype, cache):
     """Bound on |out - o|, elementwise.
 
     Scores: an operand is within 2^-22 of itself (binary16 hi + lo; three bfloat16 terms do
@@ -97,8 +98,15 @@ def tolerance(o, a, b, dtype, cache):
     terms together. exp turns an absolute error d of a score into a relative 2 d of its weight at
     most, and again of the sum that divides. Weights and values: as the operands, 2^-17 of a.
     BF16 queries may have weights rounded to BF16 (half a step, 2^-8) before a BF16 cache, binary16
-    (2^-11) before an 8-bit one. The result is rounded to dtype (half a step)."""
+    (2^-11) before an 8-bit one. The result is rounded to dtype (half a step).
+
+    Before an 8-bit cache a weight times its value's scale is held in binary16, whose smallest step
+    is 2^-24: as hi + lo it is off by up to 2^-25, however small it is itself, where the row's largest
+    weight and the largest scale make 2^13 (F32) or 2^5 (BF16) to twice that. So each of the keys
+    may add 2^-38 (2^-30) of the largest value, which u sums; 2^-37 (2^-29) for the factor of two."""
     t = a * (4 * b * 2.0 ** -16 + 2.0 ** -17)
+    if cache != torch.bfloat16:
+        t = t + u * (2.0 ** -37 if dtype == torch.float32 else 2.0 ** -29)
     if dtype == torch.bfloat16:
         t = t + a * (2.0 ** -8 if cache == torch.bfloat16 else 2.0 ** -11) + (o.abs() + t) * 2.0 ** -8
     return t + 1e-37

@@ -957,7 +957,9 @@ class DecodeLinear:
 class TtsConfig:
     """Shapes of run_decode_loop's per-frame work (src/tts_native.h:29-56). Defaults: the
     Qwen3-TTS 0.6B talker (hidden 1024, FFN 3072, 28 layers) and its 5-layer code predictor
-    of the same width (mtp_project is then a copy, src/tts_native.c:88-99)."""
+    of the same width (mtp_project is then a copy, src/tts_native.c:88-99). kv_cache: the
+    talker's cache, "f32" (dense, as the reference keeps it) or paged in "bf16", "e4m3" or "i8"
+    (pages of kv_page tokens)."""
     name: str = "qwen3-tts-0.6b"
     hidden: int = 1024
     inter: int = 3072
@@ -978,6 +980,8 @@ class TtsConfig:
     temperature: float = 0.9
     top_k: int = 50
     penalty: float = 1.05
+    kv_cache: str = "f32"
+    kv_page: int = 64
 
 
 class TtsFrame:
@@ -1040,9 +1044,21 @@ class TtsFrame:
         self.trailing = (0.5 * torch.randn((frames, H), generator=g, device=device)).to(f32)
         self.draws = torch.rand((frames, c.groups), generator=g, device=device)
         # caches, tables, buffers
-        self.kc = [torch.zeros((1, c.max_seq, kvd), dtype=f32, device=device)
-                   for _ in range(c.layers)]
-        self.vc = [torch.zeros_like(k) for k in self.kc]
+        self.batch = None
+        if c.kv_cache == "f32":
+            self.kc = [torch.zeros((1, c.max_seq, kvd), dtype=f32, device=device)
+                       for _ in range(c.layers)]
+            self.vc = [torch.zeros_like(k) for k in self.kc]
+        else:  # a paged cache per layer; one sequence, its pages handed out last to first
+            fmt = {"bf16": bf, "e4m3": torch.float8_e4m3fn, "i8": torch.int8}[c.kv_cache]
+            n_pages = -(-c.max_seq // c.kv_page)
+            self.kc = [lai.PagedKV.allocate(n_pages, c.n_kv, c.kv_page, c.head_dim, fmt, device)
+                       for _ in range(c.layers)]
+            self.vc = None
+            i32 = dict(dtype=torch.int32, device=device)
+            self.kv_len = torch.ones(1, **i32)  # keys with the frame's own: pos + 1
+            self.batch = lai.PagedBatch(torch.arange(2, **i32), self.kv_len,
+                                        torch.arange(n_pages - 1, -1, -1, **i32)[None])
         self.cp_kc = [torch.zeros((1, c.groups, kvd), dtype=f32, device=device)
                       for _ in range(c.cp_layers)]
         self.cp_vc = [torch.zeros_like(k) for k in self.cp_kc]
@@ -1050,7 +1066,8 @@ class TtsFrame:
         self.cos, self.sin = lai.rope_table(pos_all, c.max_seq, c.head_dim, c.theta,
                                             device=device)
         self.cp_pos = torch.arange(c.groups, dtype=torch.int32, device=device)
-        self.scr = lai.decode_attention_scratch(1, c.n_q, c.n_kv, c.max_seq, device)
+        self.scr = lai.decode_attention_scratch(1, c.n_q, c.n_kv, c.max_seq, device) \
+            if self.batch is None else lai.paged_attention_scratch(c.head_dim, device)
         self.cp_scr = lai.decode_attention_scratch(1, c.n_q, c.n_kv, c.groups, device)
         self.pos = torch.zeros(1, dtype=torch.int32, device=device)
         self.x = torch.zeros((1, H), dtype=f32, device=device)
@@ -1081,10 +1098,17 @@ class TtsFrame:
         act = self.act[:, :inter]
         for i, L in enumerate(layers):
             lai.gemv(self.x, L["wqkv"], L["in_norm"], c.eps, y=self.qkv, stream=stream)
-            # per-head q/k RMSNorm + RoPE at pos, cache append and attention: one launch
-            lai.decode_attention(q, k, v, kc[i], vc[i], pos, c.n_q, c.n_kv, scratch=scr,
-                                 out=self.attn, err=self.err, stream=stream,
-                                 qk=(L["q_norm"], L["k_norm"], self.cos, self.sin, c.eps))
+            if vc is not None:
+                # per-head q/k RMSNorm + RoPE at pos, cache append and attention: one launch
+                lai.decode_attention(q, k, v, kc[i], vc[i], pos, c.n_q, c.n_kv, scratch=scr,
+                                     out=self.attn, err=self.err, stream=stream,
+                                     qk=(L["q_norm"], L["k_norm"], self.cos, self.sin, c.eps))
+            else:  # the same in three, over the paged cache
+                lai.qk_norm_rope(q, k, L["q_norm"], L["k_norm"], self.cos, self.sin, pos, c.n_q,
+                                 c.n_kv, c.head_dim, c.eps, err=self.err, stream=stream)
+                lai.paged_kv_append(kc[i], self.batch, k, v, err=self.err, stream=stream)
+                lai.paged_attention(q, kc[i], self.batch, scratch=scr, out=self.attn,
+                                    err=self.err, stream=stream)
             lai.gemv_residual(self.x, self.attn, L["wo"], stream=stream)
             lai.gemv_swiglu(self.x, L["wgu"], L["post_norm"], c.eps, out=act, stream=stream)
             lai.gemv_residual(self.x, act, L["wd"], stream=stream)
@@ -1158,12 +1182,14 @@ class TtsFrame:
             lai.add(self.codec_sum, self.x, stream=stream)
         lai.add(self.codec_sum, self.trail_frame, stream=stream)
         self.pos.add_(1)
+        if self.batch is not None:
+            self.kv_len.add_(1)
 
     def launches_per_frame(self) -> int:
         """Library kernels per frame (the 2 tensor copies and the position add not counted)."""
         c = self.cfg
         per_layer = 5
-        return (c.layers * per_layer + 2 + 3 + c.groups * c.cp_layers * per_layer + 1
+        return (c.layers * (per_layer if self.batch is None else per_layer + 2) + 2 + 3 + c.groups * c.cp_layers * per_layer + 1
                 + (c.groups - 1) * 4 + 1)
 
     def weight_bytes_per_frame(self) -> int:

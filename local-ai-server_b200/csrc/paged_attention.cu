@@ -371,25 +371,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                 sc[n][0] = cs[n][0] + cs[n][2];
                 sc[n][1] = cs[n][1] + cs[n][3];
             }
-            // ---- values and scales, and the slot is free for the next chunk
-            uint32_t vr[NK][4][VW];
-#pragma unroll
-            for (int kk = 0; kk < NK; kk++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const unsigned char *p = from + Ck::kV + (16 * kk + 2 * t + (i & 1) + 8 * (i >> 1)) * Ck::kRow;
-                    if constexpr (VW == 2) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(p + 8 * g);
-                        vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < VW / 4; c++) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(p + 16 * g + 128 * c);
-                            vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
-                            vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
-                        }
-                    }
-                }
+            // ---- mask, running maximum
             float2 ks[NB], vs[NB];
             if (kF16) {
 #pragma unroll
@@ -398,9 +380,6 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     vs[n] = *reinterpret_cast<const float2 *>(from + Ck::kScaleV + (8 * n + 2 * t) * 4);
                 }
             }
-            __syncwarp();
-            if (lane == 0) bulk::mbar_arrive(&sm.empty[slot]);
-            // ---- mask, running maximum
             const bool uneven = mixed(tl, a.window, j0, kStep);
             const bool all = whole && !uneven;  // every row sees every key
             float top = neg_inf(), vtop = 0.f;
@@ -468,6 +447,25 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     pk[1] = pack2<kF16>(p0, p1);
                 }
             }
+            // ---- values
+            uint32_t vr[NK][4][VW];
+#pragma unroll
+            for (int kk = 0; kk < NK; kk++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const unsigned char *p = from + Ck::kV + (16 * kk + 2 * t + (i & 1) + 8 * (i >> 1)) * Ck::kRow;
+                    if constexpr (VW == 2) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(p + 8 * g);
+                        vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < VW / 4; c++) {
+                            const uint4 x = *reinterpret_cast<const uint4 *>(p + 16 * g + 128 * c);
+                            vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
+                            vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
+                        }
+                    }
+                }
             // What is not there may be anything, and weight 0 times it has to be 0. And a step whose
             // keys some rows of the tile see and others do not gives every row 0 x v for the keys it
             // must not see: infinities and NaN are taken out of such a step, and added to the rows
@@ -536,6 +534,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     }
                 }
             }
+            __syncwarp();
+            if (lane == 0) bulk::mbar_arrive(&sm.empty[slot]);
         }
 
         // ---- join the warps: the upper half's sums into the lower half's, those in shared memory

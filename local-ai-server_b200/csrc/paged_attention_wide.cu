@@ -13,7 +13,8 @@
 //     under the other's MMAs. A softmax thread owns a row (no shuffles) and holds the block's 128
 //     scores in registers; P overwrites S in TMEM. The maximum that weights are relative to only
 //     moves when it has grown by 2^8, so O is hardly ever rescaled.
-//   * F32 queries: one tile of 128 rows, its terms (hi + lo binary16; three bfloat16 terms over a
+//   * F32 queries: one tile of 128 rows, whose softmax the two warpgroups share (a thread of each
+//     per row, for half of the block's keys and half of the output's columns), its terms (hi + lo binary16; three bfloat16 terms over a
 //     BF16 cache) one after another into the same accumulator, smallest first, the weights the
 //     same. A block's P V starts from zero and is added to the output row, which the thread keeps
 //     in registers, so long sequences do not add up the MMA's truncated sums.
@@ -47,7 +48,7 @@ struct Cfg {
     static constexpr int MT = QF32 ? 1 : 2;
     static constexpr int R = 128 * MT;
     static constexpr int kTile = 128 * HD * 2;         // bytes of an operand tile
-    static constexpr int kStages = kF16 ? 3 : QF32 ? 4 : 5;
+    static constexpr int kStages = kF16 || QF32 ? 3 : 5;
     static constexpr int kRaw = kF16 ? 3 : 0;          // 8-bit tiles in the staging ring
     static constexpr int kRawTile = 128 * HD;
     static constexpr int kLand = kF16 ? kRaw : kStages;  // tiles that copies land in
@@ -76,6 +77,7 @@ struct Ctl {
     using C = Cfg<HD, FMT, QF32>;
     static constexpr int kScales = C::kF16 ? kU : 4;
     float kscale[kRing][kScales], vscale[kRing][kScales];  // 16-byte aligned
+    float swap[QF32 ? 2 : 1][2][QF32 ? 128 : 1];           // between the halves of a row
     uint64_t landed[C::kLand], taken[C::kLand], full[C::kStages], empty[C::kStages];
     uint64_t info[kRing], item_full[kItems], item_empty[kItems];
     Item items[kItems];
@@ -264,11 +266,11 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         }
         for (int i = 0; i < kItems; i++) {
             bulk::mbar_init(&ctl.item_full[i], 1);
-            bulk::mbar_init(&ctl.item_empty[i], 4 + 1 + 4 * MT);
+            bulk::mbar_init(&ctl.item_empty[i], 4 + 1 + 8);
         }
         for (int i = 0; i < 2; i++) {
-            bulk::mbar_init(&ctl.q_full[i], 128);
-            bulk::mbar_init(&ctl.group[i], 128);
+            bulk::mbar_init(&ctl.q_full[i], 256 / MT);
+            bulk::mbar_init(&ctl.group[i], 256 / MT);
             bulk::mbar_init(&ctl.s_full[i], 1);
             bulk::mbar_init(&ctl.p_full[i][0], 128);
             bulk::mbar_init(&ctl.p_full[i][1], 128);
@@ -319,8 +321,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
     };
     const int in_page = a.kv.page_size() - 1;
 
-    // Register shares: 2 x 128 x 192 + 2 x 128 x 64 = 512 x 128 (fewer where one warpgroup softmaxes)
-    if (wg < MT) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    // Register shares: 2 x 128 x 192 + 2 x 128 x 64 = 512 x 128
+    if (wg < 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
 
     if (warp == 13) {
@@ -580,16 +582,28 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             const uint64_t t0 = bulk::globaltimer_ns();
             while (bulk::globaltimer_ns() - t0 < 1000000ull) {}
         }
-    } else if (wg < MT) {
-        // ================= softmax: a thread per row =========================================
-        const int mt = wg;
+    } else if (wg < 2) {
+        // ================= softmax: a thread per row, or two =================================
+        // Two tiles: warpgroup = tile. One tile: warpgroup `half` has keys 64 half .. of a block and
+        // columns HD / 2 half .. of the output.
+        constexpr bool kSplit = MT == 1;
+        constexpr int kCols = kSplit ? HD / 2 : HD;
+        const int mt = kSplit ? 0 : wg, half = kSplit ? wg : 0;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + lane_base + mt * 128, t_p = t_s + kP, t_pv = tmem + lane_base + kPV + mt * 128;
+        const uint32_t t_s = tmem + lane_base + mt * 128, t_p = t_s + kP, t_pv = tmem + lane_base + kPV + mt * 128 + half * kCols;
         uint32_t n = 0, blocks = 0, n_group = 0, n_last = 0;  // this tile's blocks, all blocks, joins, last P Vs
         bool ok = true;
-        auto join = [&]() {  // all of the warpgroup, within the bound
+        auto join = [&]() {  // all that work on the tile, within the bound
             bulk::mbar_arrive(&ctl.group[mt]);
             return wait(&ctl.group[mt], n_group++ & 1);
+        };
+        // the other half's value of this row
+        auto exchange = [&](float x, float &other) -> bool {
+            float (*buf)[QF32 ? 128 : 1] = ctl.swap[QF32 ? n_group & 1 : 0];
+            buf[half][QF32 ? wt : 0] = x;
+            if (!(ok = join())) return false;
+            other = buf[1 - half][QF32 ? wt : 0];
+            return true;
         };
         while (next(ok)) {
             const int nb = it.blk1 - it.blk0;
@@ -607,11 +621,12 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             const int wrow = (warp & 3) * 32;                            // the warp's first row of it
             constexpr int kElem = QF32 ? 4 : 2, kLanes = HD * kElem / 16, kAtOnce = 32 / kLanes;
             const int run = lane % kLanes, sub = lane / kLanes;
-            // row sub + p * kAtOnce of the warp as token and head of the group, p counting up
-            int tk, gh;
-            const int step_t = a.by_group.of(kAtOnce), step_g = kAtOnce - step_t * a.group;
-            auto first_row = [&]() {
-                const int f = it.row0 + mt * 128 + wrow + sub;
+            // rows of the warp as token and head of the group, counting up by `step`
+            int tk, gh, step_t, step_g;
+            auto first_row = [&](int from, int step) {
+                step_t = a.by_group.of(step);
+                step_g = step - step_t * a.group;
+                const int f = it.row0 + mt * 128 + wrow + from;
                 tk = a.by_group.of(f);
                 gh = f - tk * a.group;
             };
@@ -625,7 +640,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 constexpr int kBatch = 32 / kAtOnce < 16 ? 32 / kAtOnce : 16;  // loads under way per lane
                 const char *src = static_cast<const char *>(qp) +
                                   ((int64_t)it.q_row0 * a.ld_q + (int64_t)head * a.group * HD) * kElem + run * 16;
-                first_row();
+                first_row(sub, kAtOnce);
 #pragma unroll 1
                 for (int p0 = 0; p0 < 32 / kAtOnce; p0 += kBatch) {
                     uint4 raw[kBatch];
@@ -637,6 +652,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                             raw[p] = __ldg(reinterpret_cast<const uint4 *>(src + (tk * a.ld_q + gh * HD) * kElem));
                         next_row();
                     }
+                    // (the other half has stored what it staged in these tiles)
+                    if (kSplit && p0 == 0 && !(ok = join())) break;
 #pragma unroll
                     for (int p = 0; p < kBatch; p++) {
                         const int rr = (p0 + p) * kAtOnce + sub;
@@ -658,6 +675,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                             const int mine = __shfl_sync(0xffffffffu, e, lane % kAtOnce * kLanes);
                             if (lane / kAtOnce == p0 + p) c = a.scale_log2 * pow2i(mine - 13);
                         }
+                        // (each half has seen all rows' maxima, and writes half of the rows)
+                        if (kSplit && ((p0 + p) * kAtOnce >= 16) != (half == 1)) continue;
                         if constexpr (QF32) {  // 4 values: half a 16-byte run of every term
                             float x[4] = {__uint_as_float(raw[p].x), __uint_as_float(raw[p].y),
                                           __uint_as_float(raw[p].z), __uint_as_float(raw[p].w)};
@@ -687,6 +706,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         }
                     }
                 }
+                if (!ok) break;
                 c = fmaxf(c, 1.2e-38f);  // masked scores, -inf, stay -inf
                 bulk::fence_proxy_async_smem();
                 bulk::mbar_arrive(&ctl.q_full[mt]);
@@ -696,7 +716,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             float m = neg_inf(), off = neg_inf(), l = 0.f, alpha = 0.f;
             int ve = kF16 ? -90 : 0;
             bool bad = false;
-            constexpr int kKeep = MT == 1 ? HD : 1;
+            constexpr int kKeep = kSplit ? kCols : 1;
             float o[kKeep];
 #pragma unroll
             for (int d = 0; d < kKeep; d++) o[d] = 0.f;
@@ -790,7 +810,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     }
 #pragma unroll
                     for (int t = 0; t < kTerms; t++) tmem_st_x16(t_p + t * 64 + 16 * g, w[t]);
-                    if (g & 1) {  // half of P is there
+                    if (g & 1) {  // 64 keys' weights are there
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                         umma::fence_before_sync();
                         bulk::mbar_arrive(&ctl.p_full[mt][g >> 1]);
@@ -844,18 +864,18 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     };
                     if (masked || is_big(top)) weigh_all(Yes{}); else weigh_all(No{});
                 } else {
-                    auto pass1 = [&](auto mask) {
-                        float top = neg_inf();
+                    float2 x[kU / 4];  // this half's keys
+                    fetch(2 * half, x);
+                    fetch(2 * half + 1, x + 16);
+                    umma::tmem_wait_ld();
+                    float top = neg_inf(), other;
+                    auto scale_half = [&](auto mask) {
 #pragma unroll
-                        for (int g = 0; g < 4; g++) {
-                            float2 x[16];
-                            fetch(g, x);
-                            umma::tmem_wait_ld();
-                            scale32(g, x, top, mask);
-                        }
-                        return top;
+                        for (int g = 0; g < 2; g++) scale32(2 * half + g, x + 16 * g, top, mask);
                     };
-                    const float top = masked ? pass1(Yes{}) : pass1(No{});
+                    if (masked) scale_half(Yes{}); else scale_half(No{});
+                    if (!exchange(top, other)) break;
+                    top = max3(top, other, other);
                     if (b > 0) {  // P V of the block before, while S waited
                         if (!(ok = wait(&ctl.pv_full[mt], (n - 1) & 1))) break;
                         saw_bad(blocks - 1);
@@ -863,18 +883,11 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     }
                     alpha = move(top, 0.f);
                     const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
-                    auto pass2 = [&](auto mask) {
-                        float ignore = 0.f;
+                    auto weigh_half = [&](auto mask) {
 #pragma unroll
-                        for (int g = 0; g < 4; g++) {
-                            float2 x[16];
-                            fetch(g, x);
-                            umma::tmem_wait_ld();
-                            scale32(g, x, ignore, mask);
-                            weigh(g, x, base, mask);
-                        }
+                        for (int g = 0; g < 2; g++) weigh(2 * half + g, x + 16 * g, base, mask);
                     };
-                    if (masked || is_big(top)) pass2(Yes{}); else pass2(No{});
+                    if (masked || is_big(top)) weigh_half(Yes{}); else weigh_half(No{});
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
@@ -884,9 +897,14 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             umma::fence_after_sync();
             saw_bad(blocks - 1);
             if (MT == 1) add_pv();
-            // columns 32 g .. of the output row, before the division (rolled where it may be: the code
-            // of all roles shares the instruction cache)
-            constexpr int kPieces = MT == 2 ? 1 : HD / 32;
+            if constexpr (kSplit) {
+                float other;
+                if (!exchange(l, other)) break;
+                l += other;
+            }
+            // 32 of this thread's columns, before the division (rolled where it may be: the code of
+            // all roles shares the instruction cache)
+            constexpr int kPieces = kSplit ? kCols / 32 : 1;
             auto piece = [&](int g, float (&x)[32]) {
                 if constexpr (MT == 2) {
                     uint32_t u[32];
@@ -910,20 +928,20 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     const int64_t at = a.kv.page_base(page, head) + (j & in_page);
                     const float vs = kF16 ? __ldg(a.kv.v_scale + at) : 1.f;
 #pragma unroll 1
-                    for (int d = 0; d < HD; d++) {
+                    for (int d = half * kCols; d < half * kCols + kCols; d++) {
                         const float v = element<FMT>(a.kv.v, at * HD + d) * vs;
                         if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) add(d, v);
                     }
                 }
             };
             // 32 columns of this thread's row into the warp's rows of the Q tile (the next item's Q
-            // is not there yet): F32 has half of its columns in the second term's tile
+            // is not there yet), the second half's in the second term's tile: 2 HD bytes a row
+            const uint32_t staged = my_rows + half * MT * C::kTile;
             auto stage = [&](int g, const float (&x)[32], float inv) {
                 if (QF32) {
-                    const uint32_t tile = my_rows + (g >= HD / 64 ? MT * C::kTile : 0);
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        st_shared16(tile + chunk_off(wt, (8 * g + i) % (HD / 8)),
+                        st_shared16(staged + chunk_off(wt, 8 * g + i),
                                     make_uint4(__float_as_uint(x[4 * i] * inv), __float_as_uint(x[4 * i + 1] * inv),
                                                __float_as_uint(x[4 * i + 2] * inv), __float_as_uint(x[4 * i + 3] * inv)));
                 } else {
@@ -931,23 +949,23 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     for (int i = 0; i < 4; i++) {
                         const float y[8] = {x[8 * i] * inv, x[8 * i + 1] * inv, x[8 * i + 2] * inv, x[8 * i + 3] * inv,
                                             x[8 * i + 4] * inv, x[8 * i + 5] * inv, x[8 * i + 6] * inv, x[8 * i + 7] * inv};
-                        st_shared16(my_rows + chunk_off(wt, 4 * g + i), pack<uint16_t>(y));
+                        st_shared16(staged + chunk_off(wt, 4 * g + i), pack<uint16_t>(y));
                     }
                 }
             };
             auto store = [&]() {  // the warp's staged rows, in whole lines
+                constexpr int kOut = HD / 8, kOutRows = 32 / kOut;  // lanes a row, rows at once
+                const int oc = lane % kOut, from = lane / kOut;
                 __syncwarp();
                 char *dst = static_cast<char *>(out) +
-                            ((int64_t)it.q_row0 * a.kv.n_kv + head) * a.group * (HD * kElem) + run * 16;
+                            ((int64_t)it.q_row0 * a.kv.n_kv + head) * a.group * (HD * kElem) + half * (HD * 2) + oc * 16;
                 const int64_t tok_bytes = (int64_t)a.kv.n_kv * a.group * (HD * kElem);
-                first_row();
+                first_row(from, kOutRows);
 #pragma unroll 4
-                for (int p = 0; p < 32 / kAtOnce; p++, next_row()) {
-                    const int rr = p * kAtOnce + sub;
+                for (int p = 0; p < 32 / kOutRows; p++, next_row()) {
+                    const int rr = p * kOutRows + from;
                     if (mt * 128 + wrow + rr >= it.rows) continue;
-                    const uint32_t tile = my_rows + (QF32 && run >= kLanes / 2 ? MT * C::kTile : 0);
-                    const uint4 v = ld_shared16(tile + chunk_off(wrow + rr, run % (HD / 8)));
-                    st_vec(dst + tk * tok_bytes + gh * (HD * kElem), v);
+                    st_vec(dst + tk * tok_bytes + gh * (HD * kElem), ld_shared16(staged + chunk_off(wrow + rr, oc)));
                 }
                 __syncwarp();
             };
@@ -957,26 +975,28 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             float mu = 0.f;
             if (!it.whole) {
                 float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * kPart;
-                pp[r] = off;
-                pp[R + r] = l;
+                if (half == 0) {
+                    pp[r] = off;
+                    pp[R + r] = l;
+                }
 #pragma unroll kPieces
-                for (int g = 0; g < HD / 32; g++) {
+                for (int g = 0; g < kCols / 32; g++) {
                     float x[32];
                     piece(g, x);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4 *>(pp + 2 * R + ((8 * g + i / 4) * R + r) * 4) =
+                        *reinterpret_cast<float4 *>(pp + 2 * R + ((half * (kCols / 4) + 8 * g + i / 4) * R + r) * 4) =
                             make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                 }
                 umma::fence_before_sync();
                 if (bad) mend([&](int d, float v) { pp[2 * R + (d / 4 * R + r) * 4 + d % 4] += v; });
                 __threadfence();
                 if (!(ok = join())) break;
-                if (wt == 0) ctl.last[mt] = atomicAdd(a.counters + it.c0 * MT + mt, 1) == it.c1 - it.c0;
+                if (wt == 0 && half == 0) ctl.last[mt] = atomicAdd(a.counters + it.c0 * MT + mt, 1) == it.c1 - it.c0;
                 if (!(ok = join())) break;
                 if (!*(volatile int *)&ctl.last[mt]) continue;
                 __threadfence();
-                if (wt == 0) a.counters[it.c0 * MT + mt] = 0;  // ready for the next call
+                if (wt == 0 && half == 0) a.counters[it.c0 * MT + mt] = 0;  // ready for the next call
                 float top = neg_inf();
                 for (int cc = it.c0; cc <= it.c1; cc++) top = fmaxf(top, __ldcg(part(cc) + r));
                 mu = top == neg_inf() ? 0.f : top;
@@ -986,7 +1006,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             }
             const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll kPieces
-            for (int g = 0; g < HD / 32; g++) {
+            for (int g = 0; g < kCols / 32; g++) {
                 float x[32];
                 if (it.whole) {
                     piece(g, x);
@@ -999,7 +1019,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         const float f = ex2(__ldcg(pc + r) - mu);
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * R + ((8 * g + i / 4) * R + r) * 4));
+                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * R + ((half * (kCols / 4) + 8 * g + i / 4) * R + r) * 4));
                             x[i] = fmaf(v.x, f, x[i]);
                             x[i + 1] = fmaf(v.y, f, x[i + 1]);
                             x[i + 2] = fmaf(v.z, f, x[i + 2]);
@@ -1013,8 +1033,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
             if (it.whole && bad)
                 mend([&](int d, float v) {
                     if (QF32) {
-                        float *p = reinterpret_cast<float *>(q_smem + (d >= HD / 2 ? MT * C::kTile : 0) +
-                                                             chunk_off(wt, d % (HD / 2) / 4) + d % 4 * 4);
+                        float *p = reinterpret_cast<float *>(q_smem + half * MT * C::kTile + chunk_off(wt, d % (HD / 2) / 4) + d % 4 * 4);
                         *p += v;
                     } else {
                         uint16_t *p = reinterpret_cast<uint16_t *>(q_smem + mt * C::kTile + chunk_off(wt, d / 8) + d % 8 * 2);

@@ -41,7 +41,6 @@ constexpr int kRows = 8;      // rows of a tile
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxCtas = kSMs * kCtasPerSm;
 constexpr int kCounters = 1024;  // ints at the front of the scratch
-constexpr int kWideRows = 32;    // more rows per sequence (on average) go to the wide kernel
 
 template <int FMT> __host__ __device__ constexpr int step_keys() { return FMT == LAI_KV_BF16 ? 16 : 32; }  // of a chunk
 template <int FMT> __host__ __device__ constexpr int block_keys() { return kWarps * step_keys<FMT>(); }
@@ -534,6 +533,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     }
                 }
             }
+            // (Not as soon as keys and values are in registers: with the release there, results were
+            // wrong now and then. Here the products have taken them.)
             __syncwarp();
             if (lane == 0) bulk::mbar_arrive(&sm.empty[slot]);
         }
@@ -710,6 +711,18 @@ int launch_few(void *out, const void *q, const AttnArgs &a, cudaStream_t st) {
     return launch_status();
 }
 
+// Which kernel. The few-row one reads the keys once per 8 rows of a sequence, the wide one once per
+// 128 or 256 but starts slowly and splits coarsely, so it wants several tiles of 8 in a sequence
+// and enough of them in all. Measured over 1500 keys, 16 heads on 8, us (few / wide):
+//   16 sequences: BF16 q, BF16 cache, 10 rows each 41 / 38, 24 rows 56 / 38; INT8 cache 16 rows
+//   43 / 49, 24 rows 55 / 49; F32 q, BF16 cache 16 rows 45 / 57, 24 rows 60 / 58; INT8 cache
+//   24 rows 49 / 57, 32 rows 62 / 57
+//   4 sequences of 32 rows: 26 / 24 (BF16 q, BF16), 28 / 31 (F32 q); 1 of 64: 19 / 25, 20 / 28.
+inline bool many_rows(int64_t rows, int n_seqs, int n_kv, bool f32, bool eight_bit) {
+    const int64_t per_seq = 8 + (eight_bit ? 8 : 0) + (f32 ? 8 : 0);
+    return rows > per_seq * n_seqs && rows / 8 * n_kv >= (f32 ? 256 : 128);
+}
+
 template <bool QF32>
 int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int n_heads,
                     const lai_paged_kv_t *kv, const lai_paged_batch_t *b, float scale, int window,
@@ -742,7 +755,8 @@ int attention_entry(void *out, const void *q, int64_t ld_q, int64_t n_rows, int 
     a.parts = reinterpret_cast<float *>(a.counters + kCounters);
     a.err = err;
     const cudaStream_t cs = as_stream(stream);
-    if (n_rows * a.group > (int64_t)kWideRows * b->n_seqs && a.scale_log2 > 1e-30f)
+    if (many_rows(n_rows * a.group, b->n_seqs, kv->n_kv_heads, QF32, kv->format != LAI_KV_BF16) &&
+        a.scale_log2 > 1e-30f)
         return attention_wide(out, q, QF32, kv->head_dim, kv->format, a, cs);
 #define LAI_FEW(FMT)                                                             \
     (kv->head_dim == 128 ? launch_few<128, FMT, QF32>(out, q, a, cs) : launch_few<64, FMT, QF32>(out, q, a, cs))

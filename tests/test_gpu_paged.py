@@ -203,16 +203,18 @@ def test_attention_window(window, cache, dtype):
 
 
 # many rows: one tile and its edges, blocks of 128 keys and theirs, several tiles, a long prefix,
-# long and short sequences in one batch, a sequence cut over many CTAs
+# long and short sequences in one batch, a sequence cut over many CTAs. (The kernel for many rows
+# needs 8 to 24 rows a sequence and 128 to 256 tiles of 8 rows over all kv heads; "many" below is
+# chosen to be above that.)
 WIDE = [([64, 65, 63], [64, 200, 129]), ([128], [128]), ([129, 200], [1000, 257]), ([700], [700]),
-        ([300, 1, 40], [4000, 777, 40]), ([100], [20000])]
+        ([300, 1, 40], [4000, 777, 40]), ([130], [20000])]
 
 
 @pytest.mark.parametrize("new,keys", WIDE)
 @pytest.mark.parametrize("cache", list(ref.FORMATS))
 @pytest.mark.parametrize("dtype", list(ref.DTYPES))
 def test_attention_wide(new, keys, cache, dtype):
-    Case(new, keys, 8, 4, 128, cache, 32, dtype, seed=len(new) + keys[0]).check()
+    Case(new, keys, 16, 8, 128, cache, 32, dtype, seed=len(new) + keys[0]).check()
 
 
 @pytest.mark.parametrize("H,Hkv,hd,page", [(4, 4, 64, 16), (6, 2, 64, 32), (8, 1, 128, 64),
@@ -220,7 +222,7 @@ def test_attention_wide(new, keys, cache, dtype):
 @pytest.mark.parametrize("cache", list(ref.FORMATS))
 @pytest.mark.parametrize("dtype", list(ref.DTYPES))
 def test_attention_wide_heads_and_pages(H, Hkv, hd, page, cache, dtype):
-    Case([150, 90], [333, 90], H, Hkv, hd, cache, page, dtype, seed=H).check()
+    Case([850, 300], [1033, 300], H, Hkv, hd, cache, page, dtype, seed=H).check()
 
 
 @pytest.mark.parametrize("window", [1, 37, 128, 300, 100000])
@@ -288,10 +290,10 @@ def test_empty_batches_do_nothing():
 @pytest.mark.parametrize("cache,dtype", [("bf16", "f32"), ("bf16", "bf16"), ("i8", "f32"), ("e4m3", "bf16")])
 def test_attention_garbage_behind_the_keys(garbage, new, keys, window, cache, dtype):
     # pages' ends, spare pages and their scales hold garbage
-    Case(new, keys, 4, 2, 128, cache, 64, dtype, seed=9, garbage=garbage).check(window=window)
+    Case(new, keys, 16, 8, 128, cache, 64, dtype, seed=9, garbage=garbage).check(window=window)
 
 
-@pytest.mark.parametrize("new,keys,window", [([6], [50], 0), ([2], [40], 8), ([200], [300], 0), ([180], [900], 60)])
+@pytest.mark.parametrize("new,keys,window", [([6], [50], 0), ([2], [40], 8), ([700], [800], 0), ([600], [900], 60)])
 @pytest.mark.parametrize("cache,dtype", [("bf16", "f32"), ("bf16", "bf16"), ("i8", "f32"), ("i8", "bf16"),
                                          ("e4m3", "f32"), ("e4m3", "bf16")])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
@@ -328,7 +330,7 @@ def test_attention_non_finite_values_reach_only_who_sees_them(new, keys, window,
         assert torch.equal(out[~sees], clean[~sees])
 
 
-@pytest.mark.parametrize("n", [4, 150])
+@pytest.mark.parametrize("n", [4, 1100])
 @pytest.mark.parametrize("cache", ["bf16", "i8"])
 def test_attention_non_finite_keys_reach_only_who_sees_them(n, cache):
     c = Case([n], [n + 30], 2, 1, 64, cache, 16, "f32", seed=4)
@@ -343,7 +345,7 @@ def test_attention_non_finite_keys_reach_only_who_sees_them(n, cache):
     assert torch.isnan(out[n // 2:]).all()
 
 
-@pytest.mark.parametrize("n", [2, 150])
+@pytest.mark.parametrize("n", [2, 400])
 def test_attention_bad_pages_and_lengths(n):
     """A page outside the pool counts as not there; a sequence with a length outside its table is
     skipped; the others are computed."""
@@ -378,14 +380,14 @@ def test_attention_bad_pages_and_lengths(n):
 
 
 # ---- numbers --------------------------------------------------------------------------------------
-@pytest.mark.parametrize("n", [1, 140])
+@pytest.mark.parametrize("n", [1, 530])
 @pytest.mark.parametrize("cache,dtype", [("bf16", "f32"), ("i8", "f32"), ("e4m3", "bf16"), ("bf16", "bf16")])
 @pytest.mark.parametrize("scale", [0.0, -0.1, 1e-6, 3.0])
 def test_attention_scales(n, cache, dtype, scale):
     Case([n], [n + 200], 4, 2, 128, cache, 16, dtype, seed=8).check(scale=scale)
 
 
-@pytest.mark.parametrize("n", [1, 140])
+@pytest.mark.parametrize("n", [1, 1100])
 @pytest.mark.parametrize("dtype", list(ref.DTYPES))
 @pytest.mark.parametrize("cache", list(ref.FORMATS))
 def test_attention_extreme_scores(n, dtype, cache):
@@ -412,7 +414,7 @@ def test_attention_extreme_scores(n, dtype, cache):
         assert (out - want[:, None]).abs().max() <= tol
 
 
-@pytest.mark.parametrize("n", [1, 140])
+@pytest.mark.parametrize("n", [1, 530])
 @pytest.mark.parametrize("cache", ["i8", "e4m3"])
 def test_attention_value_scales_over_many_orders(n, cache):
     """Value rows from 2^-40 to 2^40: the weights of small ones must not drown the large ones'."""
@@ -431,7 +433,7 @@ def test_attention_is_deterministic(cache, dtype):
     first = c.check(scratch=scratch)
     for _ in range(5):
         assert torch.equal(lai.paged_attention(c.q, c.kv, c.batch, scratch=scratch), first)
-    c = Case([300], [9000], 4, 2, 128, cache, 64, dtype, seed=13)
+    c = Case([600], [9000], 4, 2, 128, cache, 64, dtype, seed=13)
     first = c.check(scratch=scratch)  # the same scratch for the other kernel
     for _ in range(5):
         assert torch.equal(lai.paged_attention(c.q, c.kv, c.batch, scratch=scratch), first)
@@ -440,7 +442,7 @@ def test_attention_is_deterministic(cache, dtype):
 
 # ---- memory ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("cache", ["i8", "bf16"])
-@pytest.mark.parametrize("n", [1, 100])
+@pytest.mark.parametrize("n", [1, 300])
 def test_offsets_beyond_32_bits(cache, n):
     """A pool of more than 2^32 elements, its last pages in use."""
     hd, Hkv, page = 128, 8, 256
@@ -461,7 +463,7 @@ def test_offsets_beyond_32_bits(cache, n):
     assert ((out.double() - o.flatten(1)).abs() <= ref.tolerance(o, a, b, u, torch.float32, kv.k.dtype).flatten(1)).all()
 
 
-@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("n", [1, 530])
 def test_strided_rows_other_streams_and_outputs(n):
     H, Hkv, hd = 4, 2, 64
     c = Case([n, n], [n + 100, n], H, Hkv, hd, "e4m3", 16, "f32", seed=14)
@@ -486,7 +488,7 @@ def test_strided_rows_other_streams_and_outputs(n):
     assert (buf[:, Hkv * hd:2 * Hkv * hd] == 5).all()
 
 
-@pytest.mark.parametrize("n", [1, 100])
+@pytest.mark.parametrize("n", [1, 200])
 @pytest.mark.parametrize("cache", ["bf16", "i8"])
 def test_captured_in_a_graph_and_replayed_with_other_lengths(n, cache):
     """Append and attention as one graph; rows, lengths and pages change between replays."""
@@ -547,12 +549,12 @@ def test_prompt_then_tokens_equals_attention_over_the_whole_sequence(cache, dtyp
     needed. Every output equals attention over all rows so far."""
     H, Hkv, hd, page, S = 4, 2, 128, 16, 2
     dt, g = ref.DTYPES[dtype], gen(16)
-    kv = lai.PagedKV.allocate(64, Hkv, page, hd, ref.FORMATS[cache])
-    free = torch.randperm(64, generator=torch.Generator().manual_seed(1)).tolist()
-    pages = torch.full((S, 32), -1, dtype=torch.int32)
+    kv = lai.PagedKV.allocate(128, Hkv, page, hd, ref.FORMATS[cache])
+    free = torch.randperm(128, generator=torch.Generator().manual_seed(1)).tolist()
+    pages = torch.full((S, 64), -1, dtype=torch.int32)
     scratch, err = lai.paged_attention_scratch(hd), torch.zeros(1, dtype=torch.int32, device=DEV)
     lens, kept = [0] * S, [[] for _ in range(S)]
-    for new in ([100, 37], [90, 1], [1, 70], [1, 1], [1, 1], [5, 1]):
+    for new in ([600, 237], [90, 1], [1, 70], [1, 1], [1, 1], [5, 1]):
         for s, n in enumerate(new):
             lens[s] += n
             for j in range(-(-lens[s] // page)):

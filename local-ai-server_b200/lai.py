@@ -441,6 +441,7 @@ def _need_cuda(index, *tensors):
     for t in tensors:
         if t is not None and t.get_device() != index:
             index = -1
+            break
     if index < 0:
         raise ValueError("paged cache, batch and rows must be CUDA tensors of one device")
 
@@ -567,8 +568,8 @@ def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None)
     ranges these are whole sequences."""
     import torch
     fn = _paged_fn("lai_paged_kv_read", dtype)
-    k = torch.empty((rows, kv.width), dtype=dtype, device=kv.device) if k is None else k
-    v = torch.empty((rows, kv.width), dtype=dtype, device=kv.device) if v is None else v
+    k = kv.k.new_empty((rows, kv.width), dtype=dtype) if k is None else k
+    v = torch.empty_like(k) if v is None else v
     if k.dtype != dtype or v.dtype != dtype or k.shape[0] != rows or v.shape[0] != rows:
         raise ValueError("k and v must be [rows, n_kv_heads * head_dim] of dtype")
     ld = _paged_rows(k, kv.width)
@@ -610,7 +611,7 @@ def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, 
         raise ValueError("q must be [rows, n_heads * head_dim], n_heads a multiple of n_kv_heads")
     ld = _paged_rows(q, shape[1])
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=kv.device)
+        out = q.new_empty(shape)
     elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and dtype")
     if scratch is None:

@@ -370,7 +370,8 @@ LAI_API int lai_paged_kv_read_f32(float *k, float *v, int64_t ld, int64_t n_rows
  * qwen_causal_attention(out, q, K, V, n, kv_len, n_heads, n_kv, hd, scale, kv_len - n) per
  * sequence (src/tts_native.c:576-578 a prompt, :653-655 one token). A token at position p sees
  * keys p - window + 1 .. p (window 0: 0 .. p); a row that sees none (its position is negative)
- * becomes 0. q [n_rows, n_heads * head_dim] with row stride ld_q elements, out dense; query head h
+ * becomes 0. q [n_rows, n_heads * head_dim] with row stride ld_q elements, out dense and apart from
+ * q; both 16-byte aligned rows; query head h
  * reads kv head h / (n_heads / n_kv_heads), a group of at most 16. Keys in a page outside
  * [0, n_pages) count as not seen and set LAI_DEVERR_PAGE. What lies in the cache behind kv_len,
  * or at positions a row does not see, does not reach that row, whatever its bits; an infinity or

@@ -607,3 +607,34 @@ def test_attention_random(seed):
     c = Case(new, keys, H, Hkv, hd, r.choice(list(ref.FORMATS)), r.choice([16, 32, 64, 128, 256]),
              r.choice(list(ref.DTYPES)), seed=seed, garbage=math.nan)
     c.check(window=r.choice([0, 0, r.randint(1, 400)]))
+
+
+@pytest.mark.parametrize("top", [1, 40])
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("bf16", "bf16")])
+def test_more_sequences_than_are_kept_at_hand(top, cache, dtype):
+    """700 sequences: the schedule's table of sequences in shared memory holds 256."""
+    import random
+    r = random.Random(top)
+    new = [r.randint(0 if top > 1 else 1, top) for _ in range(700)]
+    keys = [n + r.choice([0, 3, r.randint(0, 300)]) for n in new]
+    Case(new, keys, 4, 2, 64, cache, 16, dtype, seed=23).check()
+
+
+@pytest.mark.parametrize("n", [6, 1100])
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("e4m3", "bf16")])
+def test_attention_non_finite_queries_stay_in_their_rows(n, cache, dtype):
+    c = Case([n], [n + 40], 2, 1, 64, cache, 16, dtype, seed=24)
+    clean = c.check()
+    q = c.q.clone()
+    q[n // 2, 70] = math.nan      # head 1 of one token
+    q[n // 3, 5] = math.inf       # head 0 of another
+    out = lai.paged_attention(q, c.kv, c.batch).view(n, 2, 64)
+    hit = torch.zeros((n, 2), dtype=torch.bool, device=DEV)
+    hit[n // 2, 1] = hit[n // 3, 0] = True
+    assert torch.isnan(out[hit]).all()
+    # The other rows keep the bounds of every row, not their bits: whether a block's weights come
+    # from the polynomial or the hardware's exponential is voted by the 32 rows of a warp (scores of
+    # 2^20 and more, and infinities, need the second), and either is within the bound of a row.
+    o, tol = (t.view(n, 2, 64)[~hit] for t in c.expected())
+    assert ((out[~hit].double() - o).abs() <= tol).all()
+    assert ((clean.view(n, 2, 64)[~hit].double() - o).abs() <= tol).all()

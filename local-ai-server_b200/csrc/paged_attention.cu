@@ -10,9 +10,9 @@
 // values in the operand layout of mma.m16n8k16, and every warp has its own keys, with no barrier
 // in the loop. One warp of a CTA only copies: it follows the page tables and keeps a ring of
 // chunks (a chunk is what a warp takes at a time) filled with bulk copies, across the ends of
-// items, so the other eight neither compute addresses nor hold loads in registers. (With loads
+// items, so the other seven neither compute addresses nor hold loads in registers. (With loads
 // straight into registers 64 x 4096 INT8 keys took 143 us, bound by their latency at the 12 warps
-// that fit; this takes KKK us.)
+// that fit; this takes 137 us.)
 //   * The sums over head_dim and over keys do not depend on the order of their terms. A lane
 //     takes 16-byte runs of K, and the query is loaded with the same permutation; a lane's n
 //     columns of V are a 16-byte run too, and the output is written back with that permutation.
@@ -248,6 +248,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     }
 
     const int n_heads = a.kv.n_kv * a.group;
+    const uint32_t zero = (uint32_t)a.kv.log_page >> 8;  // as only the host knows
     for (int n_it = 1; it.next(as); n_it++) {
         const Tile &tl = it.tl;
         const int head = it.kv_head(), blk0 = it.blk0, blk1 = it.blk1;
@@ -329,6 +330,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             const unsigned char *from = sm.ring[slot];
             const uint32_t there = sm.there[slot];
             if (there == 0) {  // none of its keys
+                __syncwarp();
                 if (lane == 0) bulk::mbar_arrive(&sm.empty[slot]);
                 continue;
             }
@@ -533,10 +535,12 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     }
                 }
             }
-            // (Not as soon as keys and values are in registers: with the release there, results were
-            // wrong now and then. Here the products have taken them.)
-            __syncwarp();
-            if (lane == 0) bulk::mbar_arrive(&sm.empty[slot]);
+            // The slot's next copy writes through the async proxy, which an arrival's release does not
+            // keep behind generic loads still in flight: with no more than __syncwarp between loads
+            // and arrival, 0.4% of calls with many short BF16 sequences were wrong. So the arrival
+            // waits for products of every load (all of the warp's: an MMA takes all lanes' operands).
+            const float after = VW == 8 ? o[0][0] + o[ND / 2][0] : o[0][0];
+            if (lane == 0) bulk::mbar_arrive(&sm.empty[slot] + (__float_as_uint(after) & zero));
         }
 
         // ---- join the warps: the upper half's sums into the lower half's, those in shared memory

@@ -638,3 +638,20 @@ def test_attention_non_finite_queries_stay_in_their_rows(n, cache, dtype):
     o, tol = (t.view(n, 2, 64)[~hit] for t in c.expected())
     assert ((out[~hit].double() - o).abs() <= tol).all()
     assert ((clean.view(n, 2, 64)[~hit].double() - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("cache,dtype", [("bf16", "f32"), ("bf16", "bf16"), ("i8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("S,new,H,Hkv", [(48, 1, 16, 8), (200, 1, 16, 8), (6, 90, 16, 8)])
+def test_attention_same_bits_in_every_call(S, new, H, Hkv, cache, dtype):
+    """Rings of copies and joined parts: 200 calls in a row give the first one's bits."""
+    import random
+    r = random.Random(S)
+    keys = [new + r.randint(0, 3000 if S < 100 else 700) for _ in range(S)]
+    c = Case([new] * S, keys, H, Hkv, 128, cache, 64 if S < 100 else 16, dtype, seed=S)
+    first = c.check()
+    scratch = lai.paged_attention_scratch(128)
+    outs = [torch.empty_like(first) for _ in range(50)]
+    for _ in range(4):
+        for o in outs:
+            lai.paged_attention(c.q, c.kv, c.batch, scratch=scratch, out=o)
+        assert all(torch.equal(o, first) for o in outs)

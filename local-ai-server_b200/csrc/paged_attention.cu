@@ -19,7 +19,8 @@
 //   * An MMA has 16 rows and a tile has 8: rows 8-15 carry the second term of the first 8. F32
 //     queries become hi + lo in binary16 (22 bits; the 8-bit formats are exact in binary16), or
 //     three bfloat16 terms (24 bits) over a BF16 cache, and so do the weights p. With BF16
-//     queries the second rows still make the weights exact to 16 bits or more.
+//     queries the second rows still make the weights exact to 16 bits or more. (One term of them
+//     over the 8-bit formats was no faster: the compiler spilt registers, 143 us for 126.)
 //   * Each block's P V starts from zero and is added to the F32 accumulators by the FMA that
 //     rescales them, so a long sequence does not add up the MMA's truncated sums.
 //   * 8-bit: a key's scale multiplies its score, a value's scale its weight. Weights in binary16
@@ -152,7 +153,6 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     constexpr int ND = HD / 8;                       // 8-column groups of the output
     constexpr int VW = HD * kBytes / 32;             // 32-bit words of V per lane and key
     constexpr float kLift = kF16 ? 13.f : 0.f;
-    constexpr bool kOne = kF16 && !QF32;             // one term of the weights will do
     static_assert(kChunks * kPerChunk == KS, "a lane's runs cover its share of head_dim");
 
     using Ck = Chunk<HD, FMT>;
@@ -435,11 +435,6 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     p1 *= vs[n].y * down;
                 }
                 uint32_t *pk = pa[n / 2] + (n & 1) * 2;
-                if (kOne) {
-                    pk[0] = pack2<kF16>(p0, p1);
-                    pk[1] = 0u;
-                    continue;
-                }
                 pk[0] = take2<kF16>(p0, p1);
                 if constexpr (kThird) {
                     pk[1] = take2<kF16>(p0, p1);
@@ -498,8 +493,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     if (kk == 0 && !kThird) mma<kF16, true>(c, pk[0], pk[1], pk[2], pk[3], b0[kk], b1[kk]);
                     else mma<kF16, false>(c, pk[0], pk[1], pk[2], pk[3], b0[kk], b1[kk]);
                 }
-                o[n][0] = fmaf(o[n][0], alpha, kOne ? c[0] : c[0] + c[2]);
-                o[n][1] = fmaf(o[n][1], alpha, kOne ? c[1] : c[1] + c[3]);
+                o[n][0] = fmaf(o[n][0], alpha, c[0] + c[2]);
+                o[n][1] = fmaf(o[n][1], alpha, c[1] + c[3]);
             };
 #pragma unroll
             for (int wd = 0; wd < VW; wd++) {
@@ -534,13 +529,16 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                         column(2 * wd + h, b0, b1);
                     }
                 }
+                if (wd == (VW == 8 ? 4 : 0)) {
+                    // The slot's next copy writes through the async proxy, which an arrival's release
+                    // does not keep behind generic loads still in flight: with no more than __syncwarp
+                    // between loads and arrival, 0.4% of calls with many short BF16 sequences were
+                    // wrong. So the arrival waits for products of every load (of all lanes: an MMA
+                    // takes the whole warp's operands).
+                    const float after = VW == 8 ? o[0][0] + o[ND / 2][0] : o[0][0];
+                    if (lane == 0) bulk::mbar_arrive(&sm.empty[slot] + (__float_as_uint(after) & zero));
+                }
             }
-            // The slot's next copy writes through the async proxy, which an arrival's release does not
-            // keep behind generic loads still in flight: with no more than __syncwarp between loads
-            // and arrival, 0.4% of calls with many short BF16 sequences were wrong. So the arrival
-            // waits for products of every load (all of the warp's: an MMA takes all lanes' operands).
-            const float after = VW == 8 ? o[0][0] + o[ND / 2][0] : o[0][0];
-            if (lane == 0) bulk::mbar_arrive(&sm.empty[slot] + (__float_as_uint(after) & zero));
         }
 
         // ---- join the warps: the upper half's sums into the lower half's, those in shared memory

@@ -584,44 +584,54 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                 }
         }
         math_sync();
-        // from here a thread owns 4 columns of a row at a time
-        float4 acc;
-        float sum, top;
+        // from here each of 128 threads owns kOwn columns of a row
+        constexpr int kOwn = kRows * HD / 128;
+        const int e = threadIdx.x * kOwn, r = e / HD, col = e % HD;
+        const bool owner = threadIdx.x < 128;
+        float acc[kOwn], sum, top;
         auto clear = [&]() {
-            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < kOwn; i++) acc[i] = 0.f;
             sum = 0.f;
-            top = neg_inf();
         };
         // adds the state (pm, pl, pv) of some keys; top is their common maximum by now
-        auto add = [&](float pm, float pl, const float4 &pv) {
+        auto add = [&](float pm, float pl, const float (&pv)[kOwn]) {
             const float f = ex2(pm - (top == neg_inf() ? 0.f : top));
             sum = fmaf(pl, f, sum);
-            acc.x = fmaf(pv.x, f, acc.x);
-            acc.y = fmaf(pv.y, f, acc.y);
-            acc.z = fmaf(pv.z, f, acc.z);
-            acc.w = fmaf(pv.w, f, acc.w);
+#pragma unroll
+            for (int i = 0; i < kOwn; i++) acc[i] = fmaf(pv[i], f, acc[i]);
         };
-        auto write = [&](int r, int col) {
+        auto write = [&]() {
             if (r >= tl.rows) return;
             const int fr = tl.row0 + r, tk = a.by_group.of(fr);
             const int64_t to = (((int64_t)tl.q_row0 + tk) * n_heads + head * a.group + (fr - tk * a.group)) * HD + col;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            if (QF32)
-                *reinterpret_cast<float4 *>(static_cast<float *>(out) + to) =
-                    make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            else
-                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + to) =
-                    make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+#pragma unroll
+            for (int i = 0; i < kOwn; i += 4)
+                if (QF32)
+                    *reinterpret_cast<float4 *>(static_cast<float *>(out) + to + i) =
+                        make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+                else
+                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + to + i) =
+                        make_uint2(pack_bf16x2(acc[i] * inv, acc[i + 1] * inv), pack_bf16x2(acc[i + 2] * inv, acc[i + 3] * inv));
+        };
+        auto take4 = [](float (&to)[kOwn], int i, const float4 &x) {
+            to[i] = x.x; to[i + 1] = x.y; to[i + 2] = x.z; to[i + 3] = x.w;
         };
         const bool alone = it.begins && it.ends;
         float *pp = a.parts + ((int64_t)blockIdx.x * 2 + (it.begins ? 1 : 0)) * part_floats(HD);
-        for (int e = threadIdx.x * 4; e < kRows * HD; e += kMath * 4) {
-            const int r = e / HD, col = e % HD;
+        if (owner) {
             clear();
+            top = neg_inf();
 #pragma unroll
             for (int x = 0; x < kHalf; x++) top = fmaxf(top, sm.m[x][r]);
 #pragma unroll
-            for (int x = 0; x < kHalf; x++) add(sm.m[x][r], sm.l[x][r], *reinterpret_cast<const float4 *>(&sm.o[x][r][col]));
+            for (int x = 0; x < kHalf; x++) {
+                float v[kOwn];
+#pragma unroll
+                for (int i = 0; i < kOwn; i += 4) take4(v, i, *reinterpret_cast<const float4 *>(&sm.o[x][r][col + i]));
+                add(sm.m[x][r], sm.l[x][r], v);
+            }
             if (FMT != LAI_KV_I8 && sm.bad == n_it && r < tl.rows) {
                 const int p = tl.pos0 + a.by_group.of(tl.row0 + r);
                 for (int j = max(blk0 * U, tl.k0); j < min(blk1 * U, tl.k1); j++) {
@@ -629,20 +639,15 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     const int page = __ldg(a.kv.pages + (int64_t)tl.seq * a.kv.max_pages + (j >> a.kv.log_page));
                     if (page < 0 || page >= a.kv.n_pages) continue;
                     const int64_t at = (a.kv.page_base(page, head) + (j & in_page)) * HD + col;
-                    float v[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        v[i] = element<FMT>(a.kv.v, at + i);
-                        v[i] = (__float_as_uint(v[i]) & 0x7f800000u) == 0x7f800000u ? v[i] : 0.f;
+                    for (int i = 0; i < kOwn; i++) {
+                        const float v = element<FMT>(a.kv.v, at + i);
+                        acc[i] += (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? v : 0.f;
                     }
-                    acc.x += v[0];
-                    acc.y += v[1];
-                    acc.z += v[2];
-                    acc.w += v[3];
                 }
             }
             if (alone) {
-                write(r, col);
+                write();
                 continue;
             }
             // parts: [row] max, [row] sum, [row][column]
@@ -650,7 +655,9 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                 pp[r] = top;
                 pp[kRows + r] = sum;
             }
-            *reinterpret_cast<float4 *>(pp + 2 * kRows + e) = acc;
+#pragma unroll
+            for (int i = 0; i < kOwn; i += 4)
+                *reinterpret_cast<float4 *>(pp + 2 * kRows + e + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
         }
         if (alone) continue;
         const int c0 = range.cta_of(it.item0), c1 = range.cta_of(it.item1 - 1);
@@ -664,39 +671,39 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         }
         math_sync();
         if (!sm.last) continue;
-        for (int e = threadIdx.x * 4; e < kRows * HD; e += kMath * 4) {
-            const int r = e / HD, col = e % HD;
-            clear();
-            constexpr int kAtOnce = 4;  // the parts in their order, so many of them under way
-            const float *from = a.parts + (int64_t)c0 * 2 * part_floats(HD);
+        if (!owner) continue;
+        // (More at once, or the parts dealt out to the warps, was not faster: a call's last CTA runs
+        // this code for the first time, and its length counts.)
+        constexpr int kAtOnce = 4;  // the parts in their order, so many of them under way
+        clear();
+        top = neg_inf();
 #pragma unroll 1
-            for (int first = c0; first <= c1; first += kAtOnce, from += kAtOnce * 2 * part_floats(HD)) {
-                float pm[kAtOnce], pl[kAtOnce];
-                float4 pv[kAtOnce];
+        for (int first = c0; first <= c1; first += kAtOnce) {
+            float pm[kAtOnce], pl[kAtOnce], pv[kAtOnce][kOwn];
 #pragma unroll
-                for (int c = 0; c < kAtOnce; c++) {
-                    pm[c] = neg_inf();
-                    pl[c] = 0.f;
-                    pv[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (first + c <= c1) {  // (the first part is its CTA's second)
-                        const float *pc = from + c * 2 * part_floats(HD) + (first + c == c0 ? part_floats(HD) : 0);
-                        pm[c] = __ldcg(pc + r);
-                        pl[c] = __ldcg(pc + kRows + r);
-                        pv[c] = __ldcg(reinterpret_cast<const float4 *>(pc + 2 * kRows + e));
-                    }
-                }
-                const float was = top, wl = sum;
-                const float4 wv = acc;
+            for (int c = 0; c < kAtOnce; c++) {
+                const int ci = min(first + c, c1);  // (the first part is its CTA's second)
+                const float *pc = a.parts + (ci * 2 + (ci == c0)) * part_floats(HD);
+                pm[c] = __ldcg(pc + r);
+                pl[c] = __ldcg(pc + kRows + r);
 #pragma unroll
-                for (int c = 0; c < kAtOnce; c++) top = fmaxf(top, pm[c]);
-                sum = 0.f;
-                acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                add(was, wl, wv);
-#pragma unroll
-                for (int c = 0; c < kAtOnce; c++) add(pm[c], pl[c], pv[c]);
+                for (int i = 0; i < kOwn; i += 4)
+                    take4(pv[c], i, __ldcg(reinterpret_cast<const float4 *>(pc + 2 * kRows + e + i)));
             }
-            write(r, col);
+#pragma unroll
+            for (int c = 1; c < kAtOnce; c++)
+                if (first + c > c1) pm[c] = neg_inf(), pl[c] = 0.f;  // the last one again: weight 0
+            const float was = top;
+#pragma unroll
+            for (int c = 0; c < kAtOnce; c++) top = fmaxf(top, pm[c]);
+            const float f = ex2(was - (top == neg_inf() ? 0.f : top));
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < kOwn; i++) acc[i] *= f;
+#pragma unroll
+            for (int c = 0; c < kAtOnce; c++) add(pm[c], pl[c], pv[c]);
         }
+        write();
     }
 }
 

@@ -352,7 +352,9 @@ typedef struct {
  * lai_paged_kv_read_*: the reverse, the values the cache stands for as rows (with kv_len as the
  * lengths of q_start's ranges: whole sequences). A row whose position is negative (more rows than
  * keys) is left alone and sets LAI_DEVERR_POSITION; a page outside [0, n_pages)
- * LAI_DEVERR_PAGE. Two rows of one append must not have the same page and place. */
+ * LAI_DEVERR_PAGE. ld >= n_kv_heads * head_dim; k, v and their rows 16-byte aligned, apart from the
+ * cache and, where written, from each other. Two rows of one append must not have the same page and
+ * place. */
 LAI_API int lai_paged_kv_append_bf16(const lai_paged_kv_t *kv, const lai_paged_batch_t *batch,
                                      const lai_bf16 *k, const lai_bf16 *v, int64_t ld,
                                      int64_t n_rows, int *err, lai_stream_t stream);
@@ -370,14 +372,17 @@ LAI_API int lai_paged_kv_read_f32(float *k, float *v, int64_t ld, int64_t n_rows
  * qwen_causal_attention(out, q, K, V, n, kv_len, n_heads, n_kv, hd, scale, kv_len - n) per
  * sequence (src/tts_native.c:576-578 a prompt, :653-655 one token). A token at position p sees
  * keys p - window + 1 .. p (window 0: 0 .. p); a row that sees none (its position is negative)
- * becomes 0. q [n_rows, n_heads * head_dim] with row stride ld_q elements, out dense and apart from
- * q; both 16-byte aligned rows; query head h
- * reads kv head h / (n_heads / n_kv_heads), a group of at most 16. Keys in a page outside
- * [0, n_pages) count as not seen and set LAI_DEVERR_PAGE. What lies in the cache behind kv_len,
- * or at positions a row does not see, does not reach that row, whatever its bits; an infinity or
- * NaN that it does see makes what it touches an infinity or NaN. Scores, softmax
- * and sums are F32; with F32 q the products are exact to about F32 too (16-bit operands split
- * into terms), with BF16 q and a BF16 cache the weights of the values may be rounded to BF16.
+ * becomes 0. q [n_rows, n_heads * head_dim] with row stride ld_q elements, out dense, rows of both
+ * 16-byte aligned; out and scratch overlap neither each other nor q or the cache. Query head h
+ * reads kv head h / (n_heads / n_kv_heads), a group of at most 16. n_rows * group + n_seqs
+ * reaches 2^28, or the batch could have 2^31 blocks of keys and rows: LAI_ERR_RANGE. Keys in a page
+ * outside [0, n_pages) count as not seen and set LAI_DEVERR_PAGE. What lies in the cache behind
+ * kv_len, or at positions a row does not see, does not reach that row, whatever its bits; an
+ * infinity or NaN that it does see makes what it touches an infinity or NaN. Scores, softmax and
+ * sums are F32; with F32 q the products are exact to about F32 too (16-bit operands split into
+ * terms), with BF16 q the weights of the values may be rounded to BF16 (BF16 cache) or to
+ * binary16. The result has the same bits in every call with the same batch, but a row's bits
+ * depend on the rows it shares a batch with.
  * scratch: lai_paged_attention_scratch_bytes(head_dim) bytes, zeroed once before first use; every
  * call leaves it reusable, but two calls that may run at the same time (other streams, graphs on
  * other streams) need one each. */

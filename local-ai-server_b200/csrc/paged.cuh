@@ -53,7 +53,8 @@ __device__ __forceinline__ void flag(int *err, int bit) {
 // kernels). LAI_OK, or the error the entry returns.
 inline int check(const lai_paged_kv_t *kv, const lai_paged_batch_t *b, int64_t n_rows, View *out) {
     if (!kv || !b || !kv->k || !kv->v || n_rows < 0 || b->n_seqs < 0 ||
-        (b->n_seqs > 0 && (!b->q_start || !b->kv_len || !b->pages)) || b->max_pages <= 0 || kv->n_pages <= 0 || kv->n_kv_heads <= 0 ||
+        (b->n_seqs > 0 && (!b->q_start || !b->kv_len || !b->pages)) || b->max_pages <= 0 ||
+        kv->n_pages <= 0 || kv->n_kv_heads <= 0 ||
         (kv->head_dim != 64 && kv->head_dim != 128) || kv->format < LAI_KV_BF16 ||
         kv->format > LAI_KV_I8)
         return LAI_ERR_INVALID;

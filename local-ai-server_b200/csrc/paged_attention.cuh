@@ -98,8 +98,9 @@ struct Sched {
         Tile t = {};
         const Seq q = load_seq(a.kv, s);
         const int i = slot - base(a, s);
-        const int r0 = i * R, all = q.n * a.group;  // below 2^28 where ok
-        if (!q.ok || i < 0 || r0 >= all) return t;
+        const int all = q.n * a.group;  // below 2^28 where ok
+        if (!q.ok || all == 0 || i < 0 || i > (all - 1) / R) return t;
+        const int r0 = i * R;
         t.seq = s;
         t.row0 = r0;
         t.q_row0 = q.row0;

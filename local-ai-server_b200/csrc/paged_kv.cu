@@ -9,7 +9,9 @@
 // HBM bound: every row is read once and every cache row written once (and the other way round).
 // A group of head_dim / 8 lanes owns one (row, head) of k and of v, 8 elements per lane, so the
 // maximum is a shuffle within the group, and each global access is a whole 128- to 512-byte run.
-// What costs time beside the bytes:
+// Measured: reading 24 sequences of 4096 E4M3 tokens, 8 heads of 128, as BF16 rows 70 us (6.0 TB/s,
+// 0.93 of a copy's bandwidth); writing 40 chunks of 257 BF16 rows, 16 heads of 64, 13.8 us (4.3 TB/s:
+// half of it is starting and ending). What costs time beside the bytes:
 //   * The look-up of a row's place is a chain of loads (q_start, lengths, page). A CTA covers
 //     consecutive (row, head) pairs, several per thread; a thread per row follows the chain and
 //     leaves the place in shared memory, while an append's first rows are on their way. The

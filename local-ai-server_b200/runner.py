@@ -1189,7 +1189,8 @@ class TtsFrame:
         """Library kernels per frame (the 2 tensor copies and the position add not counted)."""
         c = self.cfg
         per_layer = 5
-        return (c.layers * (per_layer if self.batch is None else per_layer + 2) + 2 + 3 + c.groups * c.cp_layers * per_layer + 1
+        talker_layer = per_layer if self.batch is None else per_layer + 2
+        return (c.layers * talker_layer + 2 + 3 + c.groups * c.cp_layers * per_layer + 1
                 + (c.groups - 1) * 4 + 1)
 
     def weight_bytes_per_frame(self) -> int:

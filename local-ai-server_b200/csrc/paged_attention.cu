@@ -15,8 +15,11 @@
 // that fit; this takes 137 us.)
 //   Measured, 64 sequences of 4096 keys, 16 heads of 128 on 8, one token each: BF16 keys 176 us with
 // F32 q (6.1 TB/s, 0.94 of a copy's bandwidth) and 169 with BF16 q (6.4 TB/s, 0.99), so HBM; E4M3
-// 126 and INT8 137 us (4.4 and 4.0 TB/s): instructions, about 1000 per 32 keys of a warp, a third of
-// them the conversions to binary16; copying alone takes 101 us. Short calls are latency: one sequence
+// 126 and INT8 137 us (4.4 and 4.0 TB/s): the warps' latency over about 1000 instructions per 32 keys
+// (a third of them conversions to binary16; issue slots 44% used at the 14 warps that registers
+// allow), and the count of copies: 4 per chunk, 101 us on their own. V in 4 blocks apart, so that no
+// banks conflict, took 7 copies and 165 us, in 2 blocks 145; scales by 16-byte copies of the lanes
+// 145. Short calls are latency: one sequence
 // of 777 keys 10.6 us, of which finding the work 2.5, the first keys through a warp 4.7, leaving
 // parts 1.6, joining them 1.7.
 //   * The sums over head_dim and over keys do not depend on the order of their terms. A lane

@@ -25,8 +25,8 @@
 // diagonal): BF16 q, BF16 cache 465 us (1.14 PFLOP/s, 0.68 of a large BF16 matrix product's rate),
 // 8-bit 590 us; F32 q 1495 us (BF16 cache) and 1190 us (8-bit), for three and two times the products
 // of each kind. With BF16 q softmax and MMAs bound it together: a tile's block is 16384 exponentials,
-// 1024 clocks at 16 per SM and clock, and its MMAs take as many; 8-bit adds the finishers'
-// conversions, which share the softmax's issue slots.
+// 1024 clocks at 16 per SM and clock, and its MMAs take as many; 8-bit caches have room for 3 operand
+// tiles only, so conversions are not far enough ahead of the MMAs (BF16 with 3 tiles: 525 us).
 // Every wait is bounded; a wait that runs out raises LAI_DEVERR_TIMEOUT and ends the kernel.
 #include <cuda.h>
 
@@ -55,6 +55,8 @@ struct Cfg {
     static constexpr int MT = QF32 ? 1 : 2;
     static constexpr int R = 128 * MT;
     static constexpr int kTile = 128 * HD * 2;         // bytes of an operand tile
+    // What fits beside the queries. BF16 q over 2048 x 32768 keys: BF16 keys 525, 463, 464 us with 3, 4
+    // and 5 tiles; INT8 keys 582 and 608 us with 3 tiles and 3 or 2 in the staging ring, 857 with 4 and 1.
     static constexpr int kStages = kF16 || QF32 ? 3 : 5;
     static constexpr int kRaw = kF16 ? 3 : 0;          // 8-bit tiles in the staging ring
     static constexpr int kRawTile = 128 * HD;

@@ -655,3 +655,48 @@ def test_attention_same_bits_in_every_call(S, new, H, Hkv, cache, dtype):
         for o in outs:
             lai.paged_attention(c.q, c.kv, c.batch, scratch=scratch, out=o)
         assert all(torch.equal(o, first) for o in outs)
+
+
+@pytest.mark.parametrize("n", [1, 150])
+@pytest.mark.parametrize("cache,dtype", [("bf16", "bf16"), ("i8", "f32"), ("e4m3", "bf16"), ("bf16", "f32")])
+def test_attention_over_shared_pages(n, cache, dtype):
+    """A common prefix held once for three sequences, and a page that one table names twice."""
+    c = Case([n] * 3, [n + 260] * 3, 16, 8, 128, cache, 32, dtype, seed=25)
+    c.pages[1:, :8] = c.pages[0, :8]
+    c.pages[2, 5] = c.pages[2, 4]
+    c.batch = lai.PagedBatch(c.batch.q_start, c.batch.kv_len, c.pages.to(DEV))
+    c.check()
+
+
+@pytest.mark.parametrize("cache", list(ref.FORMATS))
+def test_append_attend_and_read_on_one_stream_many_steps(cache):
+    """A decode loop without a synchronisation: every step sees the keys that the ones before wrote."""
+    S, H, Hkv, hd, page, steps = 5, 8, 4, 64, 16, 40
+    g = gen(26)
+    pages, pool = ref.make_pages([steps + 7 * s for s in range(S)], page, seed=26)
+    kv = lai.PagedKV.allocate(pool, Hkv, page, hd, ref.FORMATS[cache])
+    kv_len = i32([7 * s for s in range(S)])
+    batch = lai.PagedBatch(starts([1] * S), kv_len, pages.to(DEV))
+    # the keys that are there already
+    old = [7 * s for s in range(S)]
+    x = torch.randn((2, sum(old), Hkv * hd), generator=g, device=DEV)
+    lai.paged_kv_append(kv, lai.PagedBatch(starts(old), i32(old), pages.to(DEV)), x[0], x[1])
+    rows = torch.randn((steps, S, (H + 2 * Hkv) * hd), generator=g, device=DEV)
+    scratch = lai.paged_attention_scratch(hd)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    outs = []
+    for t in range(steps):
+        kv_len.add_(1)
+        q, k, v = rows[t].split([H * hd, Hkv * hd, Hkv * hd], dim=1)
+        lai.paged_kv_append(kv, batch, k, v, err=err)
+        outs.append(lai.paged_attention(q, kv, batch, scratch=scratch, err=err))
+    assert int(err) == 0
+    kd, vd = ref.values(kv.k, kv.k_scale), ref.values(kv.v, kv.v_scale)
+    for s in range(S):
+        keys = ref.sequence(kd, pages[s], old[s] + steps), ref.sequence(vd, pages[s], old[s] + steps)
+        for t in (0, 1, 17, steps - 1):
+            n = old[s] + t + 1
+            q = rows[t, s, :H * hd].double().view(1, H, hd)
+            o, a, b, u = ref.attend(q, keys[0][:n], keys[1][:n], n - 1, hd ** -0.5, 0)
+            tol = ref.tolerance(o, a, b, u, torch.float32, ref.FORMATS[cache]).flatten()
+            assert ((outs[t][s].double() - o.flatten()).abs() <= tol).all()

@@ -474,7 +474,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             // What is not there may be anything, and weight 0 times it has to be 0. And a step whose
             // keys some rows of the tile see and others do not gives every row 0 x v for the keys it
             // must not see: infinities and NaN are taken out of such a step, and added to the rows
-            // that see them at the end.
+            // that see them at the end. (Of a part step whose rows all see the same keys nothing is
+            // taken: what is there is seen.)
             if (!all) {
 #pragma unroll
                 for (int kk = 0; kk < NK; kk++)
@@ -486,7 +487,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                         for (int w = 0; w < VW; w++) {
                             uint32_t &x = vr[kk][i][w];
                             x = ok ? x : 0u;
-                            if (FMT != LAI_KV_I8) bad |= drop_nonfinite<FMT>(x);
+                            if (FMT != LAI_KV_I8 && uneven) bad |= drop_nonfinite<FMT>(x);
                         }
                     }
             }

@@ -1,0 +1,63 @@
+"""The paged cache's attention where single numbers decide: infinities and NaN in places that are
+seen or not, scores so large that their last place passes 1, values and queries at the ends of F32."""
+import math
+
+import pytest
+
+import lai
+import paged_ref as ref
+from test_gpu_paged import DEV, Case, gen, i32
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+# ---- a value that is seen is not lost -----------------------------------------------------------
+def poke(c, j, head, col, bad):
+    """V of sequence 0's key j, as the cache holds it: a NaN's code in E4M3."""
+    page = c.kv.v.shape[2]
+    at = int(c.pages[0, j // page]), head, j % page, col
+    if c.cache == torch.bfloat16:
+        c.kv.v[at] = bad
+    else:
+        c.kv.v.view(torch.uint8)[at] = 0x7F
+
+
+# one token or several; the part step at the end (its own value among it), whole steps, the first keys
+# of a window and the one before it; and the kernel for many rows
+SEEN = [(1, 37, 0, (5, 32, 36)), (1, 37, 20, (16, 17, 31, 36)), (1, 777, 0, (700, 768, 776)), (1, 130, 100, (29, 30, 128)),
+        (3, 40, 0, (36, 37, 39)), (3, 100, 33, (64, 65, 70, 99)), (700, 800, 0, (99, 101, 500, 799)), (700, 837, 60, (70, 140, 836))]
+
+
+@pytest.mark.parametrize("cache,bad", [("bf16", math.nan), ("bf16", math.inf), ("bf16", -math.inf), ("e4m3", math.nan)])
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+@pytest.mark.parametrize("n,L,window,at", SEEN)
+def test_a_value_that_is_seen_is_not_lost(n, L, window, at, cache, dtype, bad):
+    for j in at:
+        c = Case([n], [L], 4, 2, 128, cache, 16, dtype, seed=31)
+        poke(c, j, 1, 77, bad)
+        out = lai.paged_attention(c.q, c.kv, c.batch, window=window)
+        pos = torch.arange(L - n, L, device=DEV)
+        sees = (pos >= j) & (pos < j + (window or L))
+        hit = torch.zeros((n, 4, 128), dtype=torch.bool, device=DEV)
+        hit[sees, 2:, 77] = True
+        hit = hit.view(n, -1)
+        assert not torch.isfinite(out[hit]).any(), j
+        o, tol = c.expected(window=window)  # (it leaves non-finite values out)
+        assert ((out.double() - o).abs() <= tol)[~hit].all(), j
+
+
+@pytest.mark.parametrize("n", [1, 3, 900])
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+def test_a_value_that_is_seen_beside_a_missing_page_is_not_lost(n, dtype):
+    L = n + 63
+    c = Case([n], [L], 4, 2, 128, "e4m3", 16, dtype, seed=32)
+    poke(c, 20, 1, 77, math.nan)
+    pages = c.batch.pages.clone()
+    pages[0, 0] = -1
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = lai.paged_attention(c.q, c.kv, lai.PagedBatch(c.batch.q_start, c.batch.kv_len, pages), err=err).view(n, 4, 128)
+    assert int(err) == lai.LAI_DEVERR_PAGE
+    assert torch.isnan(out[:, 2:, 77]).all()
+    out[:, 2:, 77] = 0
+    assert torch.isfinite(out).all()

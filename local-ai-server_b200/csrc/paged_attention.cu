@@ -318,6 +318,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             math_sync();
         }
 
+        // weights are 2^(score - m), m = maximum - kLift; l and o are sums of these
         float m = neg_inf(), l = 0.f, o[ND][2];
 #pragma unroll
         for (int n = 0; n < ND; n++) o[n][0] = o[n][1] = 0.f;
@@ -420,9 +421,11 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float mn = fmaxf(m, top);
-            const float mu = (mn == neg_inf() ? 0.f : mn) - kLift;
-            float alpha = ex2(m - (mu + kLift));  // m = -inf: nothing to keep
+            // (rounded up, so that weights do not pass 2^kLift; what is kept is what they are relative
+            // to, so that a maximum that did not move gives alpha = 1 whatever its last place)
+            const float mn = fmaxf(m, kF16 ? __fsub_ru(top, kLift) : top);
+            const float mu = mn == neg_inf() ? 0.f : mn;
+            float alpha = ex2(m - mu);  // m = -inf: nothing to keep
             m = mn;
             l *= alpha;
             float down = 1.f;

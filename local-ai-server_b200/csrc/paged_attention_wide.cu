@@ -720,8 +720,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 bulk::fence_proxy_async_smem();
                 bulk::mbar_arrive(&ctl.q_full[mt]);
             }
-            // Weights are 2^(score - off + kLift), off = maximum + exponent of the value scales;
-            // l and O are sums of these.
+            // Weights are 2^(score - off), off = maximum + exponent of the value scales - kLift, rounded
+            // up where scores are so large that it is not exact; l and O are sums of these.
             float m = neg_inf(), off = neg_inf(), l = 0.f, alpha = 0.f;
             int ve = kF16 ? -90 : 0;
             bool bad = false;
@@ -834,8 +834,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     // an infinite or NaN score: no weight of this row means anything any more
                     if (!(top < __int_as_float(0x7f800000))) l = __int_as_float(0x7fffffff);
                     m = fmaxf(m, top == neg_inf() ? top : top * c);
-                    const float to = m + (float)ve;
-                    if (!(to > off + slack)) return 1.f;
+                    const float to = kF16 ? __fsub_ru(__fadd_ru(m, (float)ve), C::kLift) : m;
+                    if (!(to - off > slack)) return 1.f;  // (their sum may be rounded past 2^8)
                     const float f = ex2(off - to);  // off = -inf: 0
                     off = to;
                     l *= f;
@@ -866,7 +866,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                             tmem_st_x16(t_pv + 16 * g, y);
                         }
                     }
-                    const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
+                    const float base = off == neg_inf() ? 0.f : off;
                     auto weigh_all = [&](auto mask) {
 #pragma unroll
                         for (int g = 0; g < 4; g++) weigh(g, x + 16 * g, base, mask);
@@ -891,7 +891,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         add_pv();
                     }
                     alpha = move(top, 0.f);
-                    const float base = (off == neg_inf() ? 0.f : off) - C::kLift;
+                    const float base = off == neg_inf() ? 0.f : off;
                     auto weigh_half = [&](auto mask) {
 #pragma unroll
                         for (int g = 0; g < 2; g++) weigh(2 * half + g, x + 16 * g, base, mask);

@@ -61,3 +61,25 @@ def test_a_value_that_is_seen_beside_a_missing_page_is_not_lost(n, dtype):
     assert torch.isnan(out[:, 2:, 77]).all()
     out[:, 2:, 77] = 0
     assert torch.isfinite(out).all()
+
+
+# ---- scores whose last place is 2, 4, 8 .. -----------------------------------------------------
+@pytest.mark.parametrize("n,L", [(1, 20000), (1100, 3000)])
+@pytest.mark.parametrize("cache", list(ref.FORMATS))
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+def test_equal_scores_of_any_magnitude_weigh_the_same(n, L, cache, dtype):
+    """Every key is the same, so a row is the mean of what it sees. Tolerance: half a step of a BF16
+    weight (2^-8; the means of |v| below 1, the result's own rounding as much again), and 2e-5 with
+    F32, as for other rows of equal scores."""
+    c = Case([n], [L], 2, 1, 64, cache, 64, dtype, seed=33)
+    v = ref.sequence(ref.values(c.kv.v, c.kv.v_scale), c.pages[0], L)[:, 0]
+    want = v.cumsum(0)[L - n:] / torch.arange(L - n + 1, L + 1, device=DEV)[:, None]
+    tol = 2e-5 if dtype == "f32" else 2.0 ** -6
+    for e in (9.3, 11.1, 13.7, 15.2, 20.2, 22.9, 23.9, 24.1, 24.5, 24.9, 25.3, 25.7, 26.2, 26.6, 27.1, 27.8, 28.4, 29.5, 33.0):
+        for sign in (1, -1):
+            k, q = torch.zeros_like(c.k_rows), torch.zeros_like(c.q)
+            k[:, 0] = sign * 2.0 ** (e / 2)
+            q[:, 0] = q[:, 64] = 2.0 ** (e / 2)
+            lai.paged_kv_append(c.kv, c.whole, k, c.v_rows)
+            out = lai.paged_attention(q, c.kv, c.batch, scale=1.0).double().view(n, 2, 64)
+            assert (out - want[:, None]).abs().max() <= tol, (e, sign)

@@ -32,9 +32,10 @@
 //     over the 8-bit formats was no faster: the compiler spilt registers, 143 us for 126.)
 //   * Each block's P V starts from zero and is added to the F32 accumulators by the FMA that
 //     rescales them, so a long sequence does not add up the MMA's truncated sums.
-//   * 8-bit: a key's scale multiplies its score, a value's scale its weight. Weights in binary16
-//     are taken relative to the largest value scale so far (a power of two per warp) and lifted
-//     by 2^13, so that small ones keep their bits.
+//   * 8-bit: a key's scale multiplies its score, a value's scale its weight. In binary16 these
+//     products are held relative to the row's own largest so far (which 2^-ve brings to 2^13 .. 2^14),
+//     so neither a value that another row sees nor a large one under a small weight costs a row
+//     bits: what is below 2^-38 of its largest product is rounded.
 #include "bulk_copy.cuh"
 #include "paged_attention.cuh"
 
@@ -161,7 +162,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
     constexpr int KS = HD / 16;                      // k16 steps of a score
     constexpr int ND = HD / 8;                       // 8-column groups of the output
     constexpr int VW = HD * kBytes / 32;             // 32-bit words of V per lane and key
-    constexpr float kLift = kF16 ? 13.f : 0.f;
+    constexpr int kLift = 13;                        // log2 of an 8-bit cache's largest products
     static_assert(kChunks * kPerChunk == KS, "a lane's runs cover its share of head_dim");
 
     using Ck = Chunk<HD, FMT>;
@@ -318,11 +319,11 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             math_sync();
         }
 
-        // weights are 2^(score - m), m = maximum - kLift; l and o are sums of these
-        float m = neg_inf(), l = 0.f, o[ND][2];
+        // weights are 2^(score - m), m the maximum; l is their sum, o 2^-ve times the sum of their
+        // products with the values
+        float m = neg_inf(), l = 0.f, ve = 0.f, o[ND][2];
 #pragma unroll
         for (int n = 0; n < ND; n++) o[n][0] = o[n][1] = 0.f;
-        int vexp = -126;  // accumulators are in units of 2^vexp (8-bit)
         bool bad = false;
 
         for (int blk = blk0; blk < blk1; blk++, chunk0 += kWarps) {
@@ -393,7 +394,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             }
             const bool uneven = mixed(tl, a.window, j0, kStep);
             const bool all = whole && !uneven;  // every row sees every key
-            float top = neg_inf(), vtop = 0.f;
+            float top = neg_inf();
 #pragma unroll
             for (int n = 0; n < NB; n++) {
                 const float k0 = kF16 ? row_scale * ks[n].x : row_scale, k1 = kF16 ? row_scale * ks[n].y : row_scale;
@@ -415,37 +416,42 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     }
             }
 #pragma unroll
-            for (int n = 0; n < NB; n++) {
-                top = fmaxf(top, fmaxf(sc[n][0], sc[n][1]));
-                if (kF16) vtop = fmaxf(vtop, fmaxf(vs[n].x, vs[n].y));
-            }
+            for (int n = 0; n < NB; n++) top = fmaxf(top, fmaxf(sc[n][0], sc[n][1]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // (rounded up, so that weights do not pass 2^kLift; what is kept is what they are relative
-            // to, so that a maximum that did not move gives alpha = 1 whatever its last place)
-            const float mn = fmaxf(m, kF16 ? __fsub_ru(top, kLift) : top);
+            const float mn = fmaxf(m, top);
             const float mu = mn == neg_inf() ? 0.f : mn;
-            float alpha = ex2(m - mu);  // m = -inf: nothing to keep
+            const float grown = m - mu;  // m = -inf: nothing to keep
+            float alpha = ex2(grown);    // 1 where the maximum did not move, whatever its last place
             m = mn;
-            l *= alpha;
-            float down = 1.f;
-            if (kF16) {  // a row's lanes have all of the step's value scales; the warp takes one power
-                const uint32_t u = __reduce_max_sync(0xffffffffu, __float_as_uint(vtop));
-                const int e = max(vexp, min((int)(u >> 23) - 127, 126));
-                alpha *= pow2i(vexp - e);
-                down = pow2i(-e);
-                vexp = e;
-            }
             // ---- weights
+            float lsum = 0.f, ptop = 0.f, down = 1.f;
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                sc[n][0] = ex2(sc[n][0] - mu);
+                sc[n][1] = ex2(sc[n][1] - mu);
+                lsum += sc[n][0] + sc[n][1];
+                if (kF16) {  // a masked value's scale is 0 by now
+                    sc[n][0] *= vs[n].x;
+                    sc[n][1] *= vs[n].y;
+                    ptop = fmaxf(ptop, fmaxf(fabsf(sc[n][0]), fabsf(sc[n][1])));
+                }
+            }
+            l = fmaf(l, alpha, lsum);
+            if (kF16) {
+                ptop = fmaxf(ptop, __shfl_xor_sync(0xffffffffu, ptop, 1));
+                ptop = fmaxf(ptop, __shfl_xor_sync(0xffffffffu, ptop, 2));
+                // the step's largest product, and that of what is kept, which falls as the maximum grows
+                const int e = min(max((int)(__float_as_uint(ptop) >> 23) - 127 - kLift, -126), 114);
+                const float now = fmaxf(ve + grown, (float)e);
+                alpha = ex2(grown + (ve - now));
+                down = ex2(-now);
+                ve = now;
+            }
             uint32_t pa[NK][kThird ? 6 : 4];
 #pragma unroll
             for (int n = 0; n < NB; n++) {
-                float p0 = ex2(sc[n][0] - mu), p1 = ex2(sc[n][1] - mu);
-                l += p0 + p1;
-                if (kF16) {  // a masked value's scale is 0 by now
-                    p0 *= vs[n].x * down;
-                    p1 *= vs[n].y * down;
-                }
+                float p0 = sc[n][0] * down, p1 = sc[n][1] * down;
                 uint32_t *pk = pa[n / 2] + (n & 1) * 2;
                 pk[0] = take2<kF16>(p0, p1);
                 if constexpr (kThird) {
@@ -564,7 +570,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             const int gg = 2 * t + i, n = 4 * k;
             return VW == 2 ? gg * 8 + n : kF16 ? gg * 16 + n : (gg + 8 * (n / 8)) * 8 + n % 8;
         };
-        const float unit = kF16 ? pow2i(vexp) : 1.f;
+        const float unit = kF16 ? ex2(ve) : 1.f;
         const int half = warp % kHalf;
         if (warp >= kHalf) {
             if (t == 0) sm.m[half][g] = m, sm.l[half][g] = l;

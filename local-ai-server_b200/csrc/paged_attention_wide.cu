@@ -20,7 +20,10 @@
 //     added to the output row, which the threads keep in registers, so long sequences do not add
 //     up the MMA's truncated sums.
 //   * 8-bit: key scales multiply S, value scales P; both come with the block in shared memory.
-//     Weights are relative to the largest value scale too, so that they fit binary16.
+//     Weights are relative to the row's largest product of a weight and a value's scale, so that they
+//     fit binary16 and neither a value that the row does not see nor a large one under a small weight
+//     costs it bits. Where a block's scales lie within 2^kSpread the largest stands for all of them;
+//     elsewhere every key's own counts.
 // Measured, 2048 tokens over 32768 keys, 16 heads of 128 on 8 (0.53 TFLOP of products below the
 // diagonal): BF16 q, BF16 cache 465 us (1.14 PFLOP/s, 0.68 of a large BF16 matrix product's rate),
 // 8-bit 590 us; F32 q 1495 us (BF16 cache) and 1190 us (8-bit), for three and two times the products
@@ -47,6 +50,10 @@ constexpr int kGroup = 16;     // keys per copy
 constexpr int kRing = 4;       // blocks whose scales and flags are kept
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kGrow = 8.f;   // log2 of how far weights may pass 1 before O is rescaled
+constexpr int kSpread = 12;    // log2 of how far a block's value scales lie apart at most, to go by the largest
+// log2 of the value scales that sums of weights have room for: weights reach from 2^kLift over the
+// scale, with 2^-24 of it still a normal F32, to 2^20 times 2^14 over it
+constexpr int kLowScale = -90, kTopScale = 106;
 
 template <int HD, int FMT, bool QF32>
 struct Cfg {
@@ -91,7 +98,7 @@ struct Ctl {
     uint64_t info[kRing], item_full[kItems], item_empty[kItems];
     Item items[kItems];
     uint64_t q_full[2], s_full[2], p_full[2][2], pv_full[2], group[2];
-    int vexp[kRing][4];
+    uint32_t vspan[kRing][4];  // of 32 keys' value scales the largest exponent, and 255 less the smallest
     int groups[kRing];  // bit i: 16-key group i of the block lies in a real page
     int vbad[kRing];    // the block (counted) from whose V infinities or NaN were taken out
     SeqSmem seqs;
@@ -444,7 +451,8 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                                 if (mixed && !fine) ctl.vbad[slot] = (int)blocks;
                             }
                             const uint32_t top = __reduce_max_sync(0xffffffffu, fine ? u : 0u);
-                            if (lane == 0) ctl.vexp[slot][wt >> 5] = (int)(top >> 23) - 127;
+                            const uint32_t low = __reduce_min_sync(0xffffffffu, fine && u ? u : 0x7f800000u);
+                            if (lane == 0) ctl.vspan[slot][wt >> 5] = (top >> 23) << 16 | (255u - (low >> 23));
                         }
                         if (wt == 0) ctl.groups[slot] = (int)groups;
                         __syncwarp();
@@ -720,10 +728,9 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 bulk::fence_proxy_async_smem();
                 bulk::mbar_arrive(&ctl.q_full[mt]);
             }
-            // Weights are 2^(score - off), off = maximum + exponent of the value scales - kLift, rounded
-            // up where scores are so large that it is not exact; l and O are sums of these.
-            float m = neg_inf(), off = neg_inf(), l = 0.f, alpha = 0.f;
-            int ve = kF16 ? -90 : 0;
+            // Weights are 2^(score - off); l and O are sums of these. off is the largest score, or, of an 8-bit
+            // cache, the largest score plus exponent of the value's scale, less kLift.
+            float off = neg_inf(), l = 0.f, alpha = 0.f;
             bool bad = false;
             constexpr int kKeep = kSplit ? kCols : 1;
             float o[kKeep];
@@ -764,10 +771,35 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 };
                 const float4 *k4 = reinterpret_cast<const float4 *>(ctl.kscale[slot]);
                 const float4 *v4 = reinterpret_cast<const float4 *>(ctl.vscale[slot]);
+                bool each = false;  // the scales lie apart (the same for all warps)
+                float ve = 0.f;
                 if (kF16) {
-                    const int *e4 = ctl.vexp[slot];
-                    ve = min(max(max(max(e4[0], e4[1]), max(e4[2], e4[3])), ve), 90);
+                    const uint32_t *s4 = ctl.vspan[slot];
+                    const uint32_t span = __vmaxu2(__vmaxu2(s4[0], s4[1]), __vmaxu2(s4[2], s4[3]));
+                    const int e = (int)(span >> 16);
+                    each = e + (int)(span & 255u) > 255 + kSpread;
+                    ve = (float)min(max(e - 127, kLowScale), kTopScale);
                 }
+                // the largest score (below top) plus exponent of the value's scale, of the keys from j1 to j2;
+                // rarely called, so short: S is read again
+                auto exponents = [&](int j1, int j2, float top) {
+                    float most = neg_inf();
+#pragma unroll 1
+                    for (int j = j1; j < j2; j += 16) {
+                        uint32_t y[16];
+                        umma::tmem_ld_32x32b_x16(t_s + j, y);
+                        umma::tmem_wait_ld();
+                        const uint32_t see = seen(j >> 5) >> (j & 16);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int u = __float_as_int(ctl.vscale[slot][kF16 ? j + i : 0]);
+                            const float x = __uint_as_float(y[i]) * ctl.kscale[slot][kF16 ? j + i : 0];
+                            const float e = (float)min(max((u >> 23 & 255) - 127, kLowScale), kTopScale);
+                            most = fmaxf(most, see >> i & 1 ? __fmul_rn(x, c) - top + e : neg_inf());
+                        }
+                    }
+                    return most;
+                };
                 // 32 scores with their keys' scales, masked; the maximum so far
                 auto scale32 = [&](int g, float2 *x, float &top, auto mask) {
                     const uint32_t see = decltype(mask)::value ? seen(g) : 0u;
@@ -828,16 +860,18 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                 auto fetch = [&](int g, float2 *x) {  // without waiting
                     umma::tmem_ld_32x32b_x32(t_s + 32 * g, *reinterpret_cast<uint32_t (*)[32]>(x));
                 };
-                auto is_big = [&](float top) { return __any_sync(0xffffffffu, fabsf(top * c) > 1048576.f); };
+                auto is_big = [&](float top) { return __any_sync(0xffffffffu, fabsf(top) > 1048576.f); };
                 // moves off to the block's maximum; what l and O must be multiplied with
-                auto move = [&](float top, float slack) -> float {
+                auto move = [&](float top, float e, float slack) -> float {
                     // an infinite or NaN score: no weight of this row means anything any more
                     if (!(top < __int_as_float(0x7f800000))) l = __int_as_float(0x7fffffff);
-                    m = fmaxf(m, top == neg_inf() ? top : top * c);
-                    const float to = kF16 ? __fsub_ru(__fadd_ru(m, (float)ve), C::kLift) : m;
-                    if (!(to - off > slack)) return 1.f;  // (their sum may be rounded past 2^8)
-                    const float f = ex2(off - to);  // off = -inf: 0
+                    // rounded up where scores are large, so that weights stay below 2^15; from 2^28 on
+                    // their last place passes 2^kLift
+                    const float to = kF16 && fabsf(top) < 268435456.f ? __fadd_ru(top, e - C::kLift) : top;
+                    const float d = to - off;
+                    if (!(d > slack)) return 1.f;  // (no key yet and none now: NaN)
                     off = to;
+                    const float f = ex2(-d);  // off = -inf: 0
                     l *= f;
                     return f;
                 };
@@ -852,8 +886,10 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                         for (int g = 0; g < 4; g++) scale32(g, x + 16 * g, part[g], mask);
                     };
                     if (masked) scale_all(Yes{}); else scale_all(No{});
-                    const float top = max3(max3(part[0], part[1], part[2]), part[3], part[3]);
-                    const float f = move(top, kGrow);
+                    float top = max3(max3(part[0], part[1], part[2]), part[3], part[3]);
+                    if (top != neg_inf()) top *= c;
+                    if (each) ve = exponents(0, kU, top);
+                    const float f = move(top, ve, kGrow);
                     if (b > 0 && __any_sync(0xffffffffu, f != 1.f)) {
                         // the scores' MMAs came after the last P V, so O is complete
 #pragma unroll 1
@@ -885,12 +921,18 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     if (masked) scale_half(Yes{}); else scale_half(No{});
                     if (!exchange(top, other)) break;
                     top = max3(top, other, other);
+                    if (top != neg_inf()) top *= c;
+                    if (each) {
+                        ve = exponents(64 * half, 64 * half + 64, top);
+                        if (!exchange(ve, other)) break;
+                        ve = fmaxf(ve, other);
+                    }
                     if (b > 0) {  // P V of the block before, while S waited
                         if (!(ok = wait(&ctl.pv_full[mt], (n - 1) & 1))) break;
                         saw_bad(blocks - 1);
                         add_pv();
                     }
-                    alpha = move(top, 0.f);
+                    alpha = move(top, ve, 0.f);
                     const float base = off == neg_inf() ? 0.f : off;
                     auto weigh_half = [&](auto mask) {
 #pragma unroll

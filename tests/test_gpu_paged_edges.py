@@ -83,3 +83,97 @@ def test_equal_scores_of_any_magnitude_weigh_the_same(n, L, cache, dtype):
             lai.paged_kv_append(c.kv, c.whole, k, c.v_rows)
             out = lai.paged_attention(q, c.kv, c.batch, scale=1.0).double().view(n, 2, 64)
             assert (out - want[:, None]).abs().max() <= tol, (e, sign)
+
+
+# ---- values of very different sizes --------------------------------------------------------------
+def joint(c, s, L, dtype, cache, window=0):
+    """(o, tolerance) of one sequence: as paged_ref.tolerance, but what a weight's last binary16 place
+    is worth goes by the largest product of a weight and its value, among the keys the row sees."""
+    n, H, hd = c.new[s], c.H, c.hd
+    k = ref.sequence(ref.values(c.kv.k, c.kv.k_scale), c.pages[s], L)
+    v = ref.sequence(ref.values(c.kv.v, c.kv.v_scale), c.pages[s], L)
+    q = c.q[sum(c.new[:s]):sum(c.new[:s + 1])].double().view(n, H, hd)
+    o, a, b, _ = ref.attend(q, k, v, L - n, hd ** -0.5, window)
+    G = H // c.Hkv
+    kh, vtop = k.repeat_interleave(G, 1), v.abs().amax(-1).repeat_interleave(G, 1)  # [keys, H]
+    j, p = torch.arange(L, device=DEV), torch.arange(L - n, L, device=DEV)[:, None]
+    see = (j <= p) & (j > p - (window or 1 << 40))
+    w = torch.softmax((torch.einsum("nhd,khd->hnk", q, kh) * hd ** -0.5).masked_fill(~see, -math.inf), -1)
+    u = (see.sum(-1)[None] * (w * vtop.T[:, None]).amax(-1)).T[..., None]
+    return o.flatten(1), ref.tolerance(o, a, b, u, c.dtype, c.cache).flatten(1)
+
+
+@pytest.mark.parametrize("n", [6, 1100])
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+@pytest.mark.parametrize("power", [24, 30, 42, 60, 100])
+def test_a_large_value_reaches_only_who_sees_it(n, cache, dtype, power):
+    L = n + 30
+    c = Case([n], [L], 4, 2, 128, cache, 16, dtype, seed=34)
+    j = 30 + n // 2
+    v = c.v_rows.clone()
+    v[j] *= 2.0 ** power
+    lai.paged_kv_append(c.kv, c.whole, c.k_rows, v)
+    out = lai.paged_attention(c.q, c.kv, c.batch).double()
+    o, tol = joint(c, 0, L, dtype, cache)
+    assert ((out - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [1, 6, 1100])
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+@pytest.mark.parametrize("q_std", [1.0, 30.0])
+def test_values_over_many_orders_lose_no_more_than_their_share(n, cache, dtype, q_std):
+    """Value rows from 2^-45 to 2^45, under weights from 1 to e^-100 (q_std 30): a large value under a
+    small weight takes nothing from a small value under a large one, but what it adds itself."""
+    L = n + 300
+    c = Case([n], [L], 2, 1, 64, cache, 16, dtype, seed=35, q_std=q_std)
+    v = c.v_rows * torch.exp2(torch.randint(-45, 46, (L, 1), generator=gen(6), device=DEV).float())
+    lai.paged_kv_append(c.kv, c.whole, c.k_rows, v)
+    out = lai.paged_attention(c.q, c.kv, c.batch).double()
+    o, tol = joint(c, 0, L, dtype, cache)
+    assert ((out - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [1, 6, 1100])
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+@pytest.mark.parametrize("power", [-80, -50, 70, 110])
+def test_values_of_one_extreme_size(n, cache, dtype, power):
+    c = Case([n], [n + 50], 2, 1, 64, cache, 16, dtype, seed=36)
+    lai.paged_kv_append(c.kv, c.whole, c.k_rows, c.v_rows * 2.0 ** power)
+    out = lai.paged_attention(c.q, c.kv, c.batch).double()
+    o, tol = joint(c, 0, n + 50, dtype, cache)
+    assert ((out - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [1, 6, 1100])
+@pytest.mark.parametrize("cache", list(ref.FORMATS))
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+@pytest.mark.parametrize("slope", [0.02, 0.3])
+def test_scores_that_rise_along_the_sequence(n, cache, dtype, slope):
+    """The maximum moves at every step, by little or much, while the values shrink."""
+    L = n + 900
+    c = Case([n], [L], 2, 1, 64, cache, 16, dtype, seed=38)
+    at = torch.arange(L, device=DEV)[:, None]
+    k = torch.zeros_like(c.k_rows)
+    k[:, :1] = slope * at
+    lai.paged_kv_append(c.kv, c.whole, k, c.v_rows * torch.exp2(-0.01 * at))
+    c.q.zero_()
+    c.q[:, 0], c.q[:, 64] = 8.0, -8.0
+    out = lai.paged_attention(c.q, c.kv, c.batch).double()
+    o, tol = joint(c, 0, L, dtype, cache)
+    assert ((out - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [6, 1100])
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+def test_value_scales_that_append_never_makes(n, cache, dtype):
+    """A cache filled by other means: scales that are zero, negative or below F32's normal range."""
+    L = n + 100
+    c = Case([n], [L], 4, 2, 128, cache, 16, dtype, seed=39)
+    s = c.kv.v_scale
+    pick = torch.randint(0, 8, s.shape, generator=gen(7), device=DEV)
+    s.copy_(torch.where(pick == 0, 0.0, torch.where(pick == 1, -s, torch.where(pick == 2, s * 1e-38, s))))
+    c.check()

@@ -383,8 +383,8 @@ LAI_API int lai_paged_kv_read_f32(float *k, float *v, int64_t ld, int64_t n_rows
  * terms), with BF16 q the weights of the values may be rounded to BF16 (BF16 cache) or to
  * binary16. Over an 8-bit cache a weight counts with its value's scale: what is below 2^-26 (F32 q)
  * or 2^-18 (BF16 q) of the largest such product among the keys that the row sees may be rounded
- * away. That holds for value scales of 2^-90 to 2^106 and, beside scales outside 2^-14 to 2^14, for
- * scores up to 2^27. The result has the same bits in every call with the same batch, but a row's bits
+ * away. That holds for key scales to 2^90, value scales of 2^-90 to 2^106 and, beside scales
+ * outside 2^-14 to 2^14, for scores up to 2^27. The result has the same bits in every call with the same batch, but a row's bits
  * depend on the rows it shares a batch with.
  * scratch: lai_paged_attention_scratch_bytes(head_dim) bytes, zeroed once before first use; every
  * call leaves it reusable, but two calls that may run at the same time (other streams, graphs on

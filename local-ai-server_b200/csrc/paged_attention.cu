@@ -298,7 +298,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                 }
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = (int)(top >> 23) - 127;
+                const int e = max((int)(top >> 23) - 127, -113);  // 2^(13 - e) and its reciprocal are normal
                 up = pow2i(13 - e);
                 row_scale *= pow2i(e - 13);
             }

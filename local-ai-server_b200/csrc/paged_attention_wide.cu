@@ -686,7 +686,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
 #pragma unroll
                             for (int o = kLanes / 2; o > 0; o >>= 1)
                                 top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            const int e = (int)(top >> 23) - 127;
+                            const int e = max((int)(top >> 23) - 127, -113);  // both powers are normal
                             up = pow2i(13 - e);
                             // the thread that owns the row keeps the other side of the scaling
                             const int mine = __shfl_sync(0xffffffffu, e, lane % kAtOnce * kLanes);
@@ -724,7 +724,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                     }
                 }
                 if (!ok) break;
-                c = fmaxf(c, 1.2e-38f);  // masked scores, -inf, stay -inf
+                c = fmaxf(c, 1e-44f);  // masked scores, -inf, stay -inf
                 bulk::fence_proxy_async_smem();
                 bulk::mbar_arrive(&ctl.q_full[mt]);
             }

@@ -177,3 +177,16 @@ def test_value_scales_that_append_never_makes(n, cache, dtype):
     pick = torch.randint(0, 8, s.shape, generator=gen(7), device=DEV)
     s.copy_(torch.where(pick == 0, 0.0, torch.where(pick == 1, -s, torch.where(pick == 2, s * 1e-38, s))))
     c.check()
+
+
+# ---- queries and keys at the ends of F32 ----------------------------------------------------------
+# (key scales end at 2^90: behind that only the kernel for few rows has the room)
+@pytest.mark.parametrize("n,power", [(n, p) for n in (1, 6) for p in (90, 105, 112, 114, 118, -90, -110)] +
+                         [(1100, p) for p in (60, 94, -90, -110)])
+@pytest.mark.parametrize("cache", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", list(ref.DTYPES))
+def test_small_queries_over_large_keys(n, power, cache, dtype):
+    c = Case([n], [n + 50], 2, 1, 64, cache, 16, dtype, seed=37)
+    lai.paged_kv_append(c.kv, c.whole, c.k_rows * 2.0 ** power, c.v_rows)
+    c.q *= 2.0 ** -power
+    c.check()

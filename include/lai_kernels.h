@@ -386,9 +386,9 @@ LAI_API int lai_paged_kv_read_f32(float *k, float *v, int64_t ld, int64_t n_rows
  * away. That holds for key scales to 2^90, value scales of 2^-90 to 2^106 and, beside scales
  * outside 2^-14 to 2^14, for scores up to 2^27. The result has the same bits in every call with the same batch, but a row's bits
  * depend on the rows it shares a batch with.
- * scratch: lai_paged_attention_scratch_bytes(head_dim) bytes, zeroed once before first use; every
- * call leaves it reusable, but two calls that may run at the same time (other streams, graphs on
- * other streams) need one each. */
+ * scratch: lai_paged_attention_scratch_bytes(head_dim) bytes, the first 4096 of them zeroed once
+ * before first use; every call leaves it reusable, but two calls that may run at the same time
+ * (other streams, graphs on other streams) need one each. */
 LAI_API size_t lai_paged_attention_scratch_bytes(int head_dim);
 LAI_API int lai_paged_attention_bf16(lai_bf16 *out, const lai_bf16 *q, int64_t ld_q,
                                      int64_t n_rows, int n_heads, const lai_paged_kv_t *kv,

@@ -7,6 +7,7 @@ calls fail loudly.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -548,6 +549,23 @@ def _paged_call(fn, index, stream, *args):
         raise LaiError(fn.__name__, st)
 
 
+def _made_on(stream):
+    """Where a call on `stream` makes its own tensors, so that their memory is given out, zeroed and
+    given back in that stream's order (None: the current stream, as it is)."""
+    import torch
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _handed_out(stream, *tensors):
+    """tensors, made on `stream`, go to a caller who may use and drop them on the current stream."""
+    import torch
+    if stream is not None:
+        current = torch.cuda.current_stream(tensors[0].device)
+        if current != stream:
+            for t in tensors:
+                t.record_stream(current)
+
+
 def paged_kv_append(kv, batch, k, v, err=None, stream=None):
     """Write the new tokens' rows k, v [rows, n_kv_heads * head_dim] (F32 or BF16; column blocks
     of one tensor will do) to their positions in the cache, quantising them if it is an 8-bit one."""
@@ -568,8 +586,11 @@ def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None)
     ranges these are whole sequences."""
     import torch
     fn = _paged_fn("lai_paged_kv_read", dtype)
-    k = kv.k.new_empty((rows, kv.width), dtype=dtype) if k is None else k
-    v = torch.empty_like(k) if v is None else v
+    made = [x is None for x in (k, v)]
+    if any(made):
+        with _made_on(stream):
+            k = kv.k.new_empty((rows, kv.width), dtype=dtype) if k is None else k
+            v = torch.empty_like(k) if v is None else v
     if k.dtype != dtype or v.dtype != dtype or k.shape[0] != rows or v.shape[0] != rows:
         raise ValueError("k and v must be [rows, n_kv_heads * head_dim] of dtype")
     ld = _paged_rows(k, kv.width)
@@ -578,17 +599,22 @@ def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None)
     _need_cuda(kv.index, batch.q_start, k, v, err)
     _paged_call(fn, kv.index, stream, k.data_ptr(), v.data_ptr(), ld, rows, kv._ref, batch._ref,
                 None if err is None else err.data_ptr())
+    if any(made):
+        _handed_out(stream, *(x for x, new in zip((k, v), made) if new))
     return k, v
 
 
 def paged_attention_scratch(head_dim=128, device="cuda"):
-    """Zeroed scratch for paged_attention, of one size for every batch. It serves any number of
-    calls one after another; calls that may run at the same time need one each."""
+    """Scratch for paged_attention, of one size for every batch, zeroed where it has to be. It serves
+    any number of calls one after another; calls that may run at the same time need one each."""
     import torch
-    return torch.zeros(_paged_scratch_floats(head_dim), dtype=torch.float32, device=device)
+    scratch = torch.empty(_paged_scratch_floats(head_dim), dtype=torch.float32, device=device)
+    scratch[:_PAGED_ZEROED // 4].zero_()
+    return scratch
 
 
 _PAGED_SCRATCH: dict = {}
+_PAGED_ZEROED = 4096  # bytes at the front of the scratch that a first call finds zeroed
 
 
 def _paged_scratch_floats(head_dim):
@@ -610,18 +636,21 @@ def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, 
     if len(shape) != 2 or shape[1] % kv.width:
         raise ValueError("q must be [rows, n_heads * head_dim], n_heads a multiple of n_kv_heads")
     ld = _paged_rows(q, shape[1])
-    if out is None:
-        out = q.new_empty(shape)
-    elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
+    made = out is None
+    if made or scratch is None:
+        with _made_on(stream):
+            out = q.new_empty(shape) if made else out
+            scratch = paged_attention_scratch(hd, kv.device) if scratch is None else scratch
+    if not made and (out.dtype != q.dtype or out.shape != shape or not out.is_contiguous()):
         raise ValueError("out must be contiguous, of q's shape and dtype")
-    if scratch is None:
-        scratch = paged_attention_scratch(hd, kv.device)
-    elif scratch.nbytes < 4 * _paged_scratch_floats(hd):
+    if scratch.nbytes < 4 * _paged_scratch_floats(hd):
         raise ValueError("scratch is too small: use paged_attention_scratch(head_dim)")
     _need_cuda(kv.index, batch.q_start, q, out, scratch, err)
     _paged_call(fn, kv.index, stream, out.data_ptr(), q.data_ptr(), ld, shape[0], shape[1] // hd,
                 kv._ref, batch._ref, hd ** -0.5 if scale is None else scale, window,
                 scratch.data_ptr(), None if err is None else err.data_ptr())
+    if made:
+        _handed_out(stream, out)
     return out
 
 

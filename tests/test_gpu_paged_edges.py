@@ -190,3 +190,29 @@ def test_small_queries_over_large_keys(n, power, cache, dtype):
     lai.paged_kv_append(c.kv, c.whole, c.k_rows * 2.0 ** power, c.v_rows)
     c.q *= 2.0 ** -power
     c.check()
+
+
+# ---- tensors that a call makes ---------------------------------------------------------------------
+@pytest.mark.parametrize("new,keys", [([1, 1], [20000, 900]), ([300], [9000])])
+def test_calls_on_a_stream_beside_a_busy_current_one(new, keys):
+    """Scratch and outputs that the call makes itself, while the current stream is far behind and goes
+    on making and dropping memory of the same sizes."""
+    c = Case(new, keys, 8, 4, 128, "i8", 64, "f32", seed=40)
+    want = c.check()
+    k, v = lai.paged_kv_read(c.kv, c.whole, sum(keys), torch.float32)
+    x = torch.randn((8192, 8192), device=DEV, dtype=torch.bfloat16)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        x = x @ x  # about a millisecond each
+        stale = torch.full((10_000_000,), 7.0, device=DEV)
+        del stale
+        outs.append(lai.paged_attention(c.q, c.kv, c.batch, stream=stream))
+        outs.append(lai.paged_kv_read(c.kv, c.whole, sum(keys), torch.float32, stream=stream))
+    stream.synchronize()
+    for got in outs:
+        if isinstance(got, tuple):
+            assert torch.equal(got[0], k) and torch.equal(got[1], v)
+        else:
+            assert torch.equal(got, want)

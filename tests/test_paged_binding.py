@@ -1,0 +1,72 @@
+"""What the paged cache's binding makes and checks by itself, on the host: no kernel runs."""
+import contextlib
+import types
+
+import pytest
+
+import lai
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """CPU tensors in place of CUDA ones; the entry points only note their arguments. .made: every
+    tensor that the binding makes, and the stream that was current then; .recorded: tensors that
+    were told of another stream."""
+    got = types.SimpleNamespace(made=[], recorded=[], entries=[], current="theirs")
+
+    @contextlib.contextmanager
+    def stream(s):
+        was, got.current = got.current, s
+        yield
+        got.current = was
+
+    def note(fn):
+        def made(*a, **kw):
+            t = fn(*a, **{k: v for k, v in kw.items() if k != "device"})
+            got.made.append((t.data_ptr(), got.current))
+            return t
+        return made
+
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: got.current)
+    monkeypatch.setattr(lai, "_need_cuda", lambda *a: None)
+    monkeypatch.setattr(lai, "_paged_call", lambda fn, index, s, *a: got.entries.append((fn.__name__, s, a)))
+    for name in ("empty", "zeros", "empty_like", "empty_strided"):
+        monkeypatch.setattr(torch, name, note(getattr(torch, name)))
+    monkeypatch.setattr(torch.Tensor, "new_empty", note(torch.Tensor.new_empty))
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: got.recorded.append((t.data_ptr(), s)), raising=False)
+    return got
+
+
+def cache(dtype=torch.bfloat16):
+    return lai.PagedKV(torch.ones((4, 2, 16, 64), dtype=dtype), torch.ones((4, 2, 16, 64), dtype=dtype))
+
+
+def batch(*q_start):
+    n = len(q_start) - 1
+    return lai.PagedBatch(torch.tensor(q_start, dtype=torch.int32), torch.ones(n, dtype=torch.int32),
+                          torch.tensor([[0, 1]] * n, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_what_a_call_makes_is_made_in_its_streams_order(calls, given):
+    """Scratch that is zeroed, or memory that is given back, in another stream's order than the
+    kernel's would be written under it."""
+    kv, b, q = cache(), batch(0, 3), torch.ones((3, 256))
+    mine = types.SimpleNamespace(cuda_stream=7) if given else None
+    calls.made.clear()
+    out = lai.paged_attention(q, kv, b, stream=mine)
+    k, v = lai.paged_kv_read(kv, b, 3, torch.float32, stream=mine)
+    want = mine if given else "theirs"
+    assert len(calls.made) >= 4 and all(s is want for _, s in calls.made)
+    assert [s for _, s, _ in calls.entries] == [mine, mine]
+    # what the caller gets is also known to the stream that they will use it on
+    assert calls.recorded == ([(t.data_ptr(), "theirs") for t in (out, k, v)] if given else [])
+
+
+def test_scratch_is_zeroed_where_the_kernels_count():
+    a = lai.paged_attention_scratch(64, "cpu")
+    assert a.nbytes == lai.load().lai_paged_attention_scratch_bytes(64)
+    assert not a[:1024].view(torch.int32).any()

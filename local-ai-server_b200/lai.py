@@ -424,6 +424,23 @@ def prefill_attention_rope(qkv, n_heads, n_kv_heads, head_dim, cos_t, sin_t, sca
     return out
 
 
+def _made_on(stream):
+    """Where a call on `stream` makes its own tensors, so that their memory is given out, zeroed and
+    given back in that stream's order (None: the current stream, as it is)."""
+    import torch
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _handed_out(stream, *tensors):
+    """tensors, made on `stream`, go to a caller who may use and drop them on the current stream."""
+    import torch
+    if stream is not None:
+        current = torch.cuda.current_stream(tensors[0].device)
+        if current != stream:
+            for t in tensors:
+                t.record_stream(current)
+
+
 class _PagedKVC(ctypes.Structure):
     """lai_paged_kv_t."""
     _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("n_pages", _i64),
@@ -547,23 +564,6 @@ def _paged_call(fn, index, stream, *args):
         st = fn(*args, torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream)
     if st != LAI_OK:
         raise LaiError(fn.__name__, st)
-
-
-def _made_on(stream):
-    """Where a call on `stream` makes its own tensors, so that their memory is given out, zeroed and
-    given back in that stream's order (None: the current stream, as it is)."""
-    import torch
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
-
-
-def _handed_out(stream, *tensors):
-    """tensors, made on `stream`, go to a caller who may use and drop them on the current stream."""
-    import torch
-    if stream is not None:
-        current = torch.cuda.current_stream(tensors[0].device)
-        if current != stream:
-            for t in tensors:
-                t.record_stream(current)
 
 
 def paged_kv_append(kv, batch, k, v, err=None, stream=None):
@@ -695,9 +695,11 @@ def decode_attention(q, k_new, v_new, k_cache, v_cache, pos, n_heads, n_kv_heads
     import torch
     S, max_seq = k_cache.shape[0], k_cache.shape[1]
     hd = q.shape[1] // n_heads
-    if scratch is None:
-        scratch = decode_attention_scratch(S, n_heads, n_kv_heads, max_seq, q.device)
-    out = torch.empty_like(q) if out is None else out
+    made = out is None
+    with _made_on(stream):
+        if scratch is None:
+            scratch = decode_attention_scratch(S, n_heads, n_kv_heads, max_seq, q.device)
+        out = torch.empty_like(q) if made else out
     sc = hd ** -0.5 if scale is None else scale
     if qk is None:
         call("lai_decode_attention_f32", _p(out), _p(q), _p(k_new), _p(v_new), _p(k_cache),
@@ -709,6 +711,8 @@ def decode_attention(q, k_new, v_new, k_cache, v_cache, pos, n_heads, n_kv_heads
              _p(v_cache), _p(pos), S, n_heads, n_kv_heads, hd, max_seq, sc, _p(wq), _p(wk),
              _p(cos_t), _p(sin_t), 0 if cos_t is None else cos_t.shape[0], eps, _p(scratch),
              _p(err), _s(stream))
+    if made:
+        _handed_out(stream, out)
     return out
 
 

@@ -70,3 +70,16 @@ def test_scratch_is_zeroed_where_the_kernels_count():
     a = lai.paged_attention_scratch(64, "cpu")
     assert a.nbytes == lai.load().lai_paged_attention_scratch_bytes(64)
     assert not a[:1024].view(torch.int32).any()
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_decode_attention_makes_its_own_in_its_streams_order(calls, given, monkeypatch):
+    mine = types.SimpleNamespace(cuda_stream=7) if given else None
+    monkeypatch.setattr(lai, "call", lambda *a: calls.entries.append(a))
+    monkeypatch.setattr(lai, "_s", lambda s: s)
+    kc, vc = torch.ones((2, 32, 256)), torch.ones((2, 32, 256))
+    row = torch.ones((2, 256))
+    calls.made.clear()
+    out = lai.decode_attention(torch.ones((2, 512)), row, row, kc, vc, torch.ones(2, dtype=torch.int32), 4, 2, stream=mine)
+    assert len(calls.made) == 2 and all(s is (mine if given else "theirs") for _, s in calls.made)
+    assert calls.recorded == ([(out.data_ptr(), "theirs")] if given else [])

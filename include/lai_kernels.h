@@ -332,7 +332,7 @@ LAI_API int lai_prefill_attention_rope_f32(float *out, const float *q, const flo
  * Rows before q_start[0] and behind q_start[n_seqs] are left as they are. A sequence whose
  * q_start leaves [0, n_rows], or whose kv_len leaves [0, max_pages * page_size], is skipped and
  * sets LAI_DEVERR_POSITION; so does a q_start that decreases, and then other sequences may be
- * skipped too (nothing outside the tensors is touched).
+ * skipped too (attention skips all; nothing outside the tensors is touched).
  */
 enum { LAI_KV_BF16 = 0, LAI_KV_E4M3 = 1, LAI_KV_I8 = 2 };
 typedef struct {

@@ -184,6 +184,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
         bulk::fence_barrier_init();
     }
     const AttnArgs as = cache_seqs<kThreads>(a, sm.seqs);
+    if (as.kv.n_seqs == 0) return;  // the whole grid
     const Range range = find_range<FewSched<FMT>, kThreads>(as, sm.sched);
     if (range.w0 >= range.w1) return;  // the whole CTA
 

@@ -81,8 +81,9 @@ struct Sched {
         const int64_t keys = ((int64_t)v.max_pages << v.log_page) + U;
         return slots(v.n_rows, group, v.n_seqs) * (keys / U + 1 + E) * v.n_kv;
     }
+    // (q_start never decreases here, and neither do these, wherever it leaves the rows)
     static __device__ __forceinline__ int base(const AttnArgs &a, int s) {
-        return a.kv.q_start[s] * a.group / R + s;
+        return min(max(a.kv.q_start[s], 0), (int)a.kv.n_rows) * a.group / R + s;
     }
     static __device__ __forceinline__ int cost(const Tile &t) { return t.rows ? t.blocks + E : 0; }
     // The last sequence whose slots start at or before `slot` (0 if none does).
@@ -124,21 +125,34 @@ constexpr int kSeqCache = 256;
 struct SeqSmem {
     int32_t q_start[kSeqCache + 1], kv_len[kSeqCache];
 };
-// a with its tables in shared memory (or as it is); flags sequences that are not well formed. The
-// whole CTA; ends with a barrier.
+// a with its tables in shared memory (or as it is); flags sequences that are not well formed. Where
+// q_start decreases there is no work at all (n_seqs 0): looking for a slot's sequence from its both
+// ends finds different ones then, and CTAs that disagree on who shares an item leave its counter
+// behind for the next call. The whole CTA; has a barrier.
 template <int THREADS>
 __device__ __forceinline__ AttnArgs cache_seqs(const AttnArgs &a, SeqSmem &sm) {
     AttnArgs c = a;
-    if (a.kv.n_seqs <= kSeqCache) {
-        for (int s = threadIdx.x; s <= a.kv.n_seqs; s += THREADS) sm.q_start[s] = __ldg(a.kv.q_start + s);
-        for (int s = threadIdx.x; s < a.kv.n_seqs; s += THREADS) sm.kv_len[s] = __ldg(a.kv.kv_len + s);
+    const bool keep = a.kv.n_seqs <= kSeqCache;
+    bool falls = false;
+#pragma unroll 4
+    for (int s = threadIdx.x; s < a.kv.n_seqs; s += THREADS) {
+        const int q0 = __ldg(a.kv.q_start + s), q1 = __ldg(a.kv.q_start + s + 1);
+        falls |= q1 < q0;
+        if (keep) {
+            sm.q_start[s] = q0;
+            sm.kv_len[s] = __ldg(a.kv.kv_len + s);
+            if (s + 1 == a.kv.n_seqs) sm.q_start[s + 1] = q1;
+        }
+    }
+    if (keep) {
         c.kv.q_start = sm.q_start;
         c.kv.kv_len = sm.kv_len;
     }
-    __syncthreads();
+    falls = __syncthreads_or(falls);
     if (blockIdx.x == 0)
         for (int s = threadIdx.x; s < a.kv.n_seqs; s += THREADS)
             if (!load_seq(c.kv, s).ok) flag(a.err, LAI_DEVERR_POSITION);
+    if (falls) c.kv.n_seqs = 0;
     return c;
 }
 

@@ -260,6 +260,7 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
         return;
     }
     const AttnArgs as = cache_seqs<kThreads>(a, ctl.seqs);
+    if (as.kv.n_seqs == 0) return;  // the whole grid
     // (in the place of Q, which comes behind the barrier below)
     const Range range = find_range<S, kThreads>(as, *reinterpret_cast<SchedSmem *>(q_smem));
     if (range.w0 >= range.w1) return;  // the whole CTA

@@ -216,3 +216,50 @@ def test_calls_on_a_stream_beside_a_busy_current_one(new, keys):
             assert torch.equal(got[0], k) and torch.equal(got[1], v)
         else:
             assert torch.equal(got, want)
+
+
+# ---- batches that are not well formed ---------------------------------------------------------------
+@pytest.mark.parametrize("many", [1, 8])
+@pytest.mark.parametrize("cache,dtype", [("i8", "f32"), ("bf16", "bf16")])
+def test_a_malformed_batch_leaves_the_scratch_as_it_was(many, cache, dtype):
+    """q_start that decreases, or leaves the rows by little or by all an int has: flagged, and the next
+    call with the same scratch is right."""
+    import random
+    r = random.Random(many)
+    rows, keys = 200 * many, [r.randint(100, 3000) + 200 * many for _ in range(10)]
+    c = Case([20 * many] * 10, keys, 4, 2, 128, cache, 16, dtype, seed=41)
+    scratch = lai.paged_attention_scratch(128)
+    want = c.check(scratch=scratch)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(c.q)
+    bad = [[x * many for x in (0, 76, 12, 96, 192, 154, 176, 72, 44, 43, 112)]]
+    bad += [[0] + [r.randint(0, rows) for _ in range(10)] for _ in range(60)]
+    bad += [sorted(r.choice([-2 ** 31, -5, 0, 3, rows // 2, rows, rows + 1, 2 ** 27, 2 ** 28, 2 ** 31 - 1]) for _ in range(11))
+            for _ in range(60)]
+    for q_start in bad:
+        assert len(q_start) == 11
+        fine = all(0 <= a <= b <= rows for a, b in zip(q_start, q_start[1:]))
+        err.zero_()
+        lai.paged_attention(c.q, c.kv, lai.PagedBatch(i32(q_start), c.batch.kv_len, c.batch.pages), scratch=scratch, out=out, err=err)
+        assert (int(err) != 0) != fine, q_start
+        assert not scratch[:1024].view(torch.int32).any(), q_start
+    assert torch.equal(c.check(scratch=scratch), want)
+
+
+@pytest.mark.parametrize("n", [3, 400])
+def test_sequences_beside_one_that_leaves_the_rows_are_computed(n):
+    c = Case([n, n, n], [n + 60, n + 700, n + 9], 4, 2, 64, "i8", 16, "f32", seed=42)
+    want = c.check()
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for q_start, good in (([0, n, 2 * n, 3 * n + 1], (0, 1)), ([0, n, 2 * n, 2 ** 31 - 1], (0, 1)), ([-7, n, 2 * n, 3 * n], (1, 2)),
+                          ([-2 ** 31, n, 2 * n, 2 ** 31 - 1], (1,))):
+        out = torch.full_like(c.q, 9.0)
+        err.zero_()
+        lai.paged_attention(c.q, c.kv, lai.PagedBatch(i32(q_start), c.batch.kv_len, c.batch.pages), out=out, err=err)
+        assert int(err) == lai.LAI_DEVERR_POSITION
+        for s in range(3):
+            got = out[s * n:(s + 1) * n]
+            if s in good:  # (the schedule differs, so the bits may)
+                assert (got - want[s * n:(s + 1) * n]).abs().max() <= 2e-5
+            else:
+                assert (got == 9).all()

@@ -53,10 +53,11 @@ enum {
 
 /* Bits ORed into the caller's device error word. LAI_DEVERR_TIMEOUT: a kernel's
  * bounded wait on its own asynchronous copies ran out (never expected; the kernel
- * drains what it issued and returns instead of hanging). LAI_DEVERR_SMEM_ALIGN: a
- * tensor-core kernel found its dynamic shared memory less than 1 KiB aligned and
- * computed nothing (never expected). LAI_DEVERR_PAGE: a page table entry was outside the
- * cache's pages. */
+ * drains what it issued and returns instead of hanging); what the call wrote is then not
+ * to be used, and a scratch that is zeroed before its first use has to be zeroed again.
+ * LAI_DEVERR_SMEM_ALIGN: a tensor-core kernel found its dynamic shared memory less than
+ * 1 KiB aligned and computed nothing (never expected). LAI_DEVERR_PAGE: a page table entry
+ * was outside the cache's pages. */
 enum { LAI_DEVERR_TOKEN_ID = 1, LAI_DEVERR_POSITION = 2, LAI_DEVERR_TIMEOUT = 4,
        LAI_DEVERR_SMEM_ALIGN = 8, LAI_DEVERR_PAGE = 16 };
 
@@ -387,8 +388,9 @@ LAI_API int lai_paged_kv_read_f32(float *k, float *v, int64_t ld, int64_t n_rows
  * outside 2^-14 to 2^14, for scores up to 2^27. The result has the same bits in every call with the same batch, but a row's bits
  * depend on the rows it shares a batch with.
  * scratch: lai_paged_attention_scratch_bytes(head_dim) bytes, the first 4096 of them zeroed once
- * before first use; every call leaves it reusable, but two calls that may run at the same time
- * (other streams, graphs on other streams) need one each. */
+ * before first use; every call leaves it reusable (one that set LAI_DEVERR_TIMEOUT does not: zero
+ * them again), but two calls that may run at the same time (other streams, graphs on other streams)
+ * need one each. */
 LAI_API size_t lai_paged_attention_scratch_bytes(int head_dim);
 LAI_API int lai_paged_attention_bf16(lai_bf16 *out, const lai_bf16 *q, int64_t ld_q,
                                      int64_t n_rows, int n_heads, const lai_paged_kv_t *kv,

@@ -606,7 +606,8 @@ def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None)
 
 def paged_attention_scratch(head_dim=128, device="cuda"):
     """Scratch for paged_attention, of one size for every batch, zeroed where it has to be. It serves
-    any number of calls one after another; calls that may run at the same time need one each."""
+    any number of calls one after another; calls that may run at the same time need one each. After a
+    call that set LAI_DEVERR_TIMEOUT it has to be made again."""
     import torch
     scratch = torch.empty(_paged_scratch_floats(head_dim), dtype=torch.float32, device=device)
     scratch[:_PAGED_ZEROED // 4].zero_()

@@ -114,6 +114,22 @@ template <int FMT> __device__ __forceinline__ bool drop_nonfinite(uint32_t &x) {
     return gone != 0;
 }
 
+// 16 or 8 bytes of shared memory by one instruction: none of them arrives apart from the others.
+__device__ __forceinline__ uint4 slot_load16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 slot_load8(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 slot_scales(uint32_t at) {
+    const uint2 v = slot_load8(at);
+    return make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+}
+
 // One stored element as F32, without its scale.
 template <int FMT> __device__ __forceinline__ float element(const unsigned char *v, int64_t i) {
     if (FMT == LAI_KV_BF16) return to_f(reinterpret_cast<const uint16_t *>(v)[i]);
@@ -339,7 +355,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             }
             __syncwarp();
             wait(&sm.full[slot], (id / kRing) & 1);
-            const unsigned char *from = sm.ring[slot];
+            const uint32_t from = bulk::smem_addr(sm.ring[slot]);  // read by slot_load alone
             const uint32_t there = sm.there[slot];
             if (there == 0) {  // none of its keys
                 __syncwarp();
@@ -359,7 +375,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
                     if (s % kPerChunk == 0)
-                        kr[n] = *reinterpret_cast<const uint4 *>(from + (8 * n + g) * Ck::kRow + 16 * t + 64 * (s / kPerChunk));
+                        kr[n] = slot_load16(from + (8 * n + g) * Ck::kRow + 16 * t + 64 * (s / kPerChunk));
                     const uint4 r = kr[n];
                     uint32_t b0, b1;
                     if constexpr (kF16) {
@@ -389,8 +405,8 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             if (kF16) {
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
-                    ks[n] = *reinterpret_cast<const float2 *>(from + Ck::kScaleK + (8 * n + 2 * t) * 4);
-                    vs[n] = *reinterpret_cast<const float2 *>(from + Ck::kScaleV + (8 * n + 2 * t) * 4);
+                    ks[n] = slot_scales(from + Ck::kScaleK + (8 * n + 2 * t) * 4);
+                    vs[n] = slot_scales(from + Ck::kScaleV + (8 * n + 2 * t) * 4);
                 }
             }
             const bool uneven = mixed(tl, a.window, j0, kStep);
@@ -468,14 +484,14 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
             for (int kk = 0; kk < NK; kk++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const unsigned char *p = from + Ck::kV + (16 * kk + 2 * t + (i & 1) + 8 * (i >> 1)) * Ck::kRow;
+                    const uint32_t p = from + Ck::kV + (16 * kk + 2 * t + (i & 1) + 8 * (i >> 1)) * Ck::kRow;
                     if constexpr (VW == 2) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(p + 8 * g);
+                        const uint2 x = slot_load8(p + 8 * g);
                         vr[kk][i][0] = x.x; vr[kk][i][1] = x.y;
                     } else {
 #pragma unroll
                         for (int c = 0; c < VW / 4; c++) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(p + 16 * g + 128 * c);
+                            const uint4 x = slot_load16(p + 16 * g + 128 * c);
                             vr[kk][i][4 * c] = x.x; vr[kk][i][4 * c + 1] = x.y;
                             vr[kk][i][4 * c + 2] = x.z; vr[kk][i][4 * c + 3] = x.w;
                         }
@@ -554,7 +570,7 @@ paged_attn_few_kernel(void *out, const void *__restrict__ qp, const AttnArgs a) 
                     // does not keep behind generic loads still in flight: with no more than __syncwarp
                     // between loads and arrival, 0.4% of calls with many short BF16 sequences were
                     // wrong. So the arrival waits for products of every load (of all lanes: an MMA
-                    // takes the whole warp's operands).
+                    // takes the whole warp's operands; of all bytes of a load: it is one instruction).
                     const float after = VW == 8 ? o[0][0] + o[ND / 2][0] : o[0][0];
                     if (lane == 0) bulk::mbar_arrive(&sm.empty[slot] + (__float_as_uint(after) & zero));
                 }

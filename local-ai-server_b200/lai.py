@@ -536,7 +536,7 @@ def _paged_rows(t, width):
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or shape[1] != width or (stride[1] != 1 and width != 1):
         raise ValueError(f"rows must be [n, {width}] with adjacent elements")
-    return stride[0] if shape[0] > 1 else max(stride[0], width)
+    return stride[0] if shape[0] > 1 else width  # (a single row's stride says nothing)
 
 
 _PAGED_FN: dict = {}

@@ -83,3 +83,13 @@ def test_decode_attention_makes_its_own_in_its_streams_order(calls, given, monke
     out = lai.decode_attention(torch.ones((2, 512)), row, row, kc, vc, torch.ones(2, dtype=torch.int32), 4, 2, stream=mine)
     assert len(calls.made) == 2 and all(s is (mine if given else "theirs") for _, s in calls.made)
     assert calls.recorded == ([(out.data_ptr(), "theirs")] if given else [])
+
+
+def test_a_single_row_needs_no_stride(calls):
+    """One token's k and v as column blocks of different tensors, at any stride."""
+    kv, b = cache(), batch(0, 1)
+    k, v = torch.ones((1, 301))[:, 8:136], torch.ones((1, 128))
+    lai.paged_kv_append(kv, b, k, v)
+    lai.paged_attention(torch.ones((1, 999))[:, :256], kv, b, out=torch.ones((1, 256)))
+    assert [a[4] for name, _, a in calls.entries if "append" in name] == [128]
+    assert [a[2] for name, _, a in calls.entries if "attention" in name] == [256]

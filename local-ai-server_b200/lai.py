@@ -584,13 +584,13 @@ def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None)
     """The reverse of paged_kv_append: (k, v) [rows, n_kv_heads * head_dim], the values the cache
     stands for at the positions of the batch's rows. With kv_len as the lengths of q_start's
     ranges these are whole sequences."""
-    import torch
     fn = _paged_fn("lai_paged_kv_read", dtype)
     made = [x is None for x in (k, v)]
-    if any(made):
+    if any(made):  # (one of them alone has the row stride of the other)
+        ld = kv.width if all(made) else _paged_rows(v if k is None else k, kv.width)
         with _made_on(stream):
-            k = kv.k.new_empty((rows, kv.width), dtype=dtype) if k is None else k
-            v = torch.empty_like(k) if v is None else v
+            k = kv.k.new_empty((rows, ld), dtype=dtype)[:, :kv.width] if k is None else k
+            v = kv.k.new_empty((rows, ld), dtype=dtype)[:, :kv.width] if v is None else v
     if k.dtype != dtype or v.dtype != dtype or k.shape[0] != rows or v.shape[0] != rows:
         raise ValueError("k and v must be [rows, n_kv_heads * head_dim] of dtype")
     ld = _paged_rows(k, kv.width)

@@ -93,3 +93,11 @@ def test_a_single_row_needs_no_stride(calls):
     lai.paged_attention(torch.ones((1, 999))[:, :256], kv, b, out=torch.ones((1, 256)))
     assert [a[4] for name, _, a in calls.entries if "append" in name] == [128]
     assert [a[2] for name, _, a in calls.entries if "attention" in name] == [256]
+
+
+def test_read_makes_one_of_k_and_v_beside_the_other(calls):
+    kv, b, buf = cache(), batch(0, 3), torch.ones((3, 400))
+    for kw in (dict(k=buf[:, 16:144]), dict(v=buf[:, 16:144])):
+        k, v = lai.paged_kv_read(kv, b, 3, torch.float32, **kw)
+        assert k.shape == v.shape == (3, 128) and k.stride() == v.stride() == (400, 1)
+        assert calls.entries[-1][2][2] == 400

@@ -646,9 +646,11 @@ def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, 
         raise ValueError("out must be contiguous, of q's shape and dtype")
     if scratch.nbytes < 4 * _paged_scratch_floats(hd):
         raise ValueError("scratch is too small: use paged_attention_scratch(head_dim)")
+    if window < 0:
+        raise ValueError("window must not be negative")
     _need_cuda(kv.index, batch.q_start, q, out, scratch, err)
     _paged_call(fn, kv.index, stream, out.data_ptr(), q.data_ptr(), ld, shape[0], shape[1] // hd,
-                kv._ref, batch._ref, hd ** -0.5 if scale is None else scale, window,
+                kv._ref, batch._ref, hd ** -0.5 if scale is None else scale, min(window, 0x7fffffff),
                 scratch.data_ptr(), None if err is None else err.data_ptr())
     if made:
         _handed_out(stream, out)

@@ -101,3 +101,13 @@ def test_read_makes_one_of_k_and_v_beside_the_other(calls):
         k, v = lai.paged_kv_read(kv, b, 3, torch.float32, **kw)
         assert k.shape == v.shape == (3, 128) and k.stride() == v.stride() == (400, 1)
         assert calls.entries[-1][2][2] == 400
+
+
+def test_windows_of_any_length(calls):
+    kv, b, q = cache(), batch(0, 3), torch.ones((3, 256))
+    for window, want in ((0, 0), (7, 7), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1), (2 ** 32 + 5, 2 ** 31 - 1)):
+        lai.paged_attention(q, kv, b, window=window)
+        assert calls.entries[-1][2][8] == want
+    for window in (-1, -2 ** 32):
+        with pytest.raises(ValueError):
+            lai.paged_attention(q, kv, b, window=window)

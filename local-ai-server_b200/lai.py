@@ -644,7 +644,7 @@ def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, 
             scratch = paged_attention_scratch(hd, kv.device) if scratch is None else scratch
     if not made and (out.dtype != q.dtype or out.shape != shape or not out.is_contiguous()):
         raise ValueError("out must be contiguous, of q's shape and dtype")
-    if scratch.nbytes < 4 * _paged_scratch_floats(hd):
+    if scratch.nbytes < 4 * _paged_scratch_floats(hd) or not scratch.is_contiguous():
         raise ValueError("scratch is too small: use paged_attention_scratch(head_dim)")
     if window < 0:
         raise ValueError("window must not be negative")

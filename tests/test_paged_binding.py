@@ -111,3 +111,9 @@ def test_windows_of_any_length(calls):
     for window in (-1, -2 ** 32):
         with pytest.raises(ValueError):
             lai.paged_attention(q, kv, b, window=window)
+
+
+def test_refuses_a_scratch_that_only_looks_large(calls):
+    kv, b, q = cache(), batch(0, 3), torch.ones((3, 256))
+    with pytest.raises(ValueError):
+        lai.paged_attention(q, kv, b, scratch=torch.ones(1).expand(lai._paged_scratch_floats(64)))

@@ -7,7 +7,6 @@ calls fail loudly.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import re
@@ -424,21 +423,22 @@ def prefill_attention_rope(qkv, n_heads, n_kv_heads, head_dim, cos_t, sin_t, sca
     return out
 
 
-def _made_on(stream):
-    """Where a call on `stream` makes its own tensors, so that their memory is given out, zeroed and
-    given back in that stream's order (None: the current stream, as it is)."""
+def _made_on(stream, make, *args, **kw):
+    """make(*args, **kw) as a call on `stream` makes its own tensors: their memory is given out, zeroed
+    and given back in that stream's order (None: the current stream's)."""
+    if stream is None:
+        return make(*args, **kw)
     import torch
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+    with torch.cuda.stream(stream):
+        return make(*args, **kw)
 
 
-def _handed_out(stream, *tensors):
-    """tensors, made on `stream`, go to a caller who may use and drop them on the current stream."""
+def _handed_out(stream, t):
+    """t, made on `stream` (not None), goes to a caller who may use and drop it on the current one."""
     import torch
-    if stream is not None:
-        current = torch.cuda.current_stream(tensors[0].device)
-        if current != stream:
-            for t in tensors:
-                t.record_stream(current)
+    current = torch.cuda.current_stream(t.device)
+    if current != stream:
+        t.record_stream(current)
 
 
 class _PagedKVC(ctypes.Structure):
@@ -584,13 +584,16 @@ def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None)
     """The reverse of paged_kv_append: (k, v) [rows, n_kv_heads * head_dim], the values the cache
     stands for at the positions of the batch's rows. With kv_len as the lengths of q_start's
     ranges these are whole sequences."""
+    import torch
     fn = _paged_fn("lai_paged_kv_read", dtype)
-    made = [x is None for x in (k, v)]
-    if any(made):  # (one of them alone has the row stride of the other)
-        ld = kv.width if all(made) else _paged_rows(v if k is None else k, kv.width)
-        with _made_on(stream):
-            k = kv.k.new_empty((rows, ld), dtype=dtype)[:, :kv.width] if k is None else k
-            v = kv.k.new_empty((rows, ld), dtype=dtype)[:, :kv.width] if v is None else v
+    made_k, made_v, width = k is None, v is None, kv.width
+    if made_k and made_v:
+        k = _made_on(stream, kv.k.new_empty, (rows, width), dtype=dtype)
+        v = _made_on(stream, torch.empty_like, k)
+    elif made_k:  # with the row stride of the other
+        k = _made_on(stream, kv.k.new_empty, (rows, _paged_rows(v, width)), dtype=dtype)[:, :width]
+    elif made_v:
+        v = _made_on(stream, kv.k.new_empty, (rows, _paged_rows(k, width)), dtype=dtype)[:, :width]
     if k.dtype != dtype or v.dtype != dtype or k.shape[0] != rows or v.shape[0] != rows:
         raise ValueError("k and v must be [rows, n_kv_heads * head_dim] of dtype")
     ld = _paged_rows(k, kv.width)
@@ -599,8 +602,11 @@ def paged_kv_read(kv, batch, rows, dtype, k=None, v=None, err=None, stream=None)
     _need_cuda(kv.index, batch.q_start, k, v, err)
     _paged_call(fn, kv.index, stream, k.data_ptr(), v.data_ptr(), ld, rows, kv._ref, batch._ref,
                 None if err is None else err.data_ptr())
-    if any(made):
-        _handed_out(stream, *(x for x, new in zip((k, v), made) if new))
+    if stream is not None:
+        if made_k:
+            _handed_out(stream, k)
+        if made_v:
+            _handed_out(stream, v)
     return k, v
 
 
@@ -638,13 +644,13 @@ def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, 
         raise ValueError("q must be [rows, n_heads * head_dim], n_heads a multiple of n_kv_heads")
     ld = _paged_rows(q, shape[1])
     made = out is None
-    if made or scratch is None:
-        with _made_on(stream):
-            out = q.new_empty(shape) if made else out
-            scratch = paged_attention_scratch(hd, kv.device) if scratch is None else scratch
-    if not made and (out.dtype != q.dtype or out.shape != shape or not out.is_contiguous()):
+    if made:
+        out = _made_on(stream, q.new_empty, shape)
+    elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and dtype")
-    if scratch.nbytes < 4 * _paged_scratch_floats(hd) or not scratch.is_contiguous():
+    if scratch is None:
+        scratch = _made_on(stream, paged_attention_scratch, hd, kv.device)
+    elif scratch.nbytes < 4 * _paged_scratch_floats(hd) or not scratch.is_contiguous():
         raise ValueError("scratch is too small: use paged_attention_scratch(head_dim)")
     if window < 0:
         raise ValueError("window must not be negative")
@@ -652,7 +658,7 @@ def paged_attention(q, kv, batch, scale=None, window=0, scratch=None, out=None, 
     _paged_call(fn, kv.index, stream, out.data_ptr(), q.data_ptr(), ld, shape[0], shape[1] // hd,
                 kv._ref, batch._ref, hd ** -0.5 if scale is None else scale, min(window, 0x7fffffff),
                 scratch.data_ptr(), None if err is None else err.data_ptr())
-    if made:
+    if made and stream is not None:
         _handed_out(stream, out)
     return out
 
@@ -699,10 +705,9 @@ def decode_attention(q, k_new, v_new, k_cache, v_cache, pos, n_heads, n_kv_heads
     S, max_seq = k_cache.shape[0], k_cache.shape[1]
     hd = q.shape[1] // n_heads
     made = out is None
-    with _made_on(stream):
-        if scratch is None:
-            scratch = decode_attention_scratch(S, n_heads, n_kv_heads, max_seq, q.device)
-        out = torch.empty_like(q) if made else out
+    if scratch is None:
+        scratch = _made_on(stream, decode_attention_scratch, S, n_heads, n_kv_heads, max_seq, q.device)
+    out = _made_on(stream, torch.empty_like, q) if made else out
     sc = hd ** -0.5 if scale is None else scale
     if qk is None:
         call("lai_decode_attention_f32", _p(out), _p(q), _p(k_new), _p(v_new), _p(k_cache),
@@ -714,7 +719,7 @@ def decode_attention(q, k_new, v_new, k_cache, v_cache, pos, n_heads, n_kv_heads
              _p(v_cache), _p(pos), S, n_heads, n_kv_heads, hd, max_seq, sc, _p(wq), _p(wk),
              _p(cos_t), _p(sin_t), 0 if cos_t is None else cos_t.shape[0], eps, _p(scratch),
              _p(err), _s(stream))
-    if made:
+    if made and stream is not None:
         _handed_out(stream, out)
     return out
 

@@ -69,12 +69,9 @@ struct Cfg {
     static constexpr int kRawTile = 128 * HD;
     static constexpr int kLand = kF16 ? kRaw : kStages;  // tiles that copies land in
     // binary16 weights: 2^kLift at the row's maximum, at most 2^14 with kGrow (two tiles) and a value
-    // scale's mantissa, so that small ones are held to 2^-25 of 2^kLift
+    // scale's mantissa, so that small ones are held to 2^-25 of 2^kLift (of 2^(kLift - kSpread), where
+    // the block's largest scale is not that of the row's largest product)
     static constexpr float kLift = !kF16 ? 0.f : QF32 ? 13.f : 5.f;
-    // Of 8 exponentials, those that the FMA pipe takes: with 8-bit caches 2 (2048 tokens over 32768
-    // INT8 keys, 16 heads of 128: 587 us with none, 588 with 1, 524 with 2, 640 with 3), with BF16
-    // ones none (466, 467, 476, 477 us).
-    static constexpr int kPolyOf8 = kF16 ? 2 : 0;
     using S = Sched<R, kU, 3>;
 };
 
@@ -203,24 +200,6 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
-}
-// 2^y for y <= 127, below 2^-126 as 2^-126: n = round(y), and on [-1/2, 1/2] the cubic with the
-// smallest relative error, 7.5e-5 (2^-13.7; the weights are rounded to 2^-9 or 2^-12 after it).
-// It runs on the FMA pipe, where there is room beside the exponential unit (16 a cycle and SM),
-// which bounds the softmax otherwise.
-__device__ __forceinline__ float2 exp2_poly(float2 y) {
-    const float kBig = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
-    const float2 big = make_float2(kBig, kBig), nbig = make_float2(-kBig, -kBig);
-    y = make_float2(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
-    const float2 n = __fadd2_rn(y, big);
-    const float2 r = __fadd2_rn(n, nbig);
-    const float2 f = __fadd2_rn(y, make_float2(-r.x, -r.y));
-    float2 p = __ffma2_rn(make_float2(0.05517167f, 0.05517167f), f, make_float2(0.24261112f, 0.24261112f));
-    p = __ffma2_rn(p, f, make_float2(0.69326099f, 0.69326099f));
-    p = __ffma2_rn(p, f, make_float2(0.99992807f, 0.99992807f));
-    // p is within a factor of 2 of 1: adding n to its exponent cannot pass zero or infinity
-    return make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + __float_as_uint(p.x)),
-                       __uint_as_float((__float_as_uint(n.y) << 23) + __float_as_uint(p.y)));
 }
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
@@ -838,12 +817,9 @@ paged_attn_wide_kernel(void *out, const void *__restrict__ qp, const AttnArgs a,
                                            ? make_float2(__fsub_rn(__fmul_rn(x[i + h].x, c), base),
                                                          __fsub_rn(__fmul_rn(x[i + h].y, c), base))
                                            : __ffma2_rn(x[i + h], c2, nb2);
-                            // (a masked score's weight must be exactly 0, and F32 results exact; scores
-                            // of 2^20 and more are rounded before the subtraction as the maximum was)
-                            if (!QF32 && !decltype(mask)::value && ((i + h) * C::kPolyOf8 & 7) < C::kPolyOf8)
-                                p = exp2_poly(p);
-                            else
-                                p = make_float2(ex2(p.x), ex2(p.y));
+                            // (scores of 2^20 and more are rounded before the subtraction, as the
+                            // maximum was)
+                            p = make_float2(ex2(p.x), ex2(p.y));
                             sum[h] = __fadd2_rn(sum[h], p);
                             if (kF16) p = __fmul2_rn(p, h ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y));
 #pragma unroll

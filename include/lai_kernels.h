@@ -379,13 +379,14 @@ LAI_API int lai_paged_kv_read_f32(float *k, float *v, int64_t ld, int64_t n_rows
  * reaches 2^28, or the batch could have 2^31 blocks of keys and rows: LAI_ERR_RANGE. Keys in a page
  * outside [0, n_pages) count as not seen and set LAI_DEVERR_PAGE. What lies in the cache behind
  * kv_len, or at positions a row does not see, does not reach that row, whatever its bits; an
- * infinity or NaN that it does see makes what it touches an infinity or NaN. Scores, softmax and
- * sums are F32; with F32 q the products are exact to about F32 too (16-bit operands split into
- * terms), with BF16 q the weights of the values may be rounded to BF16 (BF16 cache) or to
- * binary16. Over an 8-bit cache a weight counts with its value's scale: what is below 2^-26 (F32 q)
- * or 2^-18 (BF16 q) of the largest such product among the keys that the row sees may be rounded
- * away. That holds for key scales to 2^90, value scales of 2^-90 to 2^106 and, beside scales
- * outside 2^-14 to 2^14, for scores up to 2^27. The result has the same bits in every call with the same batch, but a row's bits
+ * infinity or NaN that it does see makes what it touches an infinity or NaN (but a score of
+ * -infinity may weigh 0). Scores, softmax and sums are F32; with F32 q the products are exact to
+ * about F32 too (16-bit operands split into terms), with BF16 q the weights of the values may be
+ * rounded to BF16 (BF16 cache) or to binary16. Over an 8-bit cache a weight counts with its value's
+ * scale: what is below 2^-26 (F32 q) or 2^-18 (BF16 q) of the largest such product among the keys
+ * that the row sees may be rounded away. That holds for key scales to 2^90, value scales of 2^-90 to
+ * 2^106 and, beside scales outside 2^-14 to 2^14, for scores up to 2^27. The result has the same
+ * bits in every call with the same batch, but a row's bits, and how much more than this it keeps,
  * depend on the rows it shares a batch with.
  * scratch: lai_paged_attention_scratch_bytes(head_dim) bytes, the first 4096 of them zeroed once
  * before first use; every call leaves it reusable (one that set LAI_DEVERR_TIMEOUT does not: zero

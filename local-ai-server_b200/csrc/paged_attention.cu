@@ -12,14 +12,14 @@
 // chunks (a chunk is what a warp takes at a time) filled with bulk copies, across the ends of
 // items, so the other seven neither compute addresses nor hold loads in registers. (With loads
 // straight into registers 64 x 4096 INT8 keys took 143 us, bound by their latency at the 12 warps
-// that fit; this takes 137 us.)
-//   Measured, 64 sequences of 4096 keys, 16 heads of 128 on 8, one token each: BF16 keys 176 us with
-// F32 q (6.1 TB/s, 0.94 of a copy's bandwidth) and 169 with BF16 q (6.4 TB/s, 0.99), so HBM; E4M3
-// 126 and INT8 137 us (4.4 and 4.0 TB/s): the warps' latency over about 1000 instructions per 32 keys
-// (a third of them conversions to binary16; issue slots 44% used at the 14 warps that registers
+// that fit, when this took 137.)
+//   Measured, 64 sequences of 4096 keys, 16 heads of 128 on 8, one token each: BF16 keys 174 us with
+// F32 q (6.15 TB/s, 0.95 of a copy's bandwidth) and 166 with BF16 q (6.5 TB/s, 1.00), so HBM; E4M3
+// 109 and INT8 121 us (5.1 and 4.6 TB/s): the warps' latency over about 1000 instructions per 32 keys
+// (a third of them conversions to binary16; issue slots 46% used at the 14 warps that registers
 // allow), and the count of copies: 4 per chunk, 101 us on their own. V in 4 blocks apart, so that no
-// banks conflict, took 7 copies and 165 us, in 2 blocks 145; scales by 16-byte copies of the lanes
-// 145. Short calls are latency: one sequence
+// banks conflict, took 7 copies and 165 us, in 2 blocks 145, scales by 16-byte copies of the lanes
+// 145, each when the rest took 137. Short calls are latency: one sequence
 // of 777 keys 10.6 us, of which finding the work 2.5, the first keys through a warp 4.7, leaving
 // parts 1.6, joining them 1.7.
 //   * The sums over head_dim and over keys do not depend on the order of their terms. A lane
@@ -29,7 +29,7 @@
 //     queries become hi + lo in binary16 (22 bits; the 8-bit formats are exact in binary16), or
 //     three bfloat16 terms (24 bits) over a BF16 cache, and so do the weights p. With BF16
 //     queries the second rows still make the weights exact to 16 bits or more. (One term of them
-//     over the 8-bit formats was no faster: the compiler spilt registers, 143 us for 126.)
+//     over the 8-bit formats was no faster: the compiler spilt registers, 143 us when two took 126.)
 //   * Each block's P V starts from zero and is added to the F32 accumulators by the FMA that
 //     rescales them, so a long sequence does not add up the MMA's truncated sums.
 //   * 8-bit: a key's scale multiplies its score, a value's scale its weight. In binary16 these

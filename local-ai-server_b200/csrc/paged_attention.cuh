@@ -126,9 +126,9 @@ struct SeqSmem {
     int32_t q_start[kSeqCache + 1], kv_len[kSeqCache];
 };
 // a with its tables in shared memory (or as it is); flags sequences that are not well formed. Where
-// q_start decreases there is no work at all (n_seqs 0): looking for a slot's sequence from its both
-// ends finds different ones then, and CTAs that disagree on who shares an item leave its counter
-// behind for the next call. The whole CTA; has a barrier.
+// q_start decreases there is no work at all (n_seqs 0): bisection and stepping would find different
+// sequences for a slot then, and CTAs that disagree on who shares an item leave its counter behind
+// for the next call. The whole CTA; has a barrier.
 template <int THREADS>
 __device__ __forceinline__ AttnArgs cache_seqs(const AttnArgs &a, SeqSmem &sm) {
     AttnArgs c = a;

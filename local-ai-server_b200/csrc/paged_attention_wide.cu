@@ -27,9 +27,10 @@
 // Measured, 2048 tokens over 32768 keys, 16 heads of 128 on 8 (0.53 TFLOP of products below the
 // diagonal): BF16 q, BF16 cache 474 us (1.12 PFLOP/s, 0.67 of a large BF16 matrix product's rate),
 // 8-bit 580 to 590 us; F32 q 1575 us (BF16 cache) and 1230 us (8-bit), for three and two times the
-// products of each kind (all of them 5% less on a cool GPU). With BF16 q softmax and MMAs bound it together: a tile's block is 16384 exponentials,
-// 1024 clocks at 16 per SM and clock, and its MMAs take as many; 8-bit caches have room for 3 operand
-// tiles only, so conversions are not far enough ahead of the MMAs (BF16 with 3 tiles: 525 us).
+// products of each kind; runs differ by 5% with the power cap. With BF16 q softmax and MMAs bound it
+// together: a tile's block is 16384 exponentials, 1024 clocks at 16 per SM and clock, and its MMAs take
+// as many; 8-bit caches have room for 3 operand tiles only, so conversions are not far enough ahead of
+// the MMAs (BF16 with 3 tiles: 525 us).
 // Every wait is bounded; a wait that runs out raises LAI_DEVERR_TIMEOUT and ends the kernel.
 #include <cuda.h>
 
